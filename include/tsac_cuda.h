@@ -408,6 +408,180 @@ int tsac_cuda_range_encode_tree(const float* masses, const uint16_t* symbols, si
 int tsac_cuda_range_decode_tree(const uint8_t* bytes, size_t size, const float* masses, size_t count,
                                 uint16_t* symbols);
 
+/* ---- drafted decoding over a paged key/value cache ---------------------
+ * No counterpart in the reference.  For programs that sample or continue
+ * token sequences from a probability model (the codec's own streams keep
+ * tsac_cuda_attention's exact order): several tokens are drafted as a tree,
+ * checked in one step, and the accepted ones kept.  Node 0 of a tree is the
+ * last known token, whose keys and values are not in the cache yet; node n's
+ * parent is a node before it.  All calls are asynchronous on `stream`,
+ * allocate nothing, never read the device from the host, and may be captured
+ * into a CUDA graph.  The device that holds the buffers must be current.
+ * Faults that only the device can see (an invalid sequence, page or position,
+ * a sequence named twice) skip the entry concerned, leave its outputs as they
+ * were, and OR bit 16 into *error_word (nullable); none reads or writes
+ * outside the buffers as long as the counts given here are true.  Two calls
+ * on one cache must not overlap unless both only read it. */
+
+enum tsac_cuda_value_type
+{
+    TSAC_CUDA_BF16 = 0,
+    TSAC_CUDA_FP16 = 1,
+    TSAC_CUDA_FP32 = 2
+};
+
+/* Nodes of one tree, at most. */
+#define TSAC_CUDA_MAX_NODES 64
+/* Sequences named by one call, and sequences of one cache, at most. */
+#define TSAC_CUDA_MAX_LIST 4096
+#define TSAC_CUDA_MAX_SEQUENCES 65536
+
+/* A cache of `sequences` token sequences over one pool of pages.  Position i
+ * of a sequence is slot i % page_size of the page that its table names at
+ * i / page_size, in every layer and for keys and values alike.
+ *   pool     device [layers][2: keys, values][pages][page_size][kv_heads][head_dim]
+ *   tables   device int32 [sequences][max_pages]; entries from counts[s] on are -1
+ *   counts   device int32 [sequences], pages that the sequence holds
+ *   lengths  device int32 [sequences], committed positions
+ *   refs     device int32 [pages], table entries that name the page; 0 = free.
+ * These three tensors are the allocator's whole state: pages are taken lowest
+ * first, so results do not depend on scheduling.  An empty cache has tables
+ * -1 and the rest 0.  type: BF16 or FP16; page_size a power of two up to
+ * 1024; kv_heads * head_dim a multiple of 8, up to 65,536; pool 16-byte
+ * aligned; pages up to 2^24, max_pages up to 2^20. */
+typedef struct tsac_cuda_paged_cache
+{
+    void* pool;
+    int32_t* tables;
+    int32_t* counts;
+    int32_t* lengths;
+    int32_t* refs;
+    size_t layers, pages, page_size, kv_heads, head_dim, sequences, max_pages;
+    int type;
+} tsac_cuda_paged_cache;
+
+/* Makes positions [length, length + positions[i]) of each listed sequence
+ * writable: takes free pages behind the held ones, and gives the sequence its
+ * own copy (all layers) of each page in that range that others hold too.
+ *   sequences  device int32 [count], distinct, or NULL: 0 .. count - 1
+ *   positions  device int32 [count], each >= 0
+ *   slots      pages that one sequence's range can touch, at most
+ *              (max_pages always suffices)
+ *   scratch    device, >= tsac_cuda_cache_reserve_scratch_bytes(count, slots), 16-byte aligned
+ * All or nothing: too few free pages change nothing and OR 8 into
+ * *error_word; an invalid entry (bit 16) changes nothing either. */
+size_t tsac_cuda_cache_reserve_scratch_bytes(size_t count, size_t slots);
+int tsac_cuda_cache_reserve(const tsac_cuda_paged_cache* cache, const int32_t* sequences,
+                            const int32_t* positions, size_t count, size_t slots, void* scratch,
+                            size_t scratch_bytes, unsigned* error_word, void* stream);
+
+/* children[i], which must hold no page, becomes a copy of parents[i] that
+ * shares the pages of its committed positions (device int32 [count] each).
+ * A pair whose child is named twice, or is some pair's parent, is refused. */
+int tsac_cuda_cache_fork(const tsac_cuda_paged_cache* cache, const int32_t* parents,
+                         const int32_t* children, size_t count, unsigned* error_word, void* stream);
+
+/* Gives back the pages behind position positions[i] of each listed sequence
+ * (positions NULL: all pages), and shortens its length to that if it is
+ * longer.  A page becomes free when its last sequence gives it back. */
+int tsac_cuda_cache_release(const tsac_cuda_paged_cache* cache, const int32_t* sequences,
+                            const int32_t* positions, size_t count, unsigned* error_word, void* stream);
+
+/* Stores rows of one layer: row n < nodes[i] of entry i goes to position
+ * start + n, start = starts[i] (starts NULL: the sequence's length).  The
+ * pages must be the sequence's own (tsac_cuda_cache_reserve).
+ *   keys, values  device [count][max_nodes][kv_heads][head_dim] of the cache's
+ *                 type with the given strides in elements (multiples of 8; the
+ *                 last dimension is contiguous), 16-byte aligned
+ *   nodes         device int32 [count] or NULL: max_nodes each
+ * max_nodes may be any length here (a prompt, for instance). */
+int tsac_cuda_cache_append(const tsac_cuda_paged_cache* cache, size_t layer, const void* keys,
+                           const ptrdiff_t key_strides[3], const void* values,
+                           const ptrdiff_t value_strides[3], const int32_t* sequences,
+                           const int32_t* nodes, const int32_t* starts, size_t count,
+                           size_t max_nodes, unsigned* error_word, void* stream);
+
+/* Keeps the accepted rows: in every layer row start + path[i][j] moves to
+ * start + j for j < accepted[i], and the sequence's new length start +
+ * accepted[i] is written to lengths_out [sequences] (the cache's own lengths,
+ * or another buffer that overlaps neither them nor starts; other sequences'
+ * entries are left as they were).
+ *   path  device int32 [count][width], ascending; entries from accepted[i] on
+ *         are not read
+ *   starts device int32 [count] or NULL: the sequences' lengths */
+int tsac_cuda_cache_keep(const tsac_cuda_paged_cache* cache, const int32_t* sequences,
+                         const int32_t* path, const int32_t* accepted, const int32_t* starts,
+                         int32_t* lengths_out, size_t count, size_t width, unsigned* error_word,
+                         void* stream);
+
+/* Moves the pages in use to the lower end of the pool, the fewest that do:
+ * with L pages in use, the k-th used page from L on moves to the k-th free
+ * page below L.  tables_out [sequences][max_pages] and refs_out [pages] may be
+ * the cache's own; *live (device) receives L, so a caller may keep only the
+ * pool's first L pages of each plane.  Pages that moved keep their old bytes. */
+size_t tsac_cuda_cache_compact_scratch_bytes(size_t pages);
+int tsac_cuda_cache_compact(const tsac_cuda_paged_cache* cache, int32_t* tables_out, int32_t* refs_out,
+                            int32_t* live, void* scratch, size_t scratch_bytes,
+                            unsigned* error_word, void* stream);
+
+/* Attention of every node of each listed sequence's tree over the committed
+ * positions and the node's own ancestors, itself included, whose keys and
+ * values lie at positions length + ancestor:
+ *   out = softmax(scale * q k^T) v over those positions, 32-bit softmax and sums.
+ *   parents  device int32 [count][max_nodes]; -1: a root; below -1: the node
+ *            sees no drafted node, not even itself
+ *   nodes    device int32 [count] or NULL: max_nodes each.  Rows of later
+ *            nodes, and of sequences without nodes, are left as they were
+ *   query, out  device [count][max_nodes][heads][head_dim] of the cache's type
+ *            with the given strides in elements (multiples of 8; the last
+ *            dimension is contiguous), 16-byte aligned.  heads is a multiple
+ *            of kv_heads: query head h reads key head h / (heads / kv_heads)
+ *   lse      device f32 [count][max_nodes][heads] or NULL: log of the sum of
+ *            exponentials
+ *   scratch  device, >= tsac_cuda_tree_attention_scratch_bytes(cache, heads,
+ *            max_nodes), 16-byte aligned; calls that overlap need their own
+ * A row that sees nothing gives zeros and -infinity.  A value that is not
+ * finite reaches the rows that see it and no others.  max_nodes 1 is plain
+ * decoding.  head_dim 64 or 128; max_nodes <= TSAC_CUDA_MAX_NODES. */
+size_t tsac_cuda_tree_attention_scratch_bytes(const tsac_cuda_paged_cache* cache, size_t heads,
+                                              size_t max_nodes);
+int tsac_cuda_tree_attention(const tsac_cuda_paged_cache* cache, size_t layer, const int32_t* sequences,
+                             const int32_t* parents, const int32_t* nodes, const void* query,
+                             const ptrdiff_t query_strides[3], void* out, const ptrdiff_t out_strides[3],
+                             float* lse, size_t heads, size_t count, size_t max_nodes, float scale,
+                             void* scratch, size_t scratch_bytes, unsigned* error_word, void* stream);
+
+/* Checks a tree of drafted tokens against the target's probabilities from
+ * given random numbers, so that what is kept has the target's distribution.
+ * From node 0 on, the children of the current node are tried in ascending
+ * order; w is the target's row p there, x the child's token, u its coin:
+ *   draft NULL:  accepted when u * (1 - the rejected siblings' p) < p(x); the
+ *                rejected tokens then leave w
+ *   draft given: accepted when u * q(x) < w(x) with q the draft's row at the
+ *                current node; a rejection makes w = max(w - q, 0) / its sum
+ *                (w stays where that sum is 0)
+ * An accepted child becomes the current node.  Where none is accepted, the
+ * next token is the first whose cumulative w exceeds draw * the sum of w (draft
+ * NULL and nothing left: p itself).  Comparisons and sums are in 64 bits.
+ *   target, draft  device [batch][max_nodes][vocab] of `type`, row n the
+ *            distribution after node n, strides (batch, node) in elements; the
+ *            vocabulary is contiguous
+ *   tokens, parents  device int32 [batch][max_nodes]; node 0's are not read.  A
+ *            token outside the vocabulary has probability 0
+ *   coins    device f32 [batch][max_nodes], draws device f32 [batch], in [0, 1)
+ *   nodes    device int32 [batch] or NULL: max_nodes each
+ *   accepted device int32 [batch]: nodes kept, node 0 included (0 without nodes)
+ *   path     device int32 [batch][max_nodes]: the kept nodes, then -1: what
+ *            tsac_cuda_cache_keep takes
+ *   token    device int32 [batch]: the next token; -1 without nodes, or (bit 1
+ *            of *error_word) where the weights' sum is not a positive finite number */
+int tsac_cuda_draft_verify(const void* target, const ptrdiff_t target_strides[2], const void* draft,
+                           const ptrdiff_t draft_strides[2], int type, const int32_t* tokens,
+                           const int32_t* parents, const float* coins, const float* draws,
+                           const int32_t* nodes, size_t batch, size_t max_nodes, size_t vocab,
+                           int32_t* accepted, int32_t* path, int32_t* token, unsigned* error_word,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif

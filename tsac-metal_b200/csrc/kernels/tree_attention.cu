@@ -1,0 +1,624 @@
+// Attention of trees of drafted tokens over a paged key/value cache, for few
+// query rows per key head.
+//
+//   o = sum_k p_k v_k / sum_k p_k,  p_k = exp2(z_k - max z),  z = q.k scale log2(e)
+// over the committed positions and the row's own ancestors.  One pass: each
+// warp keeps a running maximum, sum and output of its rows over its share of
+// the keys, and the shares are joined at the end (warps in shared memory, CTAs
+// in a second small launch).  Sums and outputs are 32-bit; p is rounded to the
+// input type for the second product, as its operand must be.
+//
+// Bound: the keys and values cross HBM once per key head, M / 2 multiply-adds
+// per byte for M query rows; up to 32 rows that is below what mma.sync
+// sustains, so the layout is chosen for bytes in flight: each warp streams its
+// own 16 keys of a 64-key tile through a private three-stage ring (16-byte
+// asynchronous copies, any page size), so no barrier couples the warps before
+// the end of an item, and two CTAs of four warps keep up to 128 KiB in flight
+// per SM.
+#include "kernels/launch_count.hpp"
+#include "kernels/pdl.cuh"
+#include "kernels/tree_attention.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <mutex>
+
+namespace tsacb::dev
+{
+namespace
+{
+constexpr int WARPS = 4, THREADS = WARPS * 32, STAGES = 3, WARP_KEYS = 16, KEYS = WARPS * WARP_KEYS;
+
+template <class T> struct Half2;
+template <> struct Half2<__nv_bfloat16>
+{
+    static __device__ __forceinline__ std::uint32_t pack(float lo, float hi)
+    {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const std::uint32_t*>(&v);
+    }
+    static __device__ __forceinline__ std::uint16_t one(float x)
+    {
+        return __bfloat16_as_ushort(__float2bfloat16_rn(x));
+    }
+    static __device__ __forceinline__ float value(std::uint16_t x)
+    {
+        return __bfloat162float(__ushort_as_bfloat16(x));
+    }
+    static constexpr std::uint32_t exponents = 0x7f807f80u;
+    static __device__ __forceinline__ void mma(float (&d)[4], const std::uint32_t (&a)[4], std::uint32_t b0,
+                                               std::uint32_t b1)
+    {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9},"
+                     " {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+template <> struct Half2<__half>
+{
+    static __device__ __forceinline__ std::uint32_t pack(float lo, float hi)
+    {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const std::uint32_t*>(&v);
+    }
+    static __device__ __forceinline__ std::uint16_t one(float x) { return __half_as_ushort(__float2half_rn(x)); }
+    static __device__ __forceinline__ float value(std::uint16_t x) { return __half2float(__ushort_as_half(x)); }
+    static constexpr std::uint32_t exponents = 0x7c007c00u;
+    static __device__ __forceinline__ void mma(float (&d)[4], const std::uint32_t (&a)[4], std::uint32_t b0,
+                                               std::uint32_t b1)
+    {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9},"
+                     " {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+
+__device__ __forceinline__ void load_matrices(std::uint32_t address, std::uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(address)
+                 : "memory");
+}
+__device__ __forceinline__ void load_matrices_transposed(std::uint32_t address, std::uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(address)
+                 : "memory");
+}
+// 16-byte copy, or 16 zero bytes when `bytes` is 0.
+__device__ __forceinline__ void copy_16(std::uint32_t to, const void* from, unsigned bytes)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ float power_of_two(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Bit a of masks[n]: node a is node n or one of its ancestors.  Pointer
+// doubling: log2(64) rounds in place of a walk of up to 64 dependent steps.
+// A parent below -1 makes a node that sees no drafted node, not even itself;
+// one that is not before its child is reported and treated as such.
+__device__ __forceinline__ void ancestor_masks(const int* parents, int nodes, unsigned long long* masks, int* above,
+                                               unsigned* error_word, int t, int threads)
+{
+    for (int n = t; n < DRAFT_MAX_NODES; n += threads)
+    {
+        const int parent = n < nodes ? parents[n] : -2;
+        const bool wrong = parent >= n;
+        if (wrong && n < nodes && error_word)
+            atomicOr(error_word, error_cache);
+        masks[n] = parent < -1 || wrong ? 0ull : 1ull << n;
+        above[n] = wrong || parent < 0 ? -1 : parent;
+    }
+    __syncthreads();
+    for (int round = 0; round < 6; ++round)
+    {
+        unsigned long long mask[(DRAFT_MAX_NODES + 31) / 32];
+        int next[(DRAFT_MAX_NODES + 31) / 32];
+        int k = 0;
+        for (int n = t; n < DRAFT_MAX_NODES; n += threads, ++k)
+        {
+            const int up = above[n];
+            mask[k] = up >= 0 ? masks[up] : 0ull;
+            next[k] = up >= 0 ? above[up] : -1;
+        }
+        __syncthreads();
+        k = 0;
+        for (int n = t; n < DRAFT_MAX_NODES; n += threads, ++k)
+        {
+            masks[n] |= mask[k];
+            above[n] = next[k];
+        }
+        __syncthreads();
+    }
+}
+
+template <int D, int MT> struct Layout
+{
+    static constexpr int ROWS = 16 * MT;
+    static constexpr int row_bytes = 2 * D, chunks = D / 8;
+    static constexpr int stage_bytes = 2 * WARP_KEYS * row_bytes; // keys, then values
+    static constexpr int ring_bytes = WARPS * STAGES * stage_bytes;
+    static constexpr int merge_bytes = WARPS * ROWS * D * 4;
+    static constexpr int smem = ring_bytes > merge_bytes ? ring_bytes : merge_bytes;
+};
+
+template <class T, int D, int MT>
+__global__ void __launch_bounds__(THREADS, 2)
+    tree_attention_kernel(const TreeArgs a, float* pieces, TreeShared* shared_items)
+{
+    pdl_prologue();
+    using L = Layout<D, MT>;
+    using Work = TreeWork<KEYS, L::ROWS>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ unsigned long long masks[DRAFT_MAX_NODES];
+    __shared__ int above[DRAFT_MAX_NODES];
+    __shared__ long long warp_sums[WARPS];
+    __shared__ typename Work::Start found;
+    __shared__ float row_max[WARPS][L::ROWS], row_sum[WARPS][L::ROWS];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int cta = blockIdx.x;
+    const auto start = Work::template find<THREADS>(a, cta, gridDim.x, warp_sums, &found);
+    if (t == 0)
+        shared_items[cta].pieces = 0;
+    if (cta >= start.ctas)
+        return;
+    long long unit = Work::first_unit(start.units, cta, start.ctas);
+    const long long last_unit = Work::first_unit(start.units, cta + 1, start.ctas);
+    const std::uint32_t ring = static_cast<std::uint32_t>(__cvta_generic_to_shared(smem)) + warp * STAGES * L::stage_bytes;
+    const unsigned char* plane = a.cache.pool + 2ll * a.layer * a.cache.plane_bytes;
+
+    int list_entry = start.entry;
+    long long before = start.before;
+    while (unit < last_unit)
+    {
+        const auto e = Work::entry(a, list_entry);
+        if (unit >= before + e.units)
+        {
+            before += e.units;
+            ++list_entry;
+            continue;
+        }
+        const int item = static_cast<int>((unit - before) / e.tiles);
+        const int head = item / e.row_items, first_row = (item - head * e.row_items) * L::ROWS;
+        const long long item_start = before + static_cast<long long>(item) * e.tiles;
+        const int tile_begin = static_cast<int>(unit - item_start);
+        const int tile_end = static_cast<int>(min(static_cast<long long>(e.tiles), last_unit - item_start));
+        const int rows = e.nodes * a.group;
+        if (tile_end == e.tiles)
+            ancestor_masks(a.parents + static_cast<long long>(list_entry) * a.max_nodes, e.nodes, masks, above,
+                           a.error_word, t, THREADS);
+
+        // Query fragments: row lane / 4 (+ 8), columns 2 (lane % 4) (+ 8) of each 16.
+        std::uint32_t q[MT][D / 16][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+            {
+                const int row = first_row + 16 * m + 8 * r + (lane >> 2);
+                const int node = row / a.group, in_group = row - node * a.group;
+                const std::uint16_t* from = a.query + list_entry * a.query_batch + node * a.query_node +
+                                            (head * a.group + in_group) * a.query_head + 2 * (lane & 3);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                {
+                    q[m][k][r] = row < rows ? *reinterpret_cast<const std::uint32_t*>(from + 16 * k) : 0u;
+                    q[m][k][r + 2] = row < rows ? *reinterpret_cast<const std::uint32_t*>(from + 16 * k + 8) : 0u;
+                }
+            }
+        float o[MT][D / 8][4] = {};
+        float top[MT][2], sum[MT][2];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+        {
+            top[m][0] = top[m][1] = -INFINITY;
+            sum[m][0] = sum[m][1] = 0.0f;
+        }
+
+        // Byte offset of this lane's key row (lane % 16 of the warp's 16) in a tile; -1: no such key.
+        const auto key_row = [&](int tile) -> long long
+        {
+            if (tile >= tile_end)
+                return -1;
+            const bool drafted = tile == e.tiles - 1;
+            const int in_tile = warp * WARP_KEYS + (lane & 15);
+            const int position = drafted ? e.length + in_tile : tile * KEYS + in_tile;
+            if (drafted ? in_tile >= e.nodes : position >= e.length)
+                return -1;
+            const int page = cache_page(a.cache, e.sequence, e.held, position >> a.cache.page_shift);
+            if (page < 0)
+            {
+                if (a.error_word)
+                    atomicOr(a.error_word, error_cache);
+                return -1;
+            }
+            return page * a.cache.page_bytes() +
+                   static_cast<long long>(position & (a.cache.page_size() - 1)) * a.cache.row_bytes + head * L::row_bytes;
+        };
+        // Rows of L::chunks 16-byte chunks, chunk c of row r at place c ^ (r & 7): conflict-free for ldmatrix.
+        const auto fetch = [&](int stage, long long row_offset)
+        {
+            constexpr int rows_at_once = 32 / L::chunks;
+            const std::uint32_t base = ring + stage * L::stage_bytes;
+#pragma unroll
+            for (int i = 0; i < WARP_KEYS / rows_at_once; ++i)
+            {
+                const int row = i * rows_at_once + lane / L::chunks, chunk = lane % L::chunks;
+                const long long offset = __shfl_sync(0xffffffffu, row_offset, row);
+                const unsigned bytes = offset >= 0 ? 16u : 0u;
+                const unsigned char* from = plane + (offset >= 0 ? offset + 16 * chunk : 0);
+                const std::uint32_t to = base + row * L::row_bytes + ((chunk ^ (row & 7)) << 4);
+                copy_16(to, from, bytes);
+                copy_16(to + WARP_KEYS * L::row_bytes, from + a.cache.plane_bytes, bytes);
+            }
+        };
+        __syncwarp();
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s)
+        {
+            fetch(s, key_row(tile_begin + s));
+            copies_commit();
+        }
+        long long next_row = key_row(tile_begin + STAGES - 1);
+        int stage = 0;
+        for (int tile = tile_begin; tile < tile_end; ++tile)
+        {
+            // The stage refilled here was consumed in the previous step by this warp alone.
+            fetch(stage == 0 ? STAGES - 1 : stage - 1, next_row);
+            copies_commit();
+            next_row = key_row(tile + STAGES);
+            copies_wait<STAGES - 1>();
+            __syncwarp();
+            const std::uint32_t keys = ring + stage * L::stage_bytes, values = keys + WARP_KEYS * L::row_bytes;
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+
+            float s[MT][2][4] = {};
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+            {
+                // Matrices: keys 0-7 and 8-15 by the two halves of the 16 columns.
+                const int row = (lane & 7) + ((lane >> 4) << 3), chunk = 2 * k + ((lane >> 3) & 1);
+                std::uint32_t b[4];
+                load_matrices(keys + row * L::row_bytes + ((chunk ^ (row & 7)) << 4), b);
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                {
+                    Half2<T>::mma(s[m][0], q[m][k], b[0], b[1]);
+                    Half2<T>::mma(s[m][1], q[m][k], b[2], b[3]);
+                }
+            }
+            const bool drafted = tile == e.tiles - 1;
+            const int in_tile = warp * WARP_KEYS + 2 * (lane & 3); // this lane's first key
+            const int held = drafted ? e.nodes : e.length - tile * KEYS;
+            unsigned tainted = 0; // drafted rows with a value that is not finite
+            if (drafted && warp * WARP_KEYS < e.nodes)
+            {
+                for (int row = 0; row < WARP_KEYS; ++row)
+                {
+                    bool odd = false;
+                    if (lane < L::chunks)
+                    {
+                        const uint4 v = *reinterpret_cast<const uint4*>(
+                            smem + (values - static_cast<std::uint32_t>(__cvta_generic_to_shared(smem))) +
+                            row * L::row_bytes + (lane << 4));
+                        const std::uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int w = 0; w < 4; ++w)
+                        {
+                            const std::uint32_t x = words[w] & Half2<T>::exponents;
+                            odd |= (x & 0xffffu) == (Half2<T>::exponents & 0xffffu) ||
+                                   (x >> 16) == (Half2<T>::exponents >> 16);
+                        }
+                    }
+                    tainted |= __any_sync(0xffffffffu, odd) ? 1u << row : 0u;
+                }
+            }
+            std::uint32_t p[MT][4];
+            float exact_p[MT][2][4];
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                {
+                    unsigned long long sees = ~0ull;
+                    if (drafted)
+                    {
+                        const int row = first_row + 16 * m + 8 * r + (lane >> 2);
+                        sees = row < rows ? masks[row / a.group] : 0ull;
+                    }
+                    float z[4], best = top[m][r];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) // keys in_tile, + 1, + 8, + 9
+                    {
+                        const int key = in_tile + (k & 1) + 8 * (k >> 1);
+                        z[k] = s[m][k >> 1][2 * r + (k & 1)] * a.scale_log2;
+                        if (key >= held || !(sees >> key & 1ull))
+                            z[k] = -INFINITY;
+                        best = fmaxf(best, z[k]);
+                    }
+                    best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
+                    best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
+                    const float shift = best == -INFINITY ? 0.0f : best; // rows that have seen nothing yet
+                    const float scale = power_of_two(top[m][r] - shift);
+                    top[m][r] = best;
+                    float partial = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                    {
+                        z[k] = power_of_two(z[k] - shift);
+                        partial += z[k];
+                        exact_p[m][r][k] = z[k];
+                    }
+                    sum[m][r] = fmaf(sum[m][r], scale, partial);
+                    p[m][r] = Half2<T>::pack(z[0], z[1]);
+                    p[m][r + 2] = Half2<T>::pack(z[2], z[3]);
+                    if (__any_sync(0xffffffffu, scale != 1.0f))
+                    {
+#pragma unroll
+                        for (int n = 0; n < D / 8; ++n)
+                        {
+                            o[m][n][2 * r] *= scale;
+                            o[m][n][2 * r + 1] *= scale;
+                        }
+                    }
+                }
+            if (tainted)
+            {
+                // 0 x NaN would reach rows that do not see the node: take such
+                // rows out of the product and add them where they are seen.
+                const auto base = values - static_cast<std::uint32_t>(__cvta_generic_to_shared(smem));
+                for (int key = 0; key < WARP_KEYS; ++key)
+                {
+                    if (!(tainted >> key & 1u))
+                        continue;
+                    const int k = (key & 1) + 2 * (key >> 3), from = (lane & ~3) | ((key & 7) >> 1);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+                        {
+                            const int row = first_row + 16 * m + 8 * r + (lane >> 2);
+                            const bool seen = row < rows && (masks[row / a.group] >> (warp * WARP_KEYS + key) & 1ull);
+                            float weight = 0.0f;
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk)
+                            {
+                                const float w = __shfl_sync(0xffffffffu, exact_p[m][r][kk], from);
+                                weight = kk == k ? w : weight;
+                            }
+#pragma unroll
+                            for (int n = 0; n < D / 8; ++n)
+                            {
+                                const std::uint32_t v = *reinterpret_cast<const std::uint32_t*>(
+                                    smem + base + key * L::row_bytes + ((n ^ (key & 7)) << 4) + 4 * (lane & 3));
+                                if (seen)
+                                {
+                                    o[m][n][2 * r] = fmaf(weight, Half2<T>::value(v & 0xffffu), o[m][n][2 * r]);
+                                    o[m][n][2 * r + 1] = fmaf(weight, Half2<T>::value(v >> 16), o[m][n][2 * r + 1]);
+                                }
+                            }
+                        }
+                }
+                __syncwarp();
+                for (int key = 0; key < WARP_KEYS; ++key)
+                    if ((tainted >> key & 1u) && lane < L::chunks)
+                        *reinterpret_cast<uint4*>(smem + base + key * L::row_bytes + (lane << 4)) = make_uint4(0, 0, 0, 0);
+                __syncwarp();
+            }
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n)
+            {
+                // Matrices: keys 0-7 and 8-15 by the two halves of 16 output columns.
+                const int row = (lane & 7) + (((lane >> 3) & 1) << 3), chunk = 2 * n + (lane >> 4);
+                std::uint32_t b[4];
+                load_matrices_transposed(values + row * L::row_bytes + ((chunk ^ (row & 7)) << 4), b);
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                {
+                    Half2<T>::mma(o[m][2 * n], p[m], b[0], b[1]);
+                    Half2<T>::mma(o[m][2 * n + 1], p[m], b[2], b[3]);
+                }
+            }
+            __syncwarp(); // the stage may be refilled
+        }
+        copies_wait<0>();
+        // Join the warps: common maximum, scaled outputs through shared memory.
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+            {
+                sum[m][r] += __shfl_xor_sync(0xffffffffu, sum[m][r], 1);
+                sum[m][r] += __shfl_xor_sync(0xffffffffu, sum[m][r], 2);
+                if ((lane & 3) == 0)
+                {
+                    row_max[warp][16 * m + 8 * r + (lane >> 2)] = top[m][r];
+                    row_sum[warp][16 * m + 8 * r + (lane >> 2)] = sum[m][r];
+                }
+            }
+        __syncthreads();
+        float* merge = reinterpret_cast<float*>(smem);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+            {
+                const int row = 16 * m + 8 * r + (lane >> 2);
+                float best = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w)
+                    best = fmaxf(best, row_max[w][row]);
+                const float scale = best == -INFINITY ? 0.0f : power_of_two(top[m][r] - best);
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n)
+                    *reinterpret_cast<float2*>(merge + (warp * L::ROWS + row) * D + 8 * n + 2 * (lane & 3)) =
+                        make_float2(o[m][n][2 * r] * scale, o[m][n][2 * r + 1] * scale);
+            }
+        __syncthreads();
+        const bool whole = tile_begin == 0 && tile_end == e.tiles;
+        // A piece that begins its item goes to the CTA's second place, any other to its first.
+        float* piece = pieces + (2ll * cta + (tile_begin == 0)) * tree_piece_floats(L::ROWS, D);
+        for (int at = t; at < L::ROWS * (D / 4); at += THREADS)
+        {
+            const int row = at / (D / 4), column = 4 * (at - row * (D / 4));
+            if (first_row + row >= rows)
+                continue;
+            float best = -INFINITY, total = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w)
+                best = fmaxf(best, row_max[w][row]);
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w)
+            {
+                total += best == -INFINITY ? 0.0f : row_sum[w][row] * power_of_two(row_max[w][row] - best);
+                const float4 x = *reinterpret_cast<const float4*>(merge + (w * L::ROWS + row) * D + column);
+                v.x += x.x;
+                v.y += x.y;
+                v.z += x.z;
+                v.w += x.w;
+            }
+            if (!whole)
+            {
+                float* to = piece + row * (D + TREE_PIECE_HEAD);
+                *reinterpret_cast<float4*>(to + TREE_PIECE_HEAD + column) = v;
+                if (column == 0)
+                {
+                    to[0] = best;
+                    to[1] = total;
+                }
+                continue;
+            }
+            const int node = (first_row + row) / a.group, in_group = first_row + row - node * a.group;
+            const float inverse = total == 0.0f ? 0.0f : 1.0f / total; // a row that sees nothing gives zeros
+            std::uint16_t* to = a.out + list_entry * a.out_batch + node * a.out_node +
+                                (head * a.group + in_group) * a.out_head + column;
+            *reinterpret_cast<uint2*>(to) =
+                make_uint2(Half2<T>::pack(v.x * inverse, v.y * inverse), Half2<T>::pack(v.z * inverse, v.w * inverse));
+            if (a.lse && column == 0)
+                a.lse[(static_cast<long long>(list_entry) * a.max_nodes + node) * a.heads * a.group + head * a.group +
+                      in_group] = total == 0.0f ? -INFINITY : (best + log2f(total)) * 0.6931471805599453f;
+        }
+        if (tile_begin == 0 && !whole && t == 0)
+            shared_items[cta] = TreeShared{list_entry, head, first_row,
+                                           Work::owner(start.units, item_start + e.tiles - 1, start.ctas) - cta + 1, e.nodes};
+        unit = item_start + tile_end;
+        __syncthreads(); // the ring and the row statistics are free again
+    }
+}
+
+// Joins the pieces of an item that several CTAs share, in CTA order: one warp
+// per row.  Piece 0 is in the first CTA's second place, the others in their
+// CTAs' first places.
+template <class T, int D>
+__global__ void __launch_bounds__(128)
+    tree_combine_kernel(const TreeArgs a, int rows_per_item, const float* pieces,
+                        const TreeShared* shared_items)
+{
+    pdl_prologue();
+    const int cta = blockIdx.x, lane = threadIdx.x & 31;
+    const TreeShared item = shared_items[cta];
+    const int row = blockIdx.y * 4 + (threadIdx.x >> 5);
+    if (item.pieces == 0 || row >= rows_per_item || item.first_row + row >= item.nodes * a.group)
+        return;
+    const long long stride = 2 * tree_piece_floats(rows_per_item, D);
+    const auto piece = [&](int k)
+    { return pieces + (cta + k) * stride + (k == 0 ? stride / 2 : 0) + row * (D + TREE_PIECE_HEAD); };
+    float best = -INFINITY;
+    for (int k = lane; k < item.pieces; k += 32)
+        best = fmaxf(best, piece(k)[0]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1)
+        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
+    constexpr int PER = D / 32;
+    float v[PER] = {}, total = 0.0f;
+    if (best != -INFINITY)
+    {
+#pragma unroll 4
+        for (int k = 0; k < item.pieces; ++k)
+        {
+            const float* from = piece(k);
+            const float scale = power_of_two(from[0] - best);
+            total = fmaf(from[1], scale, total);
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                v[j] = fmaf(from[TREE_PIECE_HEAD + lane * PER + j], scale, v[j]);
+        }
+    }
+    const int node = (item.first_row + row) / a.group, in_group = item.first_row + row - node * a.group;
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    std::uint16_t* to = a.out + item.entry * a.out_batch + node * a.out_node + (item.head * a.group + in_group) * a.out_head;
+#pragma unroll
+    for (int j = 0; j < PER; j += 2)
+        *reinterpret_cast<std::uint32_t*>(to + lane * PER + j) = Half2<T>::pack(v[j] * inverse, v[j + 1] * inverse);
+    if (a.lse && lane == 0)
+        a.lse[(static_cast<long long>(item.entry) * a.max_nodes + node) * a.heads * a.group + item.head * a.group + in_group] =
+            total == 0.0f ? -INFINITY : (best + log2f(total)) * 0.6931471805599453f;
+}
+
+int grid_ctas()
+{
+    int device = 0, sms = 148;
+    if (cudaGetDevice(&device) == cudaSuccess)
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    return 2 * sms;
+}
+
+size_t scratch_bytes(int ctas, int rows, int head_dim)
+{
+    return static_cast<size_t>(ctas) * (2 * sizeof(float) * static_cast<size_t>(tree_piece_floats(rows, head_dim)) +
+                                        sizeof(TreeShared));
+}
+
+template <class T, int D, int MT> cudaError_t launch(const TreeArgs& a, void* scratch, cudaStream_t stream)
+{
+    using L = Layout<D, MT>;
+    static std::once_flag once[64];
+    int device = 0;
+    cudaGetDevice(&device);
+    if (device >= 0 && device < 64)
+        std::call_once(once[device],
+                       []
+                       {
+                           cudaFuncSetAttribute(tree_attention_kernel<T, D, MT>,
+                                                cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem);
+                       });
+    const int ctas = grid_ctas();
+    auto* pieces = static_cast<float*>(scratch);
+    auto* items = reinterpret_cast<TreeShared*>(pieces + 2ll * ctas * tree_piece_floats(L::ROWS, D));
+    launch_pdl(tree_attention_kernel<T, D, MT>, dim3(ctas), dim3(THREADS), L::smem, stream, a, pieces, items);
+    note_launch();
+    launch_pdl(tree_combine_kernel<T, D>, dim3(ctas, (L::ROWS + 3) / 4), dim3(128), 0, stream, a, L::ROWS,
+               static_cast<const float*>(pieces), static_cast<const TreeShared*>(items));
+    note_launch();
+    return cudaGetLastError();
+}
+
+template <class T> cudaError_t launch_type(const TreeArgs& a, void* scratch, cudaStream_t stream)
+{
+    return a.head_dim == 64 ? launch<T, 64, 1>(a, scratch, stream) : launch<T, 128, 1>(a, scratch, stream);
+}
+} // namespace
+
+size_t tree_attention_scratch(int head_dim)
+{
+    return scratch_bytes(grid_ctas(), 16, head_dim);
+}
+
+cudaError_t tree_attention(const TreeArgs& a, ValueType type, void* scratch, cudaStream_t stream)
+{
+    return type == ValueType::bf16 ? launch_type<__nv_bfloat16>(a, scratch, stream)
+                                   : launch_type<__half>(a, scratch, stream);
+}
+} // namespace tsacb::dev

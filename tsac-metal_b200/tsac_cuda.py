@@ -137,6 +137,261 @@ def qlinear(weights, scales, bias, x, y, scratch, residual=None, error_word=None
         ctypes.c_size_t(scratch.numel() * scratch.element_size()), _dev(error_word), _stream()))
 
 
+# ------------------------------------------------------- drafted decoding --
+# Paged key/value cache, tree attention and draft verification
+# (include/tsac_cuda.h states each operation).  Arguments are torch CUDA
+# tensors; calls are asynchronous on the current stream of the tensors' device
+# and may be captured into a CUDA graph.  Temporary device memory comes from
+# torch's allocator in each call, so overlapping calls and graphs share none.
+MAX_NODES = 64
+
+
+class _PagedCacheStruct(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("pool", "tables", "counts", "lengths", "refs")] + \
+               [(n, ctypes.c_size_t) for n in ("layers", "pages", "page_size", "kv_heads", "head_dim",
+                                               "sequences", "max_pages")] + [("type", ctypes.c_int)]
+
+
+_p, _n, _i = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int
+_DRAFTING = {
+    "tsac_cuda_cache_reserve_scratch_bytes": (_n, [_n, _n]),
+    "tsac_cuda_cache_reserve": (_i, [_p, _p, _p, _n, _n, _p, _n, _p, _p]),
+    "tsac_cuda_cache_fork": (_i, [_p, _p, _p, _n, _p, _p]),
+    "tsac_cuda_cache_release": (_i, [_p, _p, _p, _n, _p, _p]),
+    "tsac_cuda_cache_append": (_i, [_p, _n, _p, _p, _p, _p, _p, _p, _p, _n, _n, _p, _p]),
+    "tsac_cuda_cache_keep": (_i, [_p, _p, _p, _p, _p, _p, _n, _n, _p, _p]),
+    "tsac_cuda_cache_compact_scratch_bytes": (_n, [_n]),
+    "tsac_cuda_cache_compact": (_i, [_p, _p, _p, _p, _p, _n, _p, _p]),
+    "tsac_cuda_tree_attention_scratch_bytes": (_n, [_p, _n, _n]),
+    "tsac_cuda_tree_attention": (_i, [_p, _n, _p, _p, _p, _p, _p, _p, _p, _p, _n, _n, _n, ctypes.c_float,
+                                      _p, _n, _p, _p]),
+    "tsac_cuda_draft_verify": (_i, [_p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _n, _n, _n, _p, _p, _p, _p, _p]),
+}
+_drafting_lib = None
+
+
+def _drafting():
+    """The library with the argument types of the drafting calls declared, once."""
+    global _drafting_lib
+    if _drafting_lib is None:
+        lib = library()
+        for name, (restype, argtypes) in _DRAFTING.items():
+            fn = getattr(lib, name)
+            fn.restype, fn.argtypes = restype, argtypes
+        _drafting_lib = lib
+    return _drafting_lib
+
+
+class _Device:
+    """Makes a tensor's device current for a call, and gives its current stream."""
+
+    def __init__(self, device):
+        import torch
+        self._torch, self.index = torch, device.index
+
+    def stream(self) -> int:
+        return self._torch.cuda.current_stream(self.index).cuda_stream
+
+    def call(self, fn, *arguments) -> None:
+        cuda = self._torch.cuda
+        if cuda.current_device() == self.index:
+            status = fn(*arguments)
+        else:
+            with cuda.device(self.index):
+                status = fn(*arguments)
+        if status != OK:
+            check(status)
+
+
+def _whole(t, name, dtype, device, shape=None):
+    """Address of a contiguous tensor of the given kind; None gives a null pointer."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.device != device or not t.is_contiguous() or (shape is not None and t.shape != shape):
+        raise TsacError(f"{name} must be a contiguous {dtype} tensor on {device}"
+                        + (f" of shape {tuple(shape)}" if shape is not None else ""))
+    return t.data_ptr()
+
+
+def _rows(t, name, dtype, device, shape):
+    """Address and strides of a [entry][node][head][dim] tensor with a contiguous last dimension."""
+    if t.dtype != dtype or t.device != device or t.shape != shape or (shape[-1] > 1 and t.stride(3) != 1):
+        raise TsacError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on {device}, its last dimension contiguous")
+    # A dimension of size one is never stepped over: its stride says nothing.
+    return t.data_ptr(), (ctypes.c_ssize_t * 3)(*[t.stride(k) if shape[k] > 1 else 0 for k in range(3)])
+
+
+class PagedCache:
+    """Token sequences over one pool of key/value pages (tsac_cuda_paged_cache).
+
+    pool: [layers][2: keys, values][pages][page_size][kv_heads][head_dim], bf16
+    or fp16; tables int32 [sequences][max_pages]; counts, lengths int32
+    [sequences]; refs int32 [pages].  The tensors stay the caller's: reading,
+    saving or replacing their contents between calls is fine.
+    """
+
+    def __init__(self, pool, tables, counts, lengths, refs):
+        import torch
+        if pool.dim() != 6 or pool.shape[1] != 2 or not pool.is_cuda or pool.dtype not in (torch.bfloat16, torch.float16):
+            raise TsacError("pool must be a bf16 or fp16 CUDA tensor [layers][2][pages][page_size][kv_heads][head_dim]")
+        self.pool, self.tables, self.counts, self.lengths, self.refs = pool, tables, counts, lengths, refs
+        self.device, self.dtype = pool.device, pool.dtype
+        self._torch, self._int = torch, torch.int32
+        if tables.dim() != 2:
+            raise TsacError("tables must be [sequences][max_pages]")
+        self.layers, _, self.pages, self.page_size, self.kv_heads, self.head_dim = pool.shape
+        self.sequences, self.max_pages = tables.shape
+        s = _PagedCacheStruct()
+        s.pool = _whole(pool, "pool", pool.dtype, self.device)
+        s.tables = _whole(tables, "tables", self._int, self.device)
+        s.counts = _whole(counts, "counts", self._int, self.device, (self.sequences,))
+        s.lengths = _whole(lengths, "lengths", self._int, self.device, (self.sequences,))
+        s.refs = _whole(refs, "refs", self._int, self.device, (self.pages,))
+        for name in ("layers", "pages", "page_size", "kv_heads", "head_dim", "sequences", "max_pages"):
+            setattr(s, name, getattr(self, name))
+        s.type = 0 if pool.dtype == torch.bfloat16 else 1
+        self._struct, self._lib, self._on = s, _drafting(), _Device(self.device)
+        self._cache = ctypes.addressof(s)
+
+    @classmethod
+    def empty(cls, layers, pages, page_size, kv_heads, head_dim, sequences, max_pages, dtype=None, device="cuda"):
+        """A cache whose sequences hold nothing."""
+        import torch
+        ints = dict(dtype=torch.int32, device=device)
+        return cls(torch.zeros((layers, 2, pages, page_size, kv_heads, head_dim), dtype=dtype or torch.bfloat16, device=device),
+                   torch.full((sequences, max_pages), -1, **ints), torch.zeros(sequences, **ints),
+                   torch.zeros(sequences, **ints), torch.zeros(pages, **ints))
+
+    def _list(self, sequences, count):
+        return _whole(sequences, "sequences", self._int, self.device, (count,))
+
+    def _word(self, error_word):
+        if error_word is None:
+            return None
+        if error_word.numel() < 1 or error_word.element_size() != 4:
+            raise TsacError("error_word must hold a 32-bit word")
+        return _whole(error_word, "error_word", error_word.dtype, self.device)
+
+    def _scratch(self, nbytes):
+        return self._torch.empty(max(nbytes, 16), dtype=self._torch.uint8, device=self.device)
+
+    def reserve(self, positions, sequences=None, slots=None, error_word=None):
+        """Makes positions[i] further positions of each sequence writable (all or nothing)."""
+        count = positions.shape[0]
+        slots = slots or self.max_pages
+        nbytes = self._lib.tsac_cuda_cache_reserve_scratch_bytes(count, slots)
+        scratch = self._scratch(nbytes)
+        self._on.call(self._lib.tsac_cuda_cache_reserve, self._cache, self._list(sequences, count),
+                      _whole(positions, "positions", self._int, self.device, (count,)), count, slots,
+                      scratch.data_ptr(), scratch.numel(), self._word(error_word), self._on.stream())
+
+    def fork(self, parents, children, error_word=None):
+        """children[i], empty so far, shares the committed pages of parents[i]."""
+        count = parents.shape[0]
+        self._on.call(self._lib.tsac_cuda_cache_fork, self._cache,
+                      _whole(parents, "parents", self._int, self.device, (count,)),
+                      _whole(children, "children", self._int, self.device, (count,)), count,
+                      self._word(error_word), self._on.stream())
+
+    def release(self, sequences=None, positions=None, error_word=None):
+        """Gives back the pages behind positions[i] (None: all) of each sequence."""
+        count = sequences.shape[0] if sequences is not None else self.sequences
+        self._on.call(self._lib.tsac_cuda_cache_release, self._cache, self._list(sequences, count),
+                      _whole(positions, "positions", self._int, self.device, (count,)), count,
+                      self._word(error_word), self._on.stream())
+
+    def append(self, layer, keys, values, nodes=None, sequences=None, starts=None, error_word=None):
+        """Stores [entry][node][kv_heads][head_dim] rows of one layer behind each sequence's length (or at starts)."""
+        count, most = keys.shape[:2]
+        shape = (count, most, self.kv_heads, self.head_dim)
+        k, key_strides = _rows(keys, "keys", self.dtype, self.device, shape)
+        v, value_strides = _rows(values, "values", self.dtype, self.device, shape)
+        self._on.call(self._lib.tsac_cuda_cache_append, self._cache, layer, k, key_strides, v, value_strides,
+                      self._list(sequences, count), _whole(nodes, "nodes", self._int, self.device, (count,)),
+                      _whole(starts, "starts", self._int, self.device, (count,)), count, most,
+                      self._word(error_word), self._on.stream())
+
+    def keep(self, path, accepted, starts=None, lengths_out=None, sequences=None, error_word=None):
+        """Keeps rows start + path[i][:accepted[i]], in every layer, as the next positions."""
+        count, width = path.shape
+        out = self.lengths if lengths_out is None else lengths_out
+        self._on.call(self._lib.tsac_cuda_cache_keep, self._cache, self._list(sequences, count),
+                      _whole(path, "path", self._int, self.device),
+                      _whole(accepted, "accepted", self._int, self.device, (count,)),
+                      _whole(starts, "starts", self._int, self.device, (count,)),
+                      _whole(out, "lengths_out", self._int, self.device, (self.sequences,)), count, width,
+                      self._word(error_word), self._on.stream())
+
+    def compact(self, tables_out=None, refs_out=None, live=None, error_word=None):
+        """Moves the pages in use to the lower end of the pool; returns their number (device int32 [1])."""
+        live = self._torch.empty(1, dtype=self._int, device=self.device) if live is None else live
+        scratch = self._scratch(self._lib.tsac_cuda_cache_compact_scratch_bytes(self.pages))
+        self._on.call(self._lib.tsac_cuda_cache_compact, self._cache,
+                      _whole(self.tables if tables_out is None else tables_out, "tables_out", self._int, self.device,
+                             self.tables.shape),
+                      _whole(self.refs if refs_out is None else refs_out, "refs_out", self._int, self.device, (self.pages,)),
+                      _whole(live, "live", self._int, self.device, (1,)), scratch.data_ptr(), scratch.numel(),
+                      self._word(error_word), self._on.stream())
+        return live
+
+    def attention(self, layer, query, parents, out=None, nodes=None, sequences=None, scale=None, lse=None,
+                  error_word=None):
+        """Attention of each tree's nodes over the cache: query [entry][node][heads][head_dim] -> out."""
+        torch = self._torch
+        if query.dim() != 4:
+            raise TsacError("query must be [entry][node][heads][head_dim]")
+        count, most, heads, _ = query.shape
+        shape = (count, most, heads, self.head_dim)
+        out = torch.empty(shape, dtype=self.dtype, device=self.device) if out is None else out
+        q, query_strides = _rows(query, "query", self.dtype, self.device, shape)
+        o, out_strides = _rows(out, "out", self.dtype, self.device, shape)
+        scratch = self._scratch(self._lib.tsac_cuda_tree_attention_scratch_bytes(self._cache, heads, most))
+        self._on.call(self._lib.tsac_cuda_tree_attention, self._cache, layer, self._list(sequences, count),
+                      _whole(parents, "parents", self._int, self.device, (count, most)),
+                      _whole(nodes, "nodes", self._int, self.device, (count,)), q, query_strides, o, out_strides,
+                      _whole(lse, "lse", torch.float32, self.device, (count, most, heads)), heads, count, most,
+                      self.head_dim ** -0.5 if scale is None else scale, scratch.data_ptr(), scratch.numel(),
+                      self._word(error_word), self._on.stream())
+        return out
+
+
+def draft_verify(target, tokens, parents, coins, draws, draft=None, nodes=None, out=None, error_word=None):
+    """Checks trees of drafted tokens against the target's probabilities (tsac_cuda_draft_verify).
+
+    target [batch][nodes][vocab] (draft the same, or None), tokens and parents
+    int32 [batch][nodes], coins f32 [batch][nodes], draws f32 [batch] in [0, 1).
+    Returns (accepted [batch], path [batch][nodes], token [batch]), int32, in
+    `out` when given."""
+    import torch
+    lib = _drafting()
+    if target.dim() != 3 or not target.is_cuda:
+        raise TsacError("target must be a CUDA tensor [batch][nodes][vocab]")
+    types = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+    batch, most, vocab = target.shape
+    device, kind = target.device, target.dtype
+    for name, t in (("target", target), ("draft", draft)):
+        if t is not None and (t.dtype not in types or t.dtype != kind or t.device != device or t.shape != target.shape
+                              or (vocab > 1 and t.stride(2) != 1)):
+            raise TsacError(f"{name} must be bf16, fp16 or fp32 [batch][nodes][vocab], the vocabulary contiguous")
+    strides = (ctypes.c_ssize_t * 2)(target.stride(0), target.stride(1))
+    draft_strides = (ctypes.c_ssize_t * 2)(draft.stride(0), draft.stride(1)) if draft is not None else None
+    if out is None:
+        out = (torch.empty(batch, dtype=torch.int32, device=device), torch.empty((batch, most), dtype=torch.int32, device=device),
+               torch.empty(batch, dtype=torch.int32, device=device))
+    accepted, path, token = out
+    word = None if error_word is None else _whole(error_word, "error_word", error_word.dtype, device)
+    on = _Device(device)
+    on.call(lib.tsac_cuda_draft_verify, target.data_ptr(), strides, draft.data_ptr() if draft is not None else None,
+            draft_strides, types[kind], _whole(tokens, "tokens", torch.int32, device, (batch, most)),
+            _whole(parents, "parents", torch.int32, device, (batch, most)),
+            _whole(coins, "coins", torch.float32, device, (batch, most)),
+            _whole(draws, "draws", torch.float32, device, (batch,)),
+            _whole(nodes, "nodes", torch.int32, device, (batch,)), batch, most, vocab,
+            _whole(accepted, "accepted", torch.int32, device, (batch,)), _whole(path, "path", torch.int32, device, (batch, most)),
+            _whole(token, "token", torch.int32, device, (batch,)), word, on.stream())
+    return accepted, path, token
+
+
 # --------------------------------------------------------------- analyzer --
 @dataclasses.dataclass
 class EncodeOptions:
