@@ -222,11 +222,13 @@ int tsac_cuda_cache_compact(const tsac_cuda_paged_cache* cache, int32_t* tables_
         });
 }
 
-size_t tsac_cuda_tree_attention_scratch_bytes(const tsac_cuda_paged_cache* cache, size_t, size_t)
+size_t tsac_cuda_tree_attention_scratch_bytes(const tsac_cuda_paged_cache* cache, size_t heads, size_t max_nodes)
 {
-    return cache && (cache->head_dim == 64 || cache->head_dim == 128)
-               ? dev::tree_attention_scratch(static_cast<int>(cache->head_dim))
-               : 0;
+    if (!cache || (cache->head_dim != 64 && cache->head_dim != 128) || cache->kv_heads == 0 || heads > 65536 ||
+        max_nodes > TSAC_CUDA_MAX_NODES)
+        return 0;
+    return dev::tree_attention_scratch(static_cast<int>(cache->head_dim),
+                                       static_cast<int>(heads / cache->kv_heads * max_nodes));
 }
 
 int tsac_cuda_tree_attention(const tsac_cuda_paged_cache* cache, size_t layer, const int32_t* sequences,

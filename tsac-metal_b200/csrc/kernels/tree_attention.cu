@@ -15,12 +15,10 @@
 // asynchronous copies, any page size), so no barrier couples the warps before
 // the end of an item, and two CTAs of four warps keep up to 128 KiB in flight
 // per SM.
+#include "kernels/half_types.cuh"
 #include "kernels/launch_count.hpp"
 #include "kernels/pdl.cuh"
 #include "kernels/tree_attention.cuh"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 
 #include <mutex>
 
@@ -29,52 +27,6 @@ namespace tsacb::dev
 namespace
 {
 constexpr int WARPS = 4, THREADS = WARPS * 32, STAGES = 3, WARP_KEYS = 16, KEYS = WARPS * WARP_KEYS;
-
-template <class T> struct Half2;
-template <> struct Half2<__nv_bfloat16>
-{
-    static __device__ __forceinline__ std::uint32_t pack(float lo, float hi)
-    {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-        return *reinterpret_cast<const std::uint32_t*>(&v);
-    }
-    static __device__ __forceinline__ std::uint16_t one(float x)
-    {
-        return __bfloat16_as_ushort(__float2bfloat16_rn(x));
-    }
-    static __device__ __forceinline__ float value(std::uint16_t x)
-    {
-        return __bfloat162float(__ushort_as_bfloat16(x));
-    }
-    static constexpr std::uint32_t exponents = 0x7f807f80u;
-    static __device__ __forceinline__ void mma(float (&d)[4], const std::uint32_t (&a)[4], std::uint32_t b0,
-                                               std::uint32_t b1)
-    {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9},"
-                     " {%0, %1, %2, %3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-};
-template <> struct Half2<__half>
-{
-    static __device__ __forceinline__ std::uint32_t pack(float lo, float hi)
-    {
-        const __half2 v = __floats2half2_rn(lo, hi);
-        return *reinterpret_cast<const std::uint32_t*>(&v);
-    }
-    static __device__ __forceinline__ std::uint16_t one(float x) { return __half_as_ushort(__float2half_rn(x)); }
-    static __device__ __forceinline__ float value(std::uint16_t x) { return __half2float(__ushort_as_half(x)); }
-    static constexpr std::uint32_t exponents = 0x7c007c00u;
-    static __device__ __forceinline__ void mma(float (&d)[4], const std::uint32_t (&a)[4], std::uint32_t b0,
-                                               std::uint32_t b1)
-    {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9},"
-                     " {%0, %1, %2, %3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-};
 
 __device__ __forceinline__ void load_matrices(std::uint32_t address, std::uint32_t (&r)[4])
 {
@@ -90,58 +42,8 @@ __device__ __forceinline__ void load_matrices_transposed(std::uint32_t address, 
                  : "r"(address)
                  : "memory");
 }
-// 16-byte copy, or 16 zero bytes when `bytes` is 0.
-__device__ __forceinline__ void copy_16(std::uint32_t to, const void* from, unsigned bytes)
-{
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ float power_of_two(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// Bit a of masks[n]: node a is node n or one of its ancestors.  Pointer
-// doubling: log2(64) rounds in place of a walk of up to 64 dependent steps.
-// A parent below -1 makes a node that sees no drafted node, not even itself;
-// one that is not before its child is reported and treated as such.
-__device__ __forceinline__ void ancestor_masks(const int* parents, int nodes, unsigned long long* masks, int* above,
-                                               unsigned* error_word, int t, int threads)
-{
-    for (int n = t; n < DRAFT_MAX_NODES; n += threads)
-    {
-        const int parent = n < nodes ? parents[n] : -2;
-        const bool wrong = parent >= n;
-        if (wrong && n < nodes && error_word)
-            atomicOr(error_word, error_cache);
-        masks[n] = parent < -1 || wrong ? 0ull : 1ull << n;
-        above[n] = wrong || parent < 0 ? -1 : parent;
-    }
-    __syncthreads();
-    for (int round = 0; round < 6; ++round)
-    {
-        unsigned long long mask[(DRAFT_MAX_NODES + 31) / 32];
-        int next[(DRAFT_MAX_NODES + 31) / 32];
-        int k = 0;
-        for (int n = t; n < DRAFT_MAX_NODES; n += threads, ++k)
-        {
-            const int up = above[n];
-            mask[k] = up >= 0 ? masks[up] : 0ull;
-            next[k] = up >= 0 ? above[up] : -1;
-        }
-        __syncthreads();
-        k = 0;
-        for (int n = t; n < DRAFT_MAX_NODES; n += threads, ++k)
-        {
-            masks[n] |= mask[k];
-            above[n] = next[k];
-        }
-        __syncthreads();
-    }
-}
 
 template <int D, int MT> struct Layout
 {
@@ -173,31 +75,19 @@ __global__ void __launch_bounds__(THREADS, 2)
         shared_items[cta].pieces = 0;
     if (cta >= start.ctas)
         return;
-    long long unit = Work::first_unit(start.units, cta, start.ctas);
-    const long long last_unit = Work::first_unit(start.units, cta + 1, start.ctas);
     const std::uint32_t ring = static_cast<std::uint32_t>(__cvta_generic_to_shared(smem)) + warp * STAGES * L::stage_bytes;
     const unsigned char* plane = a.cache.pool + 2ll * a.layer * a.cache.plane_bytes;
 
-    int list_entry = start.entry;
-    long long before = start.before;
-    while (unit < last_unit)
+    typename Work::Cursor cursor(start, cta);
+    typename Work::Segment g;
+    while (cursor.next(a, g))
     {
-        const auto e = Work::entry(a, list_entry);
-        if (unit >= before + e.units)
-        {
-            before += e.units;
-            ++list_entry;
-            continue;
-        }
-        const int item = static_cast<int>((unit - before) / e.tiles);
-        const int head = item / e.row_items, first_row = (item - head * e.row_items) * L::ROWS;
-        const long long item_start = before + static_cast<long long>(item) * e.tiles;
-        const int tile_begin = static_cast<int>(unit - item_start);
-        const int tile_end = static_cast<int>(min(static_cast<long long>(e.tiles), last_unit - item_start));
-        const int rows = e.nodes * a.group;
+        const auto& e = g.e;
+        const int head = g.head, first_row = g.first_row, rows = g.rows;
+        const int tile_begin = g.tile_begin, tile_end = g.tile_end;
         if (tile_end == e.tiles)
-            ancestor_masks(a.parents + static_cast<long long>(list_entry) * a.max_nodes, e.nodes, masks, above,
-                           a.error_word, t, THREADS);
+            ancestor_masks(a.parents + static_cast<long long>(g.list_entry) * a.max_nodes, e.nodes, masks, above,
+                           a.error_word, t, [] { __syncthreads(); });
 
         // Query fragments: row lane / 4 (+ 8), columns 2 (lane % 4) (+ 8) of each 16.
         std::uint32_t q[MT][D / 16][4];
@@ -208,7 +98,7 @@ __global__ void __launch_bounds__(THREADS, 2)
             {
                 const int row = first_row + 16 * m + 8 * r + (lane >> 2);
                 const int node = row / a.group, in_group = row - node * a.group;
-                const std::uint16_t* from = a.query + list_entry * a.query_batch + node * a.query_node +
+                const std::uint16_t* from = a.query + g.list_entry * a.query_batch + node * a.query_node +
                                             (head * a.group + in_group) * a.query_head + 2 * (lane & 3);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
@@ -226,26 +116,8 @@ __global__ void __launch_bounds__(THREADS, 2)
             sum[m][0] = sum[m][1] = 0.0f;
         }
 
-        // Byte offset of this lane's key row (lane % 16 of the warp's 16) in a tile; -1: no such key.
-        const auto key_row = [&](int tile) -> long long
-        {
-            if (tile >= tile_end)
-                return -1;
-            const bool drafted = tile == e.tiles - 1;
-            const int in_tile = warp * WARP_KEYS + (lane & 15);
-            const int position = drafted ? e.length + in_tile : tile * KEYS + in_tile;
-            if (drafted ? in_tile >= e.nodes : position >= e.length)
-                return -1;
-            const int page = cache_page(a.cache, e.sequence, e.held, position >> a.cache.page_shift);
-            if (page < 0)
-            {
-                if (a.error_word)
-                    atomicOr(a.error_word, error_cache);
-                return -1;
-            }
-            return page * a.cache.page_bytes() +
-                   static_cast<long long>(position & (a.cache.page_size() - 1)) * a.cache.row_bytes + head * L::row_bytes;
-        };
+        // Lane % 16 follows one of the warp's 16 keys.
+        const auto key_row = [&](int tile) { return Work::key_row(a, g, tile, warp * WARP_KEYS + (lane & 15)); };
         // Rows of L::chunks 16-byte chunks, chunk c of row r at place c ^ (r & 7): conflict-free for ldmatrix.
         const auto fetch = [&](int stage, long long row_offset)
         {
@@ -315,11 +187,7 @@ __global__ void __launch_bounds__(THREADS, 2)
                         const std::uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                         for (int w = 0; w < 4; ++w)
-                        {
-                            const std::uint32_t x = words[w] & Half2<T>::exponents;
-                            odd |= (x & 0xffffu) == (Half2<T>::exponents & 0xffffu) ||
-                                   (x >> 16) == (Half2<T>::exponents >> 16);
-                        }
+                            odd |= nonfinite_mask<T>(words[w]) != 0;
                     }
                     tainted |= __any_sync(0xffffffffu, odd) ? 1u << row : 0u;
                 }
@@ -502,18 +370,17 @@ __global__ void __launch_bounds__(THREADS, 2)
             }
             const int node = (first_row + row) / a.group, in_group = first_row + row - node * a.group;
             const float inverse = total == 0.0f ? 0.0f : 1.0f / total; // a row that sees nothing gives zeros
-            std::uint16_t* to = a.out + list_entry * a.out_batch + node * a.out_node +
+            std::uint16_t* to = a.out + g.list_entry * a.out_batch + node * a.out_node +
                                 (head * a.group + in_group) * a.out_head + column;
             *reinterpret_cast<uint2*>(to) =
                 make_uint2(Half2<T>::pack(v.x * inverse, v.y * inverse), Half2<T>::pack(v.z * inverse, v.w * inverse));
             if (a.lse && column == 0)
-                a.lse[(static_cast<long long>(list_entry) * a.max_nodes + node) * a.heads * a.group + head * a.group +
+                a.lse[(static_cast<long long>(g.list_entry) * a.max_nodes + node) * a.heads * a.group + head * a.group +
                       in_group] = total == 0.0f ? -INFINITY : (best + log2f(total)) * 0.6931471805599453f;
         }
         if (tile_begin == 0 && !whole && t == 0)
-            shared_items[cta] = TreeShared{list_entry, head, first_row,
-                                           Work::owner(start.units, item_start + e.tiles - 1, start.ctas) - cta + 1, e.nodes};
-        unit = item_start + tile_end;
+            shared_items[cta] = TreeShared{g.list_entry, head, first_row,
+                                           Work::owner(start.units, g.item_start + e.tiles - 1, start.ctas) - cta + 1, e.nodes};
         __syncthreads(); // the ring and the row statistics are free again
     }
 }
@@ -567,23 +434,29 @@ __global__ void __launch_bounds__(128)
             total == 0.0f ? -INFINITY : (best + log2f(total)) * 0.6931471805599453f;
 }
 
-int grid_ctas()
+int sms()
 {
-    int device = 0, sms = 148;
+    int device = 0, count = 148;
     if (cudaGetDevice(&device) == cudaSuccess)
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    return 2 * sms;
+        cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device);
+    return count;
 }
 
-size_t scratch_bytes(int ctas, int rows, int head_dim)
+// CTAs of the launch and rows of one item, by rows per key head.
+struct Shape
 {
-    return static_cast<size_t>(ctas) * (2 * sizeof(float) * static_cast<size_t>(tree_piece_floats(rows, head_dim)) +
-                                        sizeof(TreeShared));
-}
+    int ctas, rows;
+    explicit Shape(int rows_per_head)
+        : ctas(tree_attention_many(rows_per_head) ? sms() : 2 * sms()),
+          rows(tree_attention_many(rows_per_head) ? tree_attention_tc_rows(rows_per_head) : 16)
+    {
+    }
+};
 
-template <class T, int D, int MT> cudaError_t launch(const TreeArgs& a, void* scratch, cudaStream_t stream)
+template <class T, int D>
+void launch_few(const TreeArgs& a, const Shape& shape, float* pieces, TreeShared* items, cudaStream_t stream)
 {
-    using L = Layout<D, MT>;
+    using L = Layout<D, 1>;
     static std::once_flag once[64];
     int device = 0;
     cudaGetDevice(&device);
@@ -591,34 +464,56 @@ template <class T, int D, int MT> cudaError_t launch(const TreeArgs& a, void* sc
         std::call_once(once[device],
                        []
                        {
-                           cudaFuncSetAttribute(tree_attention_kernel<T, D, MT>,
+                           cudaFuncSetAttribute(tree_attention_kernel<T, D, 1>,
                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem);
                        });
-    const int ctas = grid_ctas();
-    auto* pieces = static_cast<float*>(scratch);
-    auto* items = reinterpret_cast<TreeShared*>(pieces + 2ll * ctas * tree_piece_floats(L::ROWS, D));
-    launch_pdl(tree_attention_kernel<T, D, MT>, dim3(ctas), dim3(THREADS), L::smem, stream, a, pieces, items);
+    launch_pdl(tree_attention_kernel<T, D, 1>, dim3(shape.ctas), dim3(THREADS), L::smem, stream, a, pieces, items);
     note_launch();
-    launch_pdl(tree_combine_kernel<T, D>, dim3(ctas, (L::ROWS + 3) / 4), dim3(128), 0, stream, a, L::ROWS,
+}
+
+template <class T, int D> cudaError_t launch(const TreeArgs& a, ValueType type, void* scratch, cudaStream_t stream)
+{
+    const int rows = a.max_nodes * a.group;
+    const Shape shape(rows);
+    auto* pieces = static_cast<float*>(scratch);
+    auto* items = reinterpret_cast<TreeShared*>(pieces + 2ll * shape.ctas * tree_piece_floats(shape.rows, D));
+    if (tree_attention_many(rows))
+    {
+        const cudaError_t status = tree_attention_tc(a, type, pieces, items, stream);
+        if (status != cudaSuccess)
+            return status;
+    }
+    else
+    {
+        launch_few<T, D>(a, shape, pieces, items, stream);
+    }
+    launch_pdl(tree_combine_kernel<T, D>, dim3(shape.ctas, (shape.rows + 3) / 4), dim3(128), 0, stream, a, shape.rows,
                static_cast<const float*>(pieces), static_cast<const TreeShared*>(items));
     note_launch();
     return cudaGetLastError();
 }
 
-template <class T> cudaError_t launch_type(const TreeArgs& a, void* scratch, cudaStream_t stream)
+template <class T> cudaError_t launch_type(const TreeArgs& a, ValueType type, void* scratch, cudaStream_t stream)
 {
-    return a.head_dim == 64 ? launch<T, 64, 1>(a, scratch, stream) : launch<T, 128, 1>(a, scratch, stream);
+    return a.head_dim == 64 ? launch<T, 64>(a, type, scratch, stream) : launch<T, 128>(a, type, scratch, stream);
 }
 } // namespace
 
-size_t tree_attention_scratch(int head_dim)
+bool tree_attention_many(int rows)
 {
-    return scratch_bytes(grid_ctas(), 16, head_dim);
+    return rows > 16;
+}
+
+size_t tree_attention_scratch(int head_dim, int rows)
+{
+    const Shape shape(rows);
+    return static_cast<size_t>(shape.ctas) *
+           (2 * sizeof(float) * static_cast<size_t>(tree_piece_floats(shape.rows, head_dim)) + sizeof(TreeShared));
 }
 
 cudaError_t tree_attention(const TreeArgs& a, ValueType type, void* scratch, cudaStream_t stream)
 {
-    return type == ValueType::bf16 ? launch_type<__nv_bfloat16>(a, scratch, stream)
-                                   : launch_type<__half>(a, scratch, stream);
+    return type == ValueType::bf16 ? launch_type<__nv_bfloat16>(a, type, scratch, stream)
+                                   : launch_type<__half>(a, type, scratch, stream);
 }
 } // namespace tsacb::dev

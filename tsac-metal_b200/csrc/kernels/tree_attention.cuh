@@ -144,7 +144,107 @@ template <int KEYS, int ROWS> struct TreeWork
         s.ctas = sharing;
         return s;
     }
+
+    // A CTA's part of one item: tiles [tile_begin, tile_end) of its e.tiles.
+    struct Segment
+    {
+        Entry e;
+        int list_entry, head, first_row, rows, tile_begin, tile_end;
+        long long item_start; // the item's first unit
+    };
+
+    // Walks the segments of a CTA's share; every thread of the CTA may keep its own.
+    struct Cursor
+    {
+        long long unit, last_unit, before;
+        int list_entry;
+
+        __device__ __forceinline__ Cursor(const Start& s, int cta)
+            : unit(first_unit(s.units, cta, s.ctas)), last_unit(first_unit(s.units, cta + 1, s.ctas)),
+              before(s.before), list_entry(s.entry)
+        {
+        }
+        __device__ __forceinline__ bool next(const TreeArgs& a, Segment& s)
+        {
+            while (unit < last_unit)
+            {
+                s.e = entry(a, list_entry);
+                if (unit >= before + s.e.units)
+                {
+                    before += s.e.units;
+                    ++list_entry;
+                    continue;
+                }
+                const int item = static_cast<int>((unit - before) / s.e.tiles);
+                s.list_entry = list_entry;
+                s.head = item / s.e.row_items;
+                s.first_row = (item - s.head * s.e.row_items) * ROWS;
+                s.rows = s.e.nodes * a.group;
+                s.item_start = before + static_cast<long long>(item) * s.e.tiles;
+                s.tile_begin = static_cast<int>(unit - s.item_start);
+                s.tile_end = static_cast<int>(min(static_cast<long long>(s.e.tiles), last_unit - s.item_start));
+                unit = s.item_start + s.tile_end;
+                return true;
+            }
+            return false;
+        }
+    };
+
+    // Byte offset in a plane of key row `in_tile` of a tile, for one key head; -1: no such key.
+    static __device__ __forceinline__ long long key_row(const TreeArgs& a, const Segment& s, int tile, int in_tile)
+    {
+        if (tile >= s.tile_end)
+            return -1;
+        const bool drafted = tile == s.e.tiles - 1;
+        const int position = drafted ? s.e.length + in_tile : tile * KEYS + in_tile;
+        if (drafted ? in_tile >= s.e.nodes : position >= s.e.length)
+            return -1;
+        const int page = cache_page(a.cache, s.e.sequence, s.e.held, position >> a.cache.page_shift);
+        if (page < 0)
+        {
+            if (a.error_word)
+                atomicOr(a.error_word, error_cache);
+            return -1;
+        }
+        return page * a.cache.page_bytes() +
+               static_cast<long long>(position & (a.cache.page_size() - 1)) * a.cache.row_bytes +
+               2ll * s.head * a.head_dim;
+    }
 };
+
+// Bit a of masks[n]: node a is node n or one of its ancestors.  Pointer
+// doubling: log2(64) rounds in place of a walk of up to 64 dependent steps.
+// A parent below -1 makes a node that sees no drafted node, not even itself;
+// one that is not before its child is reported and treated as such.
+// Called by at least 64 threads, numbered from 0; `sync` is their barrier.
+template <class Sync>
+__device__ __forceinline__ void ancestor_masks(const int* parents, int nodes, unsigned long long* masks, int* above,
+                                               unsigned* error_word, int t, Sync&& sync)
+{
+    if (t < DRAFT_MAX_NODES)
+    {
+        const int parent = t < nodes ? parents[t] : -2;
+        const bool wrong = parent >= t;
+        if (wrong && error_word)
+            atomicOr(error_word, error_cache);
+        masks[t] = parent < -1 || wrong ? 0ull : 1ull << t;
+        above[t] = wrong || parent < 0 ? -1 : parent;
+    }
+    sync();
+    for (int round = 0; round < 6; ++round)
+    {
+        const int up = t < DRAFT_MAX_NODES ? above[t] : -1;
+        const unsigned long long mask = up >= 0 ? masks[up] : 0ull;
+        const int next = up >= 0 ? above[up] : -1;
+        sync();
+        if (t < DRAFT_MAX_NODES)
+        {
+            masks[t] |= mask;
+            above[t] = next;
+        }
+        sync();
+    }
+}
 
 // What a CTA leaves for the combining launch: the item it began and did not finish.
 struct TreeShared
@@ -160,6 +260,12 @@ inline __host__ __device__ long long tree_piece_floats(int rows, int head_dim)
     return static_cast<long long>(rows) * (head_dim + TREE_PIECE_HEAD);
 }
 
-size_t tree_attention_scratch(int head_dim);
+// The launches by rows per key head (max_nodes * group): tree_attention.cu
+// for few, tree_attention_tc.cu for many.
+bool tree_attention_many(int rows);
+size_t tree_attention_scratch(int head_dim, int rows);
 cudaError_t tree_attention(const TreeArgs& a, ValueType type, void* scratch, cudaStream_t stream);
+cudaError_t tree_attention_tc(const TreeArgs& a, ValueType type, float* pieces, TreeShared* shared_items,
+                              cudaStream_t stream);
+int tree_attention_tc_rows(int rows); // rows of one of its items
 } // namespace tsacb::dev

@@ -1,0 +1,777 @@
+// Attention of trees of drafted tokens over a paged key/value cache, for many
+// query rows per key head, on the tensor cores (tcgen05).
+//
+// The formula and the division of the work are those of tree_attention.cu and
+// tree_attention.cuh, with tiles of 128 keys and items of 128 or 256 rows.  A
+// tile of 128 keys is two products of 128 x 128 x D per 128 rows: at 128 rows
+// the tensor cores need about a third of the time that the tile's bytes take
+// to arrive, at 256 rows two thirds, and the exponentials (16 per clock and
+// SM) about as much.  So a CTA takes up to 256 rows of a key head at once, the
+// keys and values cross HBM once, and the kernel is bound by HBM as long as
+// products, exponentials and loads overlap.
+//
+// One CTA per SM, 11 warps:
+//   warps 0-3, 4-7  two softmax groups, one query row per thread.  Each has its
+//                   own scores S and output O in TMEM.  With 256 rows each
+//                   group has 128 of them and sees every tile; with 128 rows
+//                   the groups take alternate tiles of the same rows, and their
+//                   outputs are joined at the end of the item.
+//   warp 8          TMEM owner and MMA issuer: S = Q K^T from shared memory,
+//                   then O += P V with P in TMEM over the columns of S.  The
+//                   two groups' products alternate, so that one group's
+//                   exponentials overlap the other's products.
+//   warps 9, 10     producers: each key or value tile (128 rows of any pages)
+//                   by 16-byte asynchronous copies into a ring of shared-memory
+//                   slots in the 128-byte swizzle that the MMA reads; rows
+//                   behind the last position become zeros.
+// The running maximum moves only when a row's tile exceeds it by more than 8
+// (in powers of two): p then stays below 256, which bf16, fp16 and the 32-bit
+// sums hold as well as 1, and the output in TMEM is rescaled rarely.
+//
+// Every wait is bounded (tc_common.cuh).  One that gives up raises
+// error_timeout and the CTA's abort flag; softmax threads then run through
+// their loops without waiting, so that no thread waits at a barrier that
+// others have left.
+#include "kernels/half_types.cuh"
+#include "kernels/launch_count.hpp"
+#include "kernels/pdl.cuh"
+#include "kernels/tc_common.cuh"
+#include "kernels/tree_attention.cuh"
+
+namespace tsacb::dev
+{
+namespace
+{
+using namespace tc;
+
+constexpr int KEYS = 128;
+constexpr int GROUP_THREADS = 128, SOFTMAX_THREADS = 2 * GROUP_THREADS;
+// Eleven warps leave each thread 168 registers; a 13th warp would leave 128,
+// and the softmax threads would spill.
+constexpr int MMA_WARP = 8, PRODUCER_WARP = 9, PRODUCERS = 64, PRODUCER_ROWS = KEYS / 2;
+constexpr int THREADS = PRODUCER_WARP * 32 + PRODUCERS;
+constexpr int TMEM_COLUMNS = 512, OUTPUT_COLUMN = 256; // S of the groups at 0 and 128, O at 256 and 384
+constexpr float RESCALE = 8.0f;                        // powers of two
+constexpr int TAINT_SLOTS = 16; // segments that the producers can be ahead of the epilogue, and more
+
+template <int D, bool TWO> struct Tiles
+{
+    static constexpr int ROWS = TWO ? 256 : 128;
+    static constexpr int panel_bytes = KEYS * 128;           // 64 columns of 128 rows
+    static constexpr int operand_bytes = panel_bytes * (D / 64);
+    static constexpr int query_bytes = operand_bytes * (ROWS / 128);
+    static constexpr int SLOTS = D == 128 ? 5 : 10;
+    static constexpr int chunks = D / 8;
+    static constexpr int ring_offset = query_bytes;
+    static constexpr int tail_offset = ring_offset + SLOTS * operand_bytes;
+    static constexpr int tail_bytes = TWO ? 2048 : 4096; // barriers and small arrays
+    static constexpr int smem = tail_offset + tail_bytes + 1024; // the rest: alignment
+    static_assert(smem <= 227 * 1024, "shared memory of one SM");
+};
+
+template <bool TWO> struct Tail
+{
+    uint64_t full[10], empty[10];
+    uint64_t scores[2], weights[2], products[2], query, drain;
+    unsigned long long masks[DRAFT_MAX_NODES];
+    unsigned long long tainted[TAINT_SLOTS];
+    long long warp_sums[THREADS / 32];
+    float maximum[2][TWO ? 1 : GROUP_THREADS], sum[2][TWO ? 1 : GROUP_THREADS]; // of the groups' shares of a row
+    int above[DRAFT_MAX_NODES];
+    long long start[4]; // TreeWork::Start
+    uint32_t tmem;
+    int abort;
+};
+static_assert(sizeof(Tail<true>) <= 2048 && sizeof(Tail<false>) <= 4096, "tail of the shared memory");
+
+__device__ __forceinline__ void tmem_load32(uint32_t address, uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32"
+                 " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
+                 " %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+                   "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+                   "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+                   "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(address));
+}
+
+__device__ __forceinline__ uint32_t tmem_load1(uint32_t address)
+{
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(address));
+    return r;
+}
+
+__device__ __forceinline__ void tmem_store16(uint32_t address, const uint32_t* r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
+                 " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(address),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+                 "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_wait_stores()
+{
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void fence_async_proxy()
+{
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// Barrier of the softmax threads.
+__device__ __forceinline__ void softmax_sync()
+{
+    asm volatile("bar.sync 1, %0;" ::"n"(SOFTMAX_THREADS) : "memory");
+}
+
+// MN-major operand, 128-byte swizzle: 64 columns x 8 rows of k per 1024-byte
+// atom; the next 64 columns one panel further, the next 8 rows one atom.
+__device__ __forceinline__ uint64_t value_desc(uint32_t address, uint32_t panel_bytes)
+{
+    uint64_t d = static_cast<uint64_t>((address & 0x3ffffu) >> 4);
+    d |= static_cast<uint64_t>(panel_bytes >> 4) << 16;
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(2) << 61;
+    return d;
+}
+
+// kind::f16 with 32-bit accumulation, M = 128.
+template <class T> __device__ __forceinline__ constexpr uint32_t instruction(int n, bool b_mn_major)
+{
+    return (1u << 4) | (Half2<T>::mma_format << 7) | (Half2<T>::mma_format << 10) | (b_mn_major ? 1u << 16 : 0u) |
+           (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+}
+
+__device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+
+// Operand `op` of a segment of `tiles` tiles, in the order in which the MMA
+// warp first needs them: whether it is a value tile, and of which tile.
+template <bool TWO> __device__ __forceinline__ void operand(int op, int tiles, bool& value, int& tile)
+{
+    if (TWO || tiles == 1)
+    {
+        value = op & 1;
+        tile = op >> 1;
+        return;
+    }
+    // K0 K1, then V(j) K(j + 2), then the last two V.
+    const int k = op - 2, steady = 2 * (tiles - 2);
+    value = k >= steady || (k >= 0 && !(k & 1));
+    tile = k < 0 ? op : (k >= steady ? tiles - 2 + (k - steady) : (k & 1 ? (k >> 1) + 2 : k >> 1));
+}
+
+// One number for each softmax group, selected without an array in memory.
+template <class N> struct Both
+{
+    N first, second;
+    __device__ __forceinline__ N operator()(int group) const { return group ? second : first; }
+    __device__ __forceinline__ void add(int group, N n)
+    {
+        first += group ? N(0) : n;
+        second += group ? n : N(0);
+    }
+};
+
+template <class T, int D, bool TWO>
+__global__ void __launch_bounds__(THREADS, 1)
+    tree_attention_tc_kernel(const TreeArgs a, float* pieces, TreeShared* shared_items)
+{
+    pdl_prologue();
+    using L = Tiles<D, TWO>;
+    using Work = TreeWork<KEYS, L::ROWS>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                                           ~static_cast<uintptr_t>(1023));
+    Tail<TWO>& tail = *reinterpret_cast<Tail<TWO>*>(smem + L::tail_offset);
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    const int cta = blockIdx.x;
+    static_assert(sizeof(typename Work::Start) <= sizeof(tail.start));
+    const auto start = Work::template find<THREADS>(a, cta, gridDim.x, tail.warp_sums,
+                                                    reinterpret_cast<typename Work::Start*>(tail.start));
+    if (t == 0)
+        shared_items[cta].pieces = 0;
+    if (cta >= start.ctas)
+        return;
+    if (t == 0)
+    {
+        for (int s = 0; s < L::SLOTS; ++s)
+        {
+            bar_init(smem_u32(&tail.full[s]), PRODUCERS);
+            bar_init(smem_u32(&tail.empty[s]), 1);
+        }
+        for (int g = 0; g < 2; ++g)
+        {
+            bar_init(smem_u32(&tail.scores[g]), 1);
+            bar_init(smem_u32(&tail.weights[g]), GROUP_THREADS);
+            bar_init(smem_u32(&tail.products[g]), 1);
+        }
+        bar_init(smem_u32(&tail.query), SOFTMAX_THREADS);
+        bar_init(smem_u32(&tail.drain), 1);
+        for (int k = 0; k < TAINT_SLOTS; ++k)
+            tail.tainted[k] = 0;
+        tail.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == MMA_WARP)
+    {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tail.tmem)),
+                     "r"(TMEM_COLUMNS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tail.tmem;
+    volatile int* abort_flag = &tail.abort;
+    const unsigned char* plane = a.cache.pool + 2ll * a.layer * a.cache.plane_bytes;
+    bool ok = true;
+    const auto wait = [&](uint64_t& bar, int phase)
+    {
+        if (ok && !bar_wait(smem_u32(&bar), static_cast<uint32_t>(phase & 1), abort_flag))
+        {
+            ok = false;
+            *abort_flag = 1;
+            if (a.error_word)
+                atomicOr(a.error_word, error_timeout);
+        }
+        return ok;
+    };
+    typename Work::Cursor cursor(start, cta);
+    typename Work::Segment g;
+
+    if (warp >= PRODUCER_WARP)
+    {
+        // ------------------------------------------------------------ producers --
+        const int first_row = (warp - PRODUCER_WARP) * PRODUCER_ROWS; // this warp's rows of each tile
+        constexpr int rows_at_once = 32 / L::chunks;
+        int slot = 0, round = 0; // uses of the slot so far
+        for (int segment = 0; ok && cursor.next(a, g); ++segment)
+        {
+            const int tiles = g.tile_end - g.tile_begin;
+            bool value;
+            int tile;
+            operand<TWO>(0, tiles, value, tile);
+            long long low_rows, high_rows; // this lane's rows, lane and lane + 32 of the warp's
+            const auto find_rows = [&]
+            {
+                low_rows = Work::key_row(a, g, g.tile_begin + tile, first_row + lane);
+                high_rows = Work::key_row(a, g, g.tile_begin + tile, first_row + 32 + lane);
+            };
+            find_rows();
+            for (int op = 0; op < 2 * tiles; ++op)
+            {
+                const bool this_value = value, drafted = g.tile_begin + tile == g.e.tiles - 1;
+                wait(tail.empty[slot], round + 1);
+                ok = __all_sync(0xffffffffu, ok); // the warp goes on or leaves together
+                if (!ok)
+                    break;
+                const uint32_t base = smem_u32(smem + L::ring_offset + slot * L::operand_bytes);
+                const unsigned char* from = plane + (value ? a.cache.plane_bytes : 0);
+                const int chunk = lane % L::chunks;
+                const uint32_t column = base + (chunk >> 3) * L::panel_bytes;
+#pragma unroll 8
+                for (int i = 0; i < PRODUCER_ROWS / rows_at_once; ++i)
+                {
+                    const int row = i * rows_at_once + lane / L::chunks;
+                    const long long offset = __shfl_sync(0xffffffffu, i * rows_at_once < 32 ? low_rows : high_rows, row & 31);
+                    copy_16(column + (first_row + row) * 128 + (((chunk & 7) ^ (row & 7)) << 4),
+                            from + (offset >= 0 ? offset + 16 * chunk : 0), offset >= 0 ? 16u : 0u);
+                }
+                // The next tile's table entries are on their way while this one is copied.
+                if (op + 1 < 2 * tiles)
+                {
+                    operand<TWO>(op + 1, tiles, value, tile);
+                    find_rows();
+                }
+                const uint32_t bar = smem_u32(&tail.full[slot]);
+                if (this_value && drafted)
+                {
+                    // 0 x NaN would reach rows that do not see the node: values that are not
+                    // finite leave the product and are added where they are seen.
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    for (int i = 0; i < PRODUCER_ROWS / rows_at_once; ++i)
+                    {
+                        const int row = first_row + i * rows_at_once + lane / L::chunks;
+                        auto* at = reinterpret_cast<uint4*>(smem + L::ring_offset + slot * L::operand_bytes +
+                                                            (chunk >> 3) * L::panel_bytes + row * 128 +
+                                                            (((chunk & 7) ^ (row & 7)) << 4));
+                        uint4 v = *at;
+                        const uint32_t odd[4] = {nonfinite_mask<T>(v.x), nonfinite_mask<T>(v.y),
+                                                 nonfinite_mask<T>(v.z), nonfinite_mask<T>(v.w)};
+                        if (odd[0] | odd[1] | odd[2] | odd[3])
+                        {
+                            *at = make_uint4(v.x & ~odd[0], v.y & ~odd[1], v.z & ~odd[2], v.w & ~odd[3]);
+                            atomicOr(&tail.tainted[segment % TAINT_SLOTS], 1ull << (row & 63));
+                        }
+                    }
+                    bar_arrive(bar);
+                }
+                else
+                {
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+                }
+                if (++slot == L::SLOTS)
+                {
+                    slot = 0;
+                    ++round;
+                }
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    }
+    else if (warp == MMA_WARP)
+    {
+        // ------------------------------------------------------------------ MMA --
+        if (lane == 0)
+        {
+            constexpr uint32_t score_idesc = instruction<T>(KEYS, false), value_idesc = instruction<T>(D, true);
+            int slot = 0, round = 0;
+            Both<int> made{0, 0}; // products issued
+            bool any = false;
+            const auto take = [&]() -> int // the next operand's slot, once it has landed
+            {
+                const int s = slot;
+                wait(tail.full[s], round);
+                fence_async_proxy(); // the copies are generic writes, the MMA reads through the async proxy
+                if (++slot == L::SLOTS)
+                {
+                    slot = 0;
+                    ++round;
+                }
+                return s;
+            };
+            const auto score = [&](int group, int s)
+            {
+                if (!ok)
+                    return;
+                const uint32_t q = smem_u32(smem) + (TWO ? group * L::operand_bytes : 0);
+                const uint32_t k = smem_u32(smem + L::ring_offset + s * L::operand_bytes);
+                tc_fence_after();
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                {
+                    const uint32_t at = (kk >> 2) * L::panel_bytes + (kk & 3) * 32;
+                    mma_shared(tmem + group * KEYS, sw128_desc(q + at), sw128_desc(k + at), score_idesc, kk != 0);
+                }
+                mma_commit(smem_u32(&tail.scores[group]));
+                any = true;
+            };
+            const auto product = [&](int group, int s, bool accumulate)
+            {
+                if (!ok || !wait(tail.weights[group], made(group)))
+                    return;
+                const uint32_t v = smem_u32(smem + L::ring_offset + s * L::operand_bytes);
+                tc_fence_after();
+#pragma unroll
+                for (int kk = 0; kk < KEYS / 16; ++kk)
+                    mma_tmem(tmem + OUTPUT_COLUMN + group * 128, tmem + group * KEYS + 8 * kk,
+                             value_desc(v + kk * 2048, L::panel_bytes), value_idesc, accumulate || kk != 0);
+                mma_commit(smem_u32(&tail.products[group]));
+                made.add(group, 1);
+            };
+            // P lies over S: the next scores of a group wait for its product.
+            const auto after_product = [&](int group) { wait(tail.products[group], made(group) - 1); };
+            const auto free_slot = [&](int s)
+            {
+                if (ok)
+                    mma_commit(smem_u32(&tail.empty[s]));
+            };
+            for (int segment = 0; ok && cursor.next(a, g); ++segment)
+            {
+                const int tiles = g.tile_end - g.tile_begin;
+                wait(tail.query, segment);
+                if constexpr (TWO)
+                {
+                    int k = take();
+                    score(0, k);
+                    score(1, k);
+                    free_slot(k);
+                    for (int j = 0; j < tiles && ok; ++j)
+                    {
+                        const int v = take();
+                        const bool more = j + 1 < tiles;
+                        product(0, v, j > 0);
+                        if (more)
+                        {
+                            k = take();
+                            after_product(0);
+                            score(0, k);
+                        }
+                        product(1, v, j > 0);
+                        free_slot(v);
+                        if (more)
+                        {
+                            after_product(1);
+                            score(1, k);
+                            free_slot(k);
+                        }
+                    }
+                }
+                else
+                {
+                    for (int j = 0; j < 2 && j < tiles; ++j)
+                    {
+                        const int k = take();
+                        score(j, k);
+                        free_slot(k);
+                    }
+                    for (int j = 0; j < tiles && ok; ++j)
+                    {
+                        const int v = take();
+                        product(j & 1, v, j > 1);
+                        free_slot(v);
+                        if (j + 2 < tiles)
+                        {
+                            const int k = take();
+                            after_product(j & 1);
+                            score(j & 1, k);
+                            free_slot(k);
+                        }
+                    }
+                }
+            }
+            if (any)
+            {
+                mma_commit(smem_u32(&tail.drain));
+                volatile int never = 0;
+                bar_wait(smem_u32(&tail.drain), 0, &never);
+            }
+        }
+    }
+    else
+    {
+        // -------------------------------------------------------------- softmax --
+        const int group = warp >> 2, row = t & (GROUP_THREADS - 1);
+        const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        const uint32_t my_scores = lanes + group * KEYS, my_output = lanes + OUTPUT_COLUMN + group * 128;
+        // A negative scale turns the query's signs, so that the largest product stays the largest score.
+        const uint32_t turn = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
+        const float scale = fabsf(a.scale_log2);
+        int scores_seen = 0;
+        Both<int> products_seen{0, 0};
+        for (int segment = 0; cursor.next(a, g); ++segment)
+        {
+            const int tiles = g.tile_end - g.tile_begin;
+            const bool has_draft = g.tile_end == g.e.tiles;
+            const int item_row = TWO ? t : row; // this thread's row of the item
+            const bool live = g.first_row + item_row < g.rows;
+            const int node = live ? (g.first_row + item_row) / a.group : 0;
+            const int query_head = g.head * a.group + (g.first_row + item_row - node * a.group);
+            {
+                // With 128 rows the groups load half a row each.
+                constexpr int mine = TWO ? L::chunks : L::chunks / 2;
+                const int first_chunk = TWO ? 0 : group * mine;
+                const std::uint16_t* from = a.query + g.list_entry * a.query_batch + node * a.query_node +
+                                            query_head * a.query_head;
+                unsigned char* to = smem + (TWO ? group * L::operand_bytes : 0) + row * 128;
+#pragma unroll 4
+                for (int c = 0; c < mine; ++c)
+                {
+                    const int chunk = first_chunk + c;
+                    uint4 v = live ? *reinterpret_cast<const uint4*>(from + 8 * chunk) : make_uint4(0, 0, 0, 0);
+                    v = make_uint4(v.x ^ turn, v.y ^ turn, v.z ^ turn, v.w ^ turn);
+                    *reinterpret_cast<uint4*>(to + (chunk >> 3) * L::panel_bytes + (((chunk & 7) ^ (row & 7)) << 4)) = v;
+                }
+                fence_async_proxy();
+                bar_arrive(smem_u32(&tail.query));
+            }
+            if (has_draft)
+                ancestor_masks(a.parents + static_cast<long long>(g.list_entry) * a.max_nodes, g.e.nodes, tail.masks,
+                               tail.above, group == 0 && warp < 2 ? a.error_word : nullptr, t, [] { softmax_sync(); });
+            const unsigned long long sees = has_draft && live ? tail.masks[node] : 0ull;
+
+            float maximum = -INFINITY, sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int j = TWO ? 0 : group; j < tiles; j += TWO ? 1 : 2)
+            {
+                const int tile = g.tile_begin + j;
+                const bool drafted = tile == g.e.tiles - 1;
+                const int held = drafted ? 0 : g.e.length - tile * KEYS;
+                const bool masked = held < KEYS;
+                // Keys 32 c to 32 c + 31 that this row sees, one bit each.
+                const auto visible = [&](int c) -> uint32_t
+                {
+                    if (drafted)
+                        return c == 0 ? static_cast<uint32_t>(sees) : (c == 1 ? static_cast<uint32_t>(sees >> 32) : 0u);
+                    const int n = held - 32 * c;
+                    return n >= 32 ? ~0u : (n <= 0 ? 0u : (1u << n) - 1u);
+                };
+                wait(tail.scores[group], scores_seen++);
+                __syncwarp();
+                tc_fence_after();
+                float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                for (int c = 0; c < KEYS / 32; ++c)
+                {
+                    uint32_t s[32];
+                    tmem_load32(my_scores + 32 * c, s);
+                    tmem_wait_loads();
+                    if (masked)
+                    {
+                        const uint32_t bits = visible(c);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            best[k & 3] = fmaxf(best[k & 3], bits >> k & 1u ? __uint_as_float(s[k]) : -INFINITY);
+                    }
+                    else
+                    {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            best[k & 3] = fmaxf(best[k & 3], __uint_as_float(s[k]));
+                    }
+                }
+                const float highest = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+                const float top = highest == -INFINITY ? -INFINITY : highest * scale;
+                const bool first = TWO ? j == 0 : j < 2;
+                if (first)
+                {
+                    maximum = top;
+                }
+                else if (__any_sync(0xffffffffu, top > maximum + RESCALE))
+                {
+                    const float raised = fmaxf(maximum, top);
+                    const float shrink = maximum == -INFINITY ? 0.0f : power_of_two(maximum - raised);
+                    maximum = raised;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        sums[k] *= shrink;
+                    // The product before these scores is complete: they were issued after it.
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c)
+                    {
+                        uint32_t o[32];
+                        tmem_load32(my_output + 32 * c, o);
+                        tmem_wait_loads();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
+                        tmem_store16(my_output + 32 * c, o);
+                        tmem_store16(my_output + 32 * c + 16, o + 16);
+                    }
+                }
+                const float shift = maximum == -INFINITY ? 0.0f : -maximum;
+#pragma unroll 1
+                for (int c = 0; c < KEYS / 32; ++c)
+                {
+                    uint32_t s[32], p[16];
+                    tmem_load32(my_scores + 32 * c, s);
+                    tmem_wait_loads();
+                    const uint32_t bits = masked ? visible(c) : ~0u;
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2)
+                    {
+                        float x = power_of_two(fmaf(__uint_as_float(s[k]), scale, shift));
+                        float y = power_of_two(fmaf(__uint_as_float(s[k + 1]), scale, shift));
+                        if (masked)
+                        {
+                            x = bits >> k & 1u ? x : 0.0f;
+                            y = bits >> (k + 1) & 1u ? y : 0.0f;
+                        }
+                        sums[k & 3] += x;
+                        sums[(k & 3) + 1] += y;
+                        p[k / 2] = Half2<T>::pack(x, y);
+                    }
+                    tmem_store16(my_scores + 16 * c, p); // over scores that have been read
+                }
+                tmem_wait_stores();
+                tc_fence_before();
+                bar_arrive(smem_u32(&tail.weights[group]));
+            }
+            // ------------------------------------------------------- epilogue --
+            const Both<int> made{TWO ? tiles : (tiles + 1) / 2, TWO ? tiles : tiles / 2};
+            float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+            if (made(group))
+                wait(tail.products[group], products_seen(group) + made(group) - 1);
+            Both<float> part{1.0f, 1.0f}; // factors of the groups' outputs
+            if constexpr (!TWO)
+            {
+                tail.maximum[group][row] = maximum;
+                tail.sum[group][row] = sum;
+                softmax_sync();
+                // The other group has seen its product complete; this makes it visible here.
+                if (made(1 - group))
+                    wait(tail.products[1 - group], products_seen(1 - group) + made(1 - group) - 1);
+                const float m0 = tail.maximum[0][row], m1 = tail.maximum[1][row];
+                maximum = fmaxf(m0, m1);
+                part.first = m0 == -INFINITY ? 0.0f : power_of_two(m0 - maximum);
+                part.second = m1 == -INFINITY ? 0.0f : power_of_two(m1 - maximum);
+                sum = tail.sum[0][row] * part.first + tail.sum[1][row] * part.second;
+            }
+            __syncwarp();
+            tc_fence_after();
+            products_seen.first += made.first;
+            products_seen.second += made.second;
+            const unsigned long long tainted = has_draft ? tail.tainted[segment % TAINT_SLOTS] : 0ull;
+            const int draft_group = TWO ? group : (tiles - 1) & 1; // whose P is the drafted tile's
+            const bool whole = g.tile_begin == 0 && has_draft;
+            // A piece that begins its item goes to the CTA's second place, any other to its first.
+            float* piece = pieces + (2ll * cta + (g.tile_begin == 0)) * tree_piece_floats(L::ROWS, D) +
+                           item_row * (D + TREE_PIECE_HEAD);
+            std::uint16_t* out = a.out + g.list_entry * a.out_batch + node * a.out_node + query_head * a.out_head;
+            const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum; // a row that sees nothing gives zeros
+            constexpr int columns = TWO ? D : D / 2;                  // of this thread
+            const int first_column = TWO ? 0 : group * columns;
+            constexpr int step = TWO ? 32 : 16;
+#pragma unroll 1
+            for (int c = 0; c < columns; c += step)
+            {
+                const int column = first_column + c;
+                uint32_t o[step];
+                if constexpr (TWO)
+                {
+                    tmem_load32(my_output + column, o);
+                    tmem_wait_loads();
+                }
+                else
+                {
+                    uint32_t other[step];
+                    tmem_load16(lanes + OUTPUT_COLUMN + column, o); // the first group always has a tile
+                    if (made.second)
+                        tmem_load16(lanes + OUTPUT_COLUMN + 128 + column, other);
+                    tmem_wait_loads();
+#pragma unroll
+                    for (int k = 0; k < step; ++k)
+                    {
+                        float x = __uint_as_float(o[k]) * part.first;
+                        if (made.second)
+                            x = fmaf(__uint_as_float(other[k]), part.second, x);
+                        o[k] = __float_as_uint(x);
+                    }
+                }
+                for (unsigned long long rest = tainted; rest; rest &= rest - 1)
+                {
+                    const int key = __ffsll(static_cast<long long>(rest)) - 1;
+                    const uint32_t pair = tmem_load1(lanes + draft_group * KEYS + key / 2);
+                    tmem_wait_loads();
+                    const long long offset = sees >> key & 1ull ? Work::key_row(a, g, g.e.tiles - 1, key) : -1;
+                    if (offset >= 0)
+                    {
+                        const float weight = Half2<T>::value(static_cast<std::uint16_t>(key & 1 ? pair >> 16 : pair)) *
+                                             part(TWO ? 0 : draft_group);
+                        const auto* values = reinterpret_cast<const std::uint16_t*>(plane + a.cache.plane_bytes + offset) + column;
+#pragma unroll
+                        for (int k = 0; k < step; ++k)
+                            if (nonfinite_mask<T>(values[k]) & 0xffffu)
+                                o[k] = __float_as_uint(fmaf(weight, Half2<T>::value(values[k]), __uint_as_float(o[k])));
+                    }
+                    __syncwarp();
+                }
+                if (live && whole)
+                {
+#pragma unroll
+                    for (int k = 0; k < step; k += 8)
+                    {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            w[j] = Half2<T>::pack(__uint_as_float(o[k + 2 * j]) * inverse,
+                                                  __uint_as_float(o[k + 2 * j + 1]) * inverse);
+                        *reinterpret_cast<uint4*>(out + column + k) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                else if (live)
+                {
+#pragma unroll
+                    for (int k = 0; k < step; k += 4)
+                        *reinterpret_cast<uint4*>(piece + TREE_PIECE_HEAD + column + k) =
+                            make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                }
+                __syncwarp();
+            }
+            if (live && first_column == 0)
+            {
+                if (!whole)
+                {
+                    piece[0] = maximum;
+                    piece[1] = sum;
+                }
+                else if (a.lse)
+                {
+                    a.lse[(static_cast<long long>(g.list_entry) * a.max_nodes + node) * a.heads * a.group + query_head] =
+                        sum == 0.0f ? -INFINITY : (maximum + log2f(sum)) * 0.6931471805599453f;
+                }
+            }
+            if (g.tile_begin == 0 && !whole && t == 0)
+                shared_items[cta] = TreeShared{g.list_entry, g.head, g.first_row,
+                                               Work::owner(start.units, g.item_start + g.e.tiles - 1, start.ctas) - cta + 1,
+                                               g.e.nodes};
+            tc_fence_before();
+            softmax_sync(); // outputs, masks and statistics of this segment are done with
+            if (t == 0)
+                tail.tainted[segment % TAINT_SLOTS] = 0;
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == MMA_WARP)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLUMNS));
+}
+
+template <class T, int D, bool TWO>
+void launch(const TreeArgs& a, float* pieces, TreeShared* shared_items, cudaStream_t stream)
+{
+    using L = Tiles<D, TWO>;
+    static std::once_flag once[64];
+    int device = 0;
+    cudaGetDevice(&device);
+    if (device >= 0 && device < 64)
+        std::call_once(once[device],
+                       []
+                       {
+                           cudaFuncSetAttribute(tree_attention_tc_kernel<T, D, TWO>,
+                                                cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem);
+                       });
+    launch_pdl(tree_attention_tc_kernel<T, D, TWO>, dim3(sm_count()), dim3(THREADS), L::smem, stream, a, pieces,
+               shared_items);
+    note_launch();
+}
+
+template <class T>
+void launch_shape(const TreeArgs& a, float* pieces, TreeShared* shared_items, cudaStream_t stream)
+{
+    const bool two = tree_attention_tc_rows(a.max_nodes * a.group) == 256;
+    if (a.head_dim == 64)
+        two ? launch<T, 64, true>(a, pieces, shared_items, stream) : launch<T, 64, false>(a, pieces, shared_items, stream);
+    else
+        two ? launch<T, 128, true>(a, pieces, shared_items, stream) : launch<T, 128, false>(a, pieces, shared_items, stream);
+}
+} // namespace
+
+int tree_attention_tc_rows(int rows)
+{
+    return rows > 128 ? 256 : 128;
+}
+
+cudaError_t tree_attention_tc(const TreeArgs& a, ValueType type, float* pieces, TreeShared* shared_items,
+                              cudaStream_t stream)
+{
+    if (type == ValueType::bf16)
+        launch_shape<__nv_bfloat16>(a, pieces, shared_items, stream);
+    else
+        launch_shape<__half>(a, pieces, shared_items, stream);
+    return cudaGetLastError();
+}
+} // namespace tsacb::dev
