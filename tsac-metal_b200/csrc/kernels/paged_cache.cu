@@ -403,48 +403,78 @@ __global__ void __launch_bounds__(256)
 }
 
 // ------------------------------------------------------------------- append --
-// One thread per 16-byte chunk of a key or value row; neighbouring threads
-// take neighbouring chunks, so reads and writes are whole rows.  HBM-bound; a
-// row is written only into a page that its sequence holds alone.
-__global__ void __launch_bounds__(256)
-    cache_append_kernel(CacheView c, int layer, AppendRows rows, const int* sequences,
-                        const int* nodes, const int* starts, int max_nodes,
-                        long long row_count, unsigned* error_word)
+// One warp per row (its keys and its values), a lane per 16-byte chunk.  The
+// row's chunks are loaded before its page is looked up (length, count, table,
+// reference count: four dependent reads of L2), so that the two latencies
+// overlap.  A row is written only into a page that its sequence holds alone.
+constexpr int APPEND_WARPS = 4, APPEND_CHUNKS = 4; // chunks of keys and of values in flight per lane
+
+__global__ void __launch_bounds__(APPEND_WARPS * 32)
+    cache_append_kernel(CacheView c, int layer, AppendRows rows, const int* sequences, const int* nodes,
+                        const int* starts, int max_nodes, long long row_count, unsigned* error_word)
 {
     pdl_prologue();
+    const int lane = threadIdx.x & 31;
     const int row_chunks = rows.heads * rows.head_chunks;
-    const int value = blockIdx.y;
-    const long long all = row_count * row_chunks;
-    for (long long at = blockIdx.x * 256ll + threadIdx.x; at < all; at += gridDim.x * 256ll)
+    for (long long row = blockIdx.x * static_cast<long long>(APPEND_WARPS) + (threadIdx.x >> 5); row < row_count;
+         row += static_cast<long long>(gridDim.x) * APPEND_WARPS)
     {
-        const long long row = at / row_chunks;
-        const int chunk = static_cast<int>(at - row * row_chunks);
-        const int i = static_cast<int>(row / max_nodes), n = static_cast<int>(row - static_cast<long long>(i) * max_nodes);
+        // 32-bit division where it serves: the 64-bit one is a long routine.
+        const int i = row <= 0x7fffffff ? static_cast<int>(static_cast<unsigned>(row) / static_cast<unsigned>(max_nodes))
+                                        : static_cast<int>(row / max_nodes);
+        const int n = static_cast<int>(row - static_cast<long long>(i) * max_nodes);
         if (nodes && n >= nodes[i])
             continue;
-        const int sequence = cache_sequence(c, sequences, i);
-        int page = -1;
-        long long position = -1;
-        if (sequence >= 0)
+        const auto load = [&](int value, int chunk)
         {
-            const int start = starts ? starts[i] : c.lengths[sequence];
-            position = static_cast<long long>(start) + n;
-            if (start >= 0)
-                page = cache_page(c, sequence, cache_held(c, sequence),
-                                  static_cast<int>(position >> c.page_shift));
-        }
-        if (page < 0 || c.refs[page] != 1)
+            const int head = chunk / rows.head_chunks, part = chunk - head * rows.head_chunks;
+            return __ldcs(reinterpret_cast<const uint4*>(rows.source[value] + i * rows.batch_bytes[value] +
+                                                         n * rows.node_bytes[value] + head * rows.head_bytes[value]) +
+                          part);
+        };
+        uint4* place[2] = {nullptr, nullptr};
+        for (int first = lane; first - lane < row_chunks; first += 32 * APPEND_CHUNKS)
         {
-            if (chunk == 0)
-                raise(error_word, error_cache);
-            continue;
+            uint4 v[2][APPEND_CHUNKS];
+#pragma unroll
+            for (int k = 0; k < APPEND_CHUNKS; ++k)
+                if (first + 32 * k < row_chunks)
+                {
+                    v[0][k] = load(0, first + 32 * k);
+                    v[1][k] = load(1, first + 32 * k);
+                }
+            if (first == lane)
+            {
+                const int sequence = cache_sequence(c, sequences, i);
+                int page = -1;
+                long long position = -1;
+                if (sequence >= 0)
+                {
+                    const int start = starts ? starts[i] : c.lengths[sequence];
+                    position = static_cast<long long>(start) + n;
+                    if (start >= 0)
+                        page = cache_page(c, sequence, cache_held(c, sequence),
+                                          static_cast<int>(position >> c.page_shift));
+                }
+                if (page < 0 || c.refs[page] != 1)
+                {
+                    if (lane == 0)
+                        raise(error_word, error_cache);
+                    break;
+                }
+                unsigned char* to = c.pool + 2ll * layer * c.plane_bytes + page * c.page_bytes() +
+                                    (position & (c.page_size() - 1)) * c.row_bytes;
+                place[0] = reinterpret_cast<uint4*>(to);
+                place[1] = reinterpret_cast<uint4*>(to + c.plane_bytes);
+            }
+#pragma unroll
+            for (int k = 0; k < APPEND_CHUNKS; ++k)
+                if (first + 32 * k < row_chunks)
+                {
+                    place[0][first + 32 * k] = v[0][k];
+                    place[1][first + 32 * k] = v[1][k];
+                }
         }
-        const int head = chunk / rows.head_chunks, part = chunk - head * rows.head_chunks;
-        const auto* from = reinterpret_cast<const uint4*>(rows.source[value] + i * rows.batch_bytes[value] +
-                                                          n * rows.node_bytes[value] + head * rows.head_bytes[value]) + part;
-        unsigned char* to = c.pool + (2ll * layer + value) * c.plane_bytes + page * c.page_bytes() +
-                            (position & (c.page_size() - 1)) * c.row_bytes;
-        reinterpret_cast<uint4*>(to)[chunk] = __ldcs(from);
     }
 }
 
@@ -676,10 +706,10 @@ void cache_append(const CacheView& c, int layer, const AppendRows& rows, const i
                   const int* starts, int count, int max_nodes, unsigned* error_word, cudaStream_t stream)
 {
     const long long row_count = static_cast<long long>(count) * max_nodes;
-    const long long blocks = (row_count * rows.heads * rows.head_chunks + 255) / 256;
-    const int grid = static_cast<int>(blocks < copy_grid() ? blocks : copy_grid());
-    launch_pdl(cache_append_kernel, dim3(grid, 2), dim3(256), 0, stream, c, layer, rows, sequences, nodes, starts,
-               max_nodes, row_count, error_word);
+    const long long blocks = (row_count + APPEND_WARPS - 1) / APPEND_WARPS;
+    const int grid = static_cast<int>(blocks < 2 * copy_grid() ? blocks : 2 * copy_grid());
+    launch_pdl(cache_append_kernel, dim3(grid), dim3(APPEND_WARPS * 32), 0, stream, c, layer, rows, sequences, nodes,
+               starts, max_nodes, row_count, error_word);
     note_launch();
 }
 

@@ -182,43 +182,74 @@ def _drafting():
     return _drafting_lib
 
 
+def _raw_stream(index):
+    """Handle of the current stream of device `index`, by torch's direct query where it has one."""
+    import torch
+    query = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return query or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 class _Device:
     """Makes a tensor's device current for a call, and gives its current stream."""
 
-    def __init__(self, device):
+    _known = {}
+
+    def __init__(self, index):
         import torch
-        self._torch, self.index = torch, device.index
+        self.index, self._cuda, self._stream = index, torch.cuda, _raw_stream(index)
+
+    @classmethod
+    def of(cls, index):
+        on = cls._known.get(index)
+        if on is None:
+            on = cls._known[index] = cls(index)
+        return on
 
     def stream(self) -> int:
-        return self._torch.cuda.current_stream(self.index).cuda_stream
+        return self._stream(self.index)
 
     def call(self, fn, *arguments) -> None:
-        cuda = self._torch.cuda
-        if cuda.current_device() == self.index:
+        if self._cuda.current_device() == self.index:
             status = fn(*arguments)
         else:
-            with cuda.device(self.index):
+            with self._cuda.device(self.index):
                 status = fn(*arguments)
         if status != OK:
             check(status)
 
 
-def _whole(t, name, dtype, device, shape=None):
-    """Address of a contiguous tensor of the given kind; None gives a null pointer."""
+def _whole(t, name, dtype, index, shape=None):
+    """Address of a contiguous tensor of the given kind on device `index`; None gives a null pointer."""
     if t is None:
         return None
-    if t.dtype != dtype or t.device != device or not t.is_contiguous() or (shape is not None and t.shape != shape):
-        raise TsacError(f"{name} must be a contiguous {dtype} tensor on {device}"
+    if t.dtype is not dtype or t.get_device() != index or not t.is_contiguous() or (shape is not None and t.shape != shape):
+        raise TsacError(f"{name} must be a contiguous {dtype} tensor on cuda:{index}"
                         + (f" of shape {tuple(shape)}" if shape is not None else ""))
     return t.data_ptr()
 
 
-def _rows(t, name, dtype, device, shape):
+_stride_arrays = {}
+
+
+def _strides(values):
+    """A C array of strides, kept for the next call with the same ones."""
+    array = _stride_arrays.get(values)
+    if array is None:
+        if len(_stride_arrays) >= 1024:
+            _stride_arrays.clear()
+        array = _stride_arrays[values] = (ctypes.c_ssize_t * len(values))(*values)
+    return array
+
+
+def _rows(t, name, dtype, index, shape):
     """Address and strides of a [entry][node][head][dim] tensor with a contiguous last dimension."""
-    if t.dtype != dtype or t.device != device or t.shape != shape or (shape[-1] > 1 and t.stride(3) != 1):
-        raise TsacError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on {device}, its last dimension contiguous")
-    # A dimension of size one is never stepped over: its stride says nothing.
-    return t.data_ptr(), (ctypes.c_ssize_t * 3)(*[t.stride(k) if shape[k] > 1 else 0 for k in range(3)])
+    strides = t.stride()
+    if t.dtype is not dtype or t.get_device() != index or t.shape != shape or (strides[-1] != 1 and shape[-1] > 1):
+        raise TsacError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on cuda:{index}, its last dimension contiguous")
+    strides = strides[:3]
+    if 1 in shape:  # a dimension of size one is never stepped over: its stride says nothing
+        strides = tuple(0 if n == 1 else s for n, s in zip(shape, strides))
+    return t.data_ptr(), _strides(strides)
 
 
 class PagedCache:
@@ -235,22 +266,22 @@ class PagedCache:
         if pool.dim() != 6 or pool.shape[1] != 2 or not pool.is_cuda or pool.dtype not in (torch.bfloat16, torch.float16):
             raise TsacError("pool must be a bf16 or fp16 CUDA tensor [layers][2][pages][page_size][kv_heads][head_dim]")
         self.pool, self.tables, self.counts, self.lengths, self.refs = pool, tables, counts, lengths, refs
-        self.device, self.dtype = pool.device, pool.dtype
+        self.device, self.index, self.dtype = pool.device, pool.get_device(), pool.dtype
         self._torch, self._int = torch, torch.int32
         if tables.dim() != 2:
             raise TsacError("tables must be [sequences][max_pages]")
         self.layers, _, self.pages, self.page_size, self.kv_heads, self.head_dim = pool.shape
         self.sequences, self.max_pages = tables.shape
         s = _PagedCacheStruct()
-        s.pool = _whole(pool, "pool", pool.dtype, self.device)
-        s.tables = _whole(tables, "tables", self._int, self.device)
-        s.counts = _whole(counts, "counts", self._int, self.device, (self.sequences,))
-        s.lengths = _whole(lengths, "lengths", self._int, self.device, (self.sequences,))
-        s.refs = _whole(refs, "refs", self._int, self.device, (self.pages,))
+        s.pool = _whole(pool, "pool", pool.dtype, self.index)
+        s.tables = _whole(tables, "tables", self._int, self.index)
+        s.counts = _whole(counts, "counts", self._int, self.index, (self.sequences,))
+        s.lengths = _whole(lengths, "lengths", self._int, self.index, (self.sequences,))
+        s.refs = _whole(refs, "refs", self._int, self.index, (self.pages,))
         for name in ("layers", "pages", "page_size", "kv_heads", "head_dim", "sequences", "max_pages"):
             setattr(s, name, getattr(self, name))
         s.type = 0 if pool.dtype == torch.bfloat16 else 1
-        self._struct, self._lib, self._on = s, _drafting(), _Device(self.device)
+        self._struct, self._lib, self._on = s, _drafting(), _Device.of(self.index)
         self._cache = ctypes.addressof(s)
 
     @classmethod
@@ -263,14 +294,14 @@ class PagedCache:
                    torch.zeros(sequences, **ints), torch.zeros(pages, **ints))
 
     def _list(self, sequences, count):
-        return _whole(sequences, "sequences", self._int, self.device, (count,))
+        return _whole(sequences, "sequences", self._int, self.index, (count,))
 
     def _word(self, error_word):
         if error_word is None:
             return None
         if error_word.numel() < 1 or error_word.element_size() != 4:
             raise TsacError("error_word must hold a 32-bit word")
-        return _whole(error_word, "error_word", error_word.dtype, self.device)
+        return _whole(error_word, "error_word", error_word.dtype, self.index)
 
     def _scratch(self, nbytes):
         return self._torch.empty(max(nbytes, 16), dtype=self._torch.uint8, device=self.device)
@@ -282,33 +313,33 @@ class PagedCache:
         nbytes = self._lib.tsac_cuda_cache_reserve_scratch_bytes(count, slots)
         scratch = self._scratch(nbytes)
         self._on.call(self._lib.tsac_cuda_cache_reserve, self._cache, self._list(sequences, count),
-                      _whole(positions, "positions", self._int, self.device, (count,)), count, slots,
+                      _whole(positions, "positions", self._int, self.index, (count,)), count, slots,
                       scratch.data_ptr(), scratch.numel(), self._word(error_word), self._on.stream())
 
     def fork(self, parents, children, error_word=None):
         """children[i], empty so far, shares the committed pages of parents[i]."""
         count = parents.shape[0]
         self._on.call(self._lib.tsac_cuda_cache_fork, self._cache,
-                      _whole(parents, "parents", self._int, self.device, (count,)),
-                      _whole(children, "children", self._int, self.device, (count,)), count,
+                      _whole(parents, "parents", self._int, self.index, (count,)),
+                      _whole(children, "children", self._int, self.index, (count,)), count,
                       self._word(error_word), self._on.stream())
 
     def release(self, sequences=None, positions=None, error_word=None):
         """Gives back the pages behind positions[i] (None: all) of each sequence."""
         count = sequences.shape[0] if sequences is not None else self.sequences
         self._on.call(self._lib.tsac_cuda_cache_release, self._cache, self._list(sequences, count),
-                      _whole(positions, "positions", self._int, self.device, (count,)), count,
+                      _whole(positions, "positions", self._int, self.index, (count,)), count,
                       self._word(error_word), self._on.stream())
 
     def append(self, layer, keys, values, nodes=None, sequences=None, starts=None, error_word=None):
         """Stores [entry][node][kv_heads][head_dim] rows of one layer behind each sequence's length (or at starts)."""
         count, most = keys.shape[:2]
         shape = (count, most, self.kv_heads, self.head_dim)
-        k, key_strides = _rows(keys, "keys", self.dtype, self.device, shape)
-        v, value_strides = _rows(values, "values", self.dtype, self.device, shape)
+        k, key_strides = _rows(keys, "keys", self.dtype, self.index, shape)
+        v, value_strides = _rows(values, "values", self.dtype, self.index, shape)
         self._on.call(self._lib.tsac_cuda_cache_append, self._cache, layer, k, key_strides, v, value_strides,
-                      self._list(sequences, count), _whole(nodes, "nodes", self._int, self.device, (count,)),
-                      _whole(starts, "starts", self._int, self.device, (count,)), count, most,
+                      self._list(sequences, count), _whole(nodes, "nodes", self._int, self.index, (count,)),
+                      _whole(starts, "starts", self._int, self.index, (count,)), count, most,
                       self._word(error_word), self._on.stream())
 
     def keep(self, path, accepted, starts=None, lengths_out=None, sequences=None, error_word=None):
@@ -316,10 +347,10 @@ class PagedCache:
         count, width = path.shape
         out = self.lengths if lengths_out is None else lengths_out
         self._on.call(self._lib.tsac_cuda_cache_keep, self._cache, self._list(sequences, count),
-                      _whole(path, "path", self._int, self.device),
-                      _whole(accepted, "accepted", self._int, self.device, (count,)),
-                      _whole(starts, "starts", self._int, self.device, (count,)),
-                      _whole(out, "lengths_out", self._int, self.device, (self.sequences,)), count, width,
+                      _whole(path, "path", self._int, self.index),
+                      _whole(accepted, "accepted", self._int, self.index, (count,)),
+                      _whole(starts, "starts", self._int, self.index, (count,)),
+                      _whole(out, "lengths_out", self._int, self.index, (self.sequences,)), count, width,
                       self._word(error_word), self._on.stream())
 
     def compact(self, tables_out=None, refs_out=None, live=None, error_word=None):
@@ -327,10 +358,10 @@ class PagedCache:
         live = self._torch.empty(1, dtype=self._int, device=self.device) if live is None else live
         scratch = self._scratch(self._lib.tsac_cuda_cache_compact_scratch_bytes(self.pages))
         self._on.call(self._lib.tsac_cuda_cache_compact, self._cache,
-                      _whole(self.tables if tables_out is None else tables_out, "tables_out", self._int, self.device,
+                      _whole(self.tables if tables_out is None else tables_out, "tables_out", self._int, self.index,
                              self.tables.shape),
-                      _whole(self.refs if refs_out is None else refs_out, "refs_out", self._int, self.device, (self.pages,)),
-                      _whole(live, "live", self._int, self.device, (1,)), scratch.data_ptr(), scratch.numel(),
+                      _whole(self.refs if refs_out is None else refs_out, "refs_out", self._int, self.index, (self.pages,)),
+                      _whole(live, "live", self._int, self.index, (1,)), scratch.data_ptr(), scratch.numel(),
                       self._word(error_word), self._on.stream())
         return live
 
@@ -343,13 +374,13 @@ class PagedCache:
         count, most, heads, _ = query.shape
         shape = (count, most, heads, self.head_dim)
         out = torch.empty(shape, dtype=self.dtype, device=self.device) if out is None else out
-        q, query_strides = _rows(query, "query", self.dtype, self.device, shape)
-        o, out_strides = _rows(out, "out", self.dtype, self.device, shape)
+        q, query_strides = _rows(query, "query", self.dtype, self.index, shape)
+        o, out_strides = _rows(out, "out", self.dtype, self.index, shape)
         scratch = self._scratch(self._lib.tsac_cuda_tree_attention_scratch_bytes(self._cache, heads, most))
         self._on.call(self._lib.tsac_cuda_tree_attention, self._cache, layer, self._list(sequences, count),
-                      _whole(parents, "parents", self._int, self.device, (count, most)),
-                      _whole(nodes, "nodes", self._int, self.device, (count,)), q, query_strides, o, out_strides,
-                      _whole(lse, "lse", torch.float32, self.device, (count, most, heads)), heads, count, most,
+                      _whole(parents, "parents", self._int, self.index, (count, most)),
+                      _whole(nodes, "nodes", self._int, self.index, (count,)), q, query_strides, o, out_strides,
+                      _whole(lse, "lse", torch.float32, self.index, (count, most, heads)), heads, count, most,
                       self.head_dim ** -0.5 if scale is None else scale, scratch.data_ptr(), scratch.numel(),
                       self._word(error_word), self._on.stream())
         return out
@@ -367,28 +398,28 @@ def draft_verify(target, tokens, parents, coins, draws, draft=None, nodes=None, 
     if target.dim() != 3 or not target.is_cuda:
         raise TsacError("target must be a CUDA tensor [batch][nodes][vocab]")
     types = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-    batch, most, vocab = target.shape
-    device, kind = target.device, target.dtype
+    shape = target.shape
+    batch, most, vocab = shape
+    index, kind = target.get_device(), target.dtype
     for name, t in (("target", target), ("draft", draft)):
-        if t is not None and (t.dtype not in types or t.dtype != kind or t.device != device or t.shape != target.shape
+        if t is not None and (kind not in types or t.dtype is not kind or t.get_device() != index or t.shape != shape
                               or (vocab > 1 and t.stride(2) != 1)):
             raise TsacError(f"{name} must be bf16, fp16 or fp32 [batch][nodes][vocab], the vocabulary contiguous")
-    strides = (ctypes.c_ssize_t * 2)(target.stride(0), target.stride(1))
-    draft_strides = (ctypes.c_ssize_t * 2)(draft.stride(0), draft.stride(1)) if draft is not None else None
+    ints, floats, rows, ones = torch.int32, torch.float32, (batch, most), (batch,)
     if out is None:
-        out = (torch.empty(batch, dtype=torch.int32, device=device), torch.empty((batch, most), dtype=torch.int32, device=device),
-               torch.empty(batch, dtype=torch.int32, device=device))
+        device = target.device
+        out = (torch.empty(batch, dtype=ints, device=device), torch.empty(rows, dtype=ints, device=device),
+               torch.empty(batch, dtype=ints, device=device))
     accepted, path, token = out
-    word = None if error_word is None else _whole(error_word, "error_word", error_word.dtype, device)
-    on = _Device(device)
-    on.call(lib.tsac_cuda_draft_verify, target.data_ptr(), strides, draft.data_ptr() if draft is not None else None,
-            draft_strides, types[kind], _whole(tokens, "tokens", torch.int32, device, (batch, most)),
-            _whole(parents, "parents", torch.int32, device, (batch, most)),
-            _whole(coins, "coins", torch.float32, device, (batch, most)),
-            _whole(draws, "draws", torch.float32, device, (batch,)),
-            _whole(nodes, "nodes", torch.int32, device, (batch,)), batch, most, vocab,
-            _whole(accepted, "accepted", torch.int32, device, (batch,)), _whole(path, "path", torch.int32, device, (batch, most)),
-            _whole(token, "token", torch.int32, device, (batch,)), word, on.stream())
+    word = None if error_word is None else _whole(error_word, "error_word", error_word.dtype, index)
+    on = _Device.of(index)
+    on.call(lib.tsac_cuda_draft_verify, target.data_ptr(), _strides(target.stride()[:2]),
+            None if draft is None else draft.data_ptr(), None if draft is None else _strides(draft.stride()[:2]), types[kind],
+            _whole(tokens, "tokens", ints, index, rows), _whole(parents, "parents", ints, index, rows),
+            _whole(coins, "coins", floats, index, rows), _whole(draws, "draws", floats, index, ones),
+            _whole(nodes, "nodes", ints, index, ones), batch, most, vocab,
+            _whole(accepted, "accepted", ints, index, ones), _whole(path, "path", ints, index, rows),
+            _whole(token, "token", ints, index, ones), word, on.stream())
     return accepted, path, token
 
 
