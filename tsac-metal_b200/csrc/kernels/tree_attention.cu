@@ -170,13 +170,15 @@ __global__ void __launch_bounds__(THREADS, 2)
                     Half2<T>::mma(s[m][1], q[m][k], b[2], b[3]);
                 }
             }
-            const bool drafted = tile == e.tiles - 1;
-            const int in_tile = warp * WARP_KEYS + 2 * (lane & 3); // this lane's first key
-            const int held = drafted ? e.nodes : e.length - tile * KEYS;
+            const bool last = Work::is_last(g, tile);
+            const bool masked = Work::is_masked(g, tile);
+            // The warp's keys are bits `first_bit` to + 15 of the 32 that `visible` gives.
+            const int first_bit = (warp * WARP_KEYS) & 31;
+            const int first_node = Work::base(g, tile) + warp * WARP_KEYS - e.length; // of the warp's first key, if drafted
             unsigned tainted = 0; // drafted rows with a value that is not finite
-            if (drafted && warp * WARP_KEYS < e.nodes)
+            if (last && first_node > -WARP_KEYS && first_node < e.nodes)
             {
-                for (int row = 0; row < WARP_KEYS; ++row)
+                for (int row = max(0, -first_node); row < WARP_KEYS; ++row)
                 {
                     bool odd = false;
                     if (lane < L::chunks)
@@ -199,19 +201,19 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
                 {
-                    unsigned long long sees = ~0ull;
-                    if (drafted)
+                    std::uint32_t sees = ~0u;
+                    if (masked)
                     {
                         const int row = first_row + 16 * m + 8 * r + (lane >> 2);
-                        sees = row < rows ? masks[row / a.group] : 0ull;
+                        sees = Work::visible(g, tile, warp * WARP_KEYS / 32, last && row < rows ? masks[row / a.group] : 0ull) >>
+                               (first_bit + 2 * (lane & 3)); // this lane's keys: bits 0, 1, 8, 9
                     }
                     float z[4], best = top[m][r];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) // keys in_tile, + 1, + 8, + 9
+                    for (int k = 0; k < 4; ++k)
                     {
-                        const int key = in_tile + (k & 1) + 8 * (k >> 1);
                         z[k] = s[m][k >> 1][2 * r + (k & 1)] * a.scale_log2;
-                        if (key >= held || !(sees >> key & 1ull))
+                        if (!(sees >> ((k & 1) + 8 * (k >> 1)) & 1u))
                             z[k] = -INFINITY;
                         best = fmaxf(best, z[k]);
                     }
@@ -257,7 +259,7 @@ __global__ void __launch_bounds__(THREADS, 2)
                         for (int r = 0; r < 2; ++r)
                         {
                             const int row = first_row + 16 * m + 8 * r + (lane >> 2);
-                            const bool seen = row < rows && (masks[row / a.group] >> (warp * WARP_KEYS + key) & 1ull);
+                            const bool seen = row < rows && (masks[row / a.group] >> (first_node + key) & 1ull);
                             float weight = 0.0f;
 #pragma unroll
                             for (int kk = 0; kk < 4; ++kk)

@@ -43,6 +43,7 @@ template <int KEYS, int ROWS> struct TreeWork
     struct Entry
     {
         int sequence, held, length, nodes, tiles, row_items;
+        int last_base; // first position of the last tile
         long long units;
     };
 
@@ -53,7 +54,7 @@ template <int KEYS, int ROWS> struct TreeWork
         e.sequence = cache_sequence(a.cache, a.sequences, i);
         e.nodes = a.nodes ? a.nodes[i] : a.max_nodes;
         e.nodes = e.nodes < a.max_nodes ? e.nodes : a.max_nodes;
-        e.units = e.tiles = e.row_items = e.length = e.held = 0;
+        e.units = e.tiles = e.row_items = e.length = e.held = e.last_base = 0;
         if (e.nodes <= 0)
             return e;
         bool valid = e.sequence >= 0;
@@ -70,7 +71,10 @@ template <int KEYS, int ROWS> struct TreeWork
                 atomicOr(a.error_word, error_cache);
             return e;
         }
-        e.tiles = (e.length + KEYS - 1) / KEYS + 1;
+        // 64 nodes behind a multiple of 64 fit in a tile of 128, whose boxes then start on that multiple.
+        const int behind = e.length % KEYS;
+        e.last_base = e.length - (behind + e.nodes <= KEYS ? behind : e.length % (KEYS > 64 ? KEYS - 64 : 1));
+        e.tiles = (e.last_base + KEYS - 1) / KEYS + 1;
         e.row_items = (e.nodes * a.group + ROWS - 1) / ROWS;
         e.units = static_cast<long long>(e.tiles) * e.row_items * a.heads;
         return e;
@@ -190,14 +194,39 @@ template <int KEYS, int ROWS> struct TreeWork
         }
     };
 
+    static __device__ __forceinline__ bool is_last(const Segment& s, int tile) { return tile == s.e.tiles - 1; }
+    // Position of a tile's first key, and the position behind the last that it may hold.
+    static __device__ __forceinline__ int base(const Segment& s, int tile)
+    {
+        return is_last(s, tile) ? s.e.last_base : tile * KEYS;
+    }
+    static __device__ __forceinline__ int limit(const Segment& s, int tile)
+    {
+        return is_last(s, tile) ? s.e.length + s.e.nodes : s.e.last_base;
+    }
+    // Whether some of a tile's keys are not seen by every row.
+    static __device__ __forceinline__ bool is_masked(const Segment& s, int tile)
+    {
+        return is_last(s, tile) || (tile + 1) * KEYS > s.e.last_base;
+    }
+    // Keys 32 c to 32 c + 31 of a tile that a row sees, one bit each; `sees` are its drafted nodes.
+    static __device__ __forceinline__ std::uint32_t visible(const Segment& s, int tile, int c, unsigned long long sees)
+    {
+        const int committed = (is_last(s, tile) ? s.e.length : s.e.last_base) - base(s, tile) - 32 * c; // of these keys
+        std::uint32_t bits = committed >= 32 ? ~0u : (committed <= 0 ? 0u : (1u << committed) - 1u);
+        if (is_last(s, tile))
+            bits |= static_cast<std::uint32_t>(committed >= 32    ? 0ull
+                                               : committed >= 0   ? sees << committed
+                                               : committed > -64  ? sees >> -committed
+                                                                  : 0ull);
+        return bits;
+    }
+
     // Byte offset in a plane of key row `in_tile` of a tile, for one key head; -1: no such key.
     static __device__ __forceinline__ long long key_row(const TreeArgs& a, const Segment& s, int tile, int in_tile)
     {
-        if (tile >= s.tile_end)
-            return -1;
-        const bool drafted = tile == s.e.tiles - 1;
-        const int position = drafted ? s.e.length + in_tile : tile * KEYS + in_tile;
-        if (drafted ? in_tile >= s.e.nodes : position >= s.e.length)
+        const int position = base(s, tile) + in_tile;
+        if (tile >= s.tile_end || position >= limit(s, tile))
             return -1;
         const int page = cache_page(a.cache, s.e.sequence, s.e.held, position >> a.cache.page_shift);
         if (page < 0)

@@ -20,13 +20,20 @@
 //                   then O += P V with P in TMEM over the columns of S.  The
 //                   two groups' products alternate, so that one group's
 //                   exponentials overlap the other's products.
-//   warps 9, 10     producers: each key or value tile (128 rows of any pages)
-//                   by 16-byte asynchronous copies into a ring of shared-memory
-//                   slots in the 128-byte swizzle that the MMA reads; rows
-//                   behind the last position become zeros.
+//   warps 9, 10     producers, half of each key or value tile each, into a ring
+//                   of shared-memory slots in the 128-byte swizzle that the MMA
+//                   reads, by TMA: one box per page (or 64 rows) and 64 columns,
+//                   a lane each.  Value tiles with rows behind the last position
+//                   come by 16-byte asynchronous copies that make those rows
+//                   zeros, as does everything where TMA does not serve: pages of
+//                   fewer than 8 rows (a swizzle atom), or 2^31 rows in a plane.  Copies of every tile by the two warps
+//                   bound the kernel by their address arithmetic (290 against
+//                   BATCH_TREES us for 64 x 16 nodes over up to 4,096 positions).
 // The running maximum moves only when a row's tile exceeds it by more than 8
 // (in powers of two): p then stays below 256, which bf16, fp16 and the 32-bit
-// sums hold as well as 1, and the output in TMEM is rescaled rarely.
+// sums hold as well as 1, and the output in TMEM is rescaled rarely.  So a tile
+// is read once: p is computed with the maximum so far while the tile's own is
+// found, and computed again only when that has moved.
 //
 // Every wait is bounded (tc_common.cuh).  One that gives up raises
 // error_timeout and the CTA's abort flag; softmax threads then run through
@@ -84,24 +91,25 @@ template <bool TWO> struct Tail
 };
 static_assert(sizeof(Tail<true>) <= 2048 && sizeof(Tail<false>) <= 4096, "tail of the shared memory");
 
-__device__ __forceinline__ void tmem_load32(uint32_t address, uint32_t (&r)[32])
-{
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32"
-                 " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
-                 " %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
-                   "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
-                   "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
-                   "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-                 : "r"(address));
-}
-
 __device__ __forceinline__ uint32_t tmem_load1(uint32_t address)
 {
     uint32_t r;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(address));
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r)
+                 : "r"(address)
+                 : "memory");
     return r;
+}
+
+// Waits for this thread's TMEM loads; r is named so that no use of it moves before the wait.
+__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
 }
 
 __device__ __forceinline__ void tmem_store16(uint32_t address, const uint32_t* r)
@@ -121,6 +129,14 @@ __device__ __forceinline__ void tmem_wait_stores()
 __device__ __forceinline__ void fence_async_proxy()
 {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+__device__ __forceinline__ void tma_4d(uint32_t to, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+                 " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+                 : "memory");
 }
 
 // Barrier of the softmax threads.
@@ -148,22 +164,55 @@ template <class T> __device__ __forceinline__ constexpr uint32_t instruction(int
            (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
 }
 
-__device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+// The MMA warp runs converged, and only the instruction itself is predicated on
+// one lane: descriptors, which the instruction takes from uniform registers,
+// then need no transfer for each MMA (in a branch of one lane an issue took
+// about 100 cycles, the product itself 64).
+__device__ __forceinline__ bool elect_one()
 {
+    uint32_t chosen;
     asm volatile("{\n\t.reg .pred p;\n\t"
+                 "elect.sync _|p, 0xffffffff;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(chosen));
+    return chosen != 0;
+}
+
+__device__ __forceinline__ void mma_shared(bool leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                           bool accumulate)
+{
+    asm volatile("{\n\t.reg .pred p, q;\n\t"
                  "setp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-                 "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 "setp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(static_cast<uint32_t>(leader))
                  : "memory");
 }
 
-__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+__device__ __forceinline__ void mma_tmem(bool leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                         bool accumulate)
 {
-    asm volatile("{\n\t.reg .pred p;\n\t"
+    asm volatile("{\n\t.reg .pred p, q;\n\t"
                  "setp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-                 "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 "setp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(static_cast<uint32_t>(leader))
                  : "memory");
+}
+
+__device__ __forceinline__ void commit_if(bool leader, uint32_t bar)
+{
+    asm volatile("{\n\t.reg .pred q;\n\t"
+                 "setp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+                 "r"(static_cast<uint32_t>(leader))
+                 : "memory");
+}
+
+// A value that is the same in every lane, in a form that the compiler knows to be.
+__device__ __forceinline__ int uniform(int v)
+{
+    return __shfl_sync(0xffffffffu, v, 0);
 }
 
 // Operand `op` of a segment of `tiles` tiles, in the order in which the MMA
@@ -196,7 +245,8 @@ template <class N> struct Both
 
 template <class T, int D, bool TWO>
 __global__ void __launch_bounds__(THREADS, 1)
-    tree_attention_tc_kernel(const TreeArgs a, float* pieces, TreeShared* shared_items)
+    tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const TreeArgs a, const int box_rows,
+                             float* pieces, TreeShared* shared_items)
 {
     pdl_prologue();
     using L = Tiles<D, TWO>;
@@ -218,7 +268,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     {
         for (int s = 0; s < L::SLOTS; ++s)
         {
-            bar_init(smem_u32(&tail.full[s]), PRODUCERS);
+            bar_init(smem_u32(&tail.full[s]), PRODUCERS / 32);
             bar_init(smem_u32(&tail.empty[s]), 1);
         }
         for (int g = 0; g < 2; ++g)
@@ -265,72 +315,117 @@ __global__ void __launch_bounds__(THREADS, 1)
     {
         // ------------------------------------------------------------ producers --
         const int first_row = (warp - PRODUCER_WARP) * PRODUCER_ROWS; // this warp's rows of each tile
-        constexpr int rows_at_once = 32 / L::chunks;
+        constexpr int rows_at_once = 32 / L::chunks, panels = D / 64;
+        const int boxes = box_rows ? PRODUCER_ROWS / box_rows * panels : 0; // of this warp's half tile
         int slot = 0, round = 0; // uses of the slot so far
+        int copied = -1, copied_segment = 0; // a slot whose copies have been issued and not yet announced
+        int copied_nodes = -1; // its first drafted row; -1: none
+        // Announces the copied slot, once its copies have landed: all but the newest `behind` group.
+        const auto announce = [&](bool behind)
+        {
+            if (copied < 0)
+                return;
+            if (behind)
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            else
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+            if (copied_nodes >= 0)
+            {
+                // 0 x NaN would reach rows that do not see the node: values that are not
+                // finite leave the product and are added where they are seen.
+                for (int i = 0; i < PRODUCER_ROWS / rows_at_once; ++i)
+                {
+                    const int row = first_row + i * rows_at_once + lane / L::chunks, chunk = lane % L::chunks;
+                    auto* at = reinterpret_cast<uint4*>(smem + L::ring_offset + copied * L::operand_bytes +
+                                                        (chunk >> 3) * L::panel_bytes + row * 128 +
+                                                        (((chunk & 7) ^ (row & 7)) << 4));
+                    const uint4 v = *at;
+                    const uint32_t odd[4] = {nonfinite_mask<T>(v.x), nonfinite_mask<T>(v.y), nonfinite_mask<T>(v.z),
+                                             nonfinite_mask<T>(v.w)};
+                    if (row >= copied_nodes && (odd[0] | odd[1] | odd[2] | odd[3]))
+                    {
+                        *at = make_uint4(v.x & ~odd[0], v.y & ~odd[1], v.z & ~odd[2], v.w & ~odd[3]);
+                        atomicOr(&tail.tainted[copied_segment % TAINT_SLOTS], 1ull << ((row - copied_nodes) & 63));
+                    }
+                }
+            }
+            fence_async_proxy(); // the copies are generic writes, the MMA reads through the async proxy
+            __syncwarp();
+            if (lane == 0)
+                bar_arrive(smem_u32(&tail.full[copied]));
+            copied = -1;
+        };
         for (int segment = 0; ok && cursor.next(a, g); ++segment)
         {
             const int tiles = g.tile_end - g.tile_begin;
-            bool value;
-            int tile;
-            operand<TWO>(0, tiles, value, tile);
-            long long low_rows, high_rows; // this lane's rows, lane and lane + 32 of the warp's
-            const auto find_rows = [&]
-            {
-                low_rows = Work::key_row(a, g, g.tile_begin + tile, first_row + lane);
-                high_rows = Work::key_row(a, g, g.tile_begin + tile, first_row + 32 + lane);
-            };
-            find_rows();
             for (int op = 0; op < 2 * tiles; ++op)
             {
-                const bool this_value = value, drafted = g.tile_begin + tile == g.e.tiles - 1;
+                bool value;
+                int tile;
+                operand<TWO>(op, tiles, value, tile);
+                tile += g.tile_begin;
+                const uint32_t base = smem_u32(smem + L::ring_offset + slot * L::operand_bytes);
+                const uint32_t bar = smem_u32(&tail.full[slot]);
+                // Scores of keys behind the last are masked whatever they are; values have to be zeros.
+                const bool boxed = boxes && (!value || !Work::is_masked(g, tile));
+                // The tile's table entries are on their way while the slot is awaited.
+                int row_of_pool = 0;
+                long long low_rows = -1, high_rows = -1;
+                if (boxed)
+                {
+                    if (lane < boxes)
+                    {
+                        const int position = Work::base(g, tile) + first_row + lane / panels * box_rows;
+                        const int page = position < Work::limit(g, tile)
+                                             ? cache_page(a.cache, g.e.sequence, g.e.held, position >> a.cache.page_shift)
+                                             : -1;
+                        if (page < 0 && position < Work::limit(g, tile) && a.error_word)
+                            atomicOr(a.error_word, error_cache);
+                        row_of_pool = page < 0 ? a.cache.pages << a.cache.page_shift // outside: zeros
+                                               : (page << a.cache.page_shift) + (position & (a.cache.page_size() - 1));
+                    }
+                }
+                else
+                {
+                    low_rows = Work::key_row(a, g, tile, first_row + lane);
+                    high_rows = Work::key_row(a, g, tile, first_row + 32 + lane);
+                }
                 wait(tail.empty[slot], round + 1);
                 ok = __all_sync(0xffffffffu, ok); // the warp goes on or leaves together
                 if (!ok)
                     break;
-                const uint32_t base = smem_u32(smem + L::ring_offset + slot * L::operand_bytes);
-                const unsigned char* from = plane + (value ? a.cache.plane_bytes : 0);
-                const int chunk = lane % L::chunks;
-                const uint32_t column = base + (chunk >> 3) * L::panel_bytes;
-#pragma unroll 8
-                for (int i = 0; i < PRODUCER_ROWS / rows_at_once; ++i)
+                if (boxed)
                 {
-                    const int row = i * rows_at_once + lane / L::chunks;
-                    const long long offset = __shfl_sync(0xffffffffu, i * rows_at_once < 32 ? low_rows : high_rows, row & 31);
-                    copy_16(column + (first_row + row) * 128 + (((chunk & 7) ^ (row & 7)) << 4),
-                            from + (offset >= 0 ? offset + 16 * chunk : 0), offset >= 0 ? 16u : 0u);
-                }
-                // The next tile's table entries are on their way while this one is copied.
-                if (op + 1 < 2 * tiles)
-                {
-                    operand<TWO>(op + 1, tiles, value, tile);
-                    find_rows();
-                }
-                const uint32_t bar = smem_u32(&tail.full[slot]);
-                if (this_value && drafted)
-                {
-                    // 0 x NaN would reach rows that do not see the node: values that are not
-                    // finite leave the product and are added where they are seen.
-                    asm volatile("cp.async.wait_all;" ::: "memory");
-                    for (int i = 0; i < PRODUCER_ROWS / rows_at_once; ++i)
+                    if (lane == 0)
+                        bar_expect_tx(bar, L::operand_bytes / 2);
+                    __syncwarp();
+                    if (lane < boxes)
                     {
-                        const int row = first_row + i * rows_at_once + lane / L::chunks;
-                        auto* at = reinterpret_cast<uint4*>(smem + L::ring_offset + slot * L::operand_bytes +
-                                                            (chunk >> 3) * L::panel_bytes + row * 128 +
-                                                            (((chunk & 7) ^ (row & 7)) << 4));
-                        uint4 v = *at;
-                        const uint32_t odd[4] = {nonfinite_mask<T>(v.x), nonfinite_mask<T>(v.y),
-                                                 nonfinite_mask<T>(v.z), nonfinite_mask<T>(v.w)};
-                        if (odd[0] | odd[1] | odd[2] | odd[3])
-                        {
-                            *at = make_uint4(v.x & ~odd[0], v.y & ~odd[1], v.z & ~odd[2], v.w & ~odd[3]);
-                            atomicOr(&tail.tainted[segment % TAINT_SLOTS], 1ull << (row & 63));
-                        }
+                        const int box = lane / panels, panel = lane - box * panels;
+                        tma_4d(base + panel * L::panel_bytes + (first_row + box * box_rows) * 128, &map, panel * 64,
+                               g.head, row_of_pool, value, bar);
                     }
-                    bar_arrive(bar);
+                    announce(false);
                 }
                 else
                 {
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+                    const unsigned char* from = plane + (value ? a.cache.plane_bytes : 0);
+                    const int chunk = lane % L::chunks;
+                    const uint32_t column = base + (chunk >> 3) * L::panel_bytes;
+#pragma unroll 8
+                    for (int i = 0; i < PRODUCER_ROWS / rows_at_once; ++i)
+                    {
+                        const int row = i * rows_at_once + lane / L::chunks;
+                        const long long offset =
+                            __shfl_sync(0xffffffffu, i * rows_at_once < 32 ? low_rows : high_rows, row & 31);
+                        copy_16(column + (first_row + row) * 128 + (((chunk & 7) ^ (row & 7)) << 4),
+                                from + (offset >= 0 ? offset + 16 * chunk : 0), offset >= 0 ? 16u : 0u);
+                    }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    announce(true);
+                    copied = slot;
+                    copied_nodes = Work::is_last(g, tile) && value ? g.e.length - g.e.last_base : -1;
+                    copied_segment = segment;
                 }
                 if (++slot == L::SLOTS)
                 {
@@ -338,126 +433,140 @@ __global__ void __launch_bounds__(THREADS, 1)
                     ++round;
                 }
             }
+            announce(false);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
+        if (!ok) // this warp's TMA boxes land before the CTA ends
+        {
+            volatile int never = 0;
+            const int used = round * L::SLOTS + slot; // operands issued; every earlier use of a slot was waited for
+            for (int n = used > L::SLOTS ? used - L::SLOTS : 0; n < used; ++n)
+                bar_wait(smem_u32(&tail.full[n % L::SLOTS]), static_cast<uint32_t>(n / L::SLOTS & 1), &never);
+        }
     }
     else if (warp == MMA_WARP)
     {
         // ------------------------------------------------------------------ MMA --
-        if (lane == 0)
+        constexpr uint32_t score_idesc = instruction<T>(KEYS, false), value_idesc = instruction<T>(D, true);
+        const bool leader = elect_one();
+        const uint32_t tm = static_cast<uint32_t>(uniform(static_cast<int>(tmem)));
+        const uint32_t query = smem_u32(smem), ring = query + L::ring_offset;
+        int slot = 0, round = 0;
+        Both<int> made{0, 0}; // products issued
+        bool any = false;
+        const auto wait_all = [&](uint64_t& bar, int phase)
         {
-            constexpr uint32_t score_idesc = instruction<T>(KEYS, false), value_idesc = instruction<T>(D, true);
-            int slot = 0, round = 0;
-            Both<int> made{0, 0}; // products issued
-            bool any = false;
-            const auto take = [&]() -> int // the next operand's slot, once it has landed
+            wait(bar, phase);
+            ok = __all_sync(0xffffffffu, ok);
+            return ok;
+        };
+        const auto take = [&]() -> int // the next operand's slot, once it has landed
+        {
+            const int s = slot;
+            wait_all(tail.full[s], round);
+            if (++slot == L::SLOTS)
             {
-                const int s = slot;
-                wait(tail.full[s], round);
-                fence_async_proxy(); // the copies are generic writes, the MMA reads through the async proxy
-                if (++slot == L::SLOTS)
-                {
-                    slot = 0;
-                    ++round;
-                }
-                return s;
-            };
-            const auto score = [&](int group, int s)
-            {
-                if (!ok)
-                    return;
-                const uint32_t q = smem_u32(smem) + (TWO ? group * L::operand_bytes : 0);
-                const uint32_t k = smem_u32(smem + L::ring_offset + s * L::operand_bytes);
-                tc_fence_after();
+                slot = 0;
+                ++round;
+            }
+            return s;
+        };
+        const auto score = [&](int group, int s)
+        {
+            if (!ok)
+                return;
+            const uint64_t q = sw128_desc(query + (TWO ? group * L::operand_bytes : 0));
+            const uint64_t k = sw128_desc(ring + s * L::operand_bytes);
+            tc_fence_after();
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk)
-                {
-                    const uint32_t at = (kk >> 2) * L::panel_bytes + (kk & 3) * 32;
-                    mma_shared(tmem + group * KEYS, sw128_desc(q + at), sw128_desc(k + at), score_idesc, kk != 0);
-                }
-                mma_commit(smem_u32(&tail.scores[group]));
-                any = true;
-            };
-            const auto product = [&](int group, int s, bool accumulate)
+            for (int kk = 0; kk < D / 16; ++kk)
             {
-                if (!ok || !wait(tail.weights[group], made(group)))
-                    return;
-                const uint32_t v = smem_u32(smem + L::ring_offset + s * L::operand_bytes);
-                tc_fence_after();
+                constexpr int unit = 16; // of a descriptor's address
+                const int at = ((kk >> 2) * L::panel_bytes + (kk & 3) * 32) / unit;
+                mma_shared(leader, tm + group * KEYS, q + at, k + at, score_idesc, kk != 0);
+            }
+            commit_if(leader, smem_u32(&tail.scores[group]));
+            any = true;
+        };
+        const auto product = [&](int group, int s, bool accumulate)
+        {
+            if (!ok || !wait_all(tail.weights[group], made(group)))
+                return;
+            const uint64_t v = value_desc(ring + s * L::operand_bytes, L::panel_bytes);
+            tc_fence_after();
 #pragma unroll
-                for (int kk = 0; kk < KEYS / 16; ++kk)
-                    mma_tmem(tmem + OUTPUT_COLUMN + group * 128, tmem + group * KEYS + 8 * kk,
-                             value_desc(v + kk * 2048, L::panel_bytes), value_idesc, accumulate || kk != 0);
-                mma_commit(smem_u32(&tail.products[group]));
-                made.add(group, 1);
-            };
-            // P lies over S: the next scores of a group wait for its product.
-            const auto after_product = [&](int group) { wait(tail.products[group], made(group) - 1); };
-            const auto free_slot = [&](int s)
+            for (int kk = 0; kk < KEYS / 16; ++kk)
+                mma_tmem(leader, tm + OUTPUT_COLUMN + group * 128, tm + group * KEYS + 8 * kk, v + kk * 2048 / 16,
+                         value_idesc, accumulate || kk != 0);
+            commit_if(leader, smem_u32(&tail.products[group]));
+            made.add(group, 1);
+        };
+        // P lies over S: the next scores of a group wait for its product.
+        const auto after_product = [&](int group) { wait_all(tail.products[group], made(group) - 1); };
+        const auto free_slot = [&](int s)
+        {
+            if (ok)
+                commit_if(leader, smem_u32(&tail.empty[s]));
+        };
+        for (int segment = 0; ok && uniform(cursor.next(a, g)); ++segment)
+        {
+            const int tiles = uniform(g.tile_end - g.tile_begin);
+            wait_all(tail.query, segment);
+            if constexpr (TWO)
             {
-                if (ok)
-                    mma_commit(smem_u32(&tail.empty[s]));
-            };
-            for (int segment = 0; ok && cursor.next(a, g); ++segment)
-            {
-                const int tiles = g.tile_end - g.tile_begin;
-                wait(tail.query, segment);
-                if constexpr (TWO)
+                int k = take();
+                score(0, k);
+                score(1, k);
+                free_slot(k);
+                for (int j = 0; j < tiles && ok; ++j)
                 {
-                    int k = take();
-                    score(0, k);
-                    score(1, k);
-                    free_slot(k);
-                    for (int j = 0; j < tiles && ok; ++j)
+                    const int v = take();
+                    const bool more = j + 1 < tiles;
+                    product(0, v, j > 0);
+                    if (more)
                     {
-                        const int v = take();
-                        const bool more = j + 1 < tiles;
-                        product(0, v, j > 0);
-                        if (more)
-                        {
-                            k = take();
-                            after_product(0);
-                            score(0, k);
-                        }
-                        product(1, v, j > 0);
-                        free_slot(v);
-                        if (more)
-                        {
-                            after_product(1);
-                            score(1, k);
-                            free_slot(k);
-                        }
+                        k = take();
+                        after_product(0);
+                        score(0, k);
                     }
-                }
-                else
-                {
-                    for (int j = 0; j < 2 && j < tiles; ++j)
+                    product(1, v, j > 0);
+                    free_slot(v);
+                    if (more)
                     {
-                        const int k = take();
-                        score(j, k);
+                        after_product(1);
+                        score(1, k);
                         free_slot(k);
                     }
-                    for (int j = 0; j < tiles && ok; ++j)
+                }
+            }
+            else
+            {
+                for (int j = 0; j < 2 && j < tiles; ++j)
+                {
+                    const int k = take();
+                    score(j, k);
+                    free_slot(k);
+                }
+                for (int j = 0; j < tiles && ok; ++j)
+                {
+                    const int v = take();
+                    product(j & 1, v, j > 1);
+                    free_slot(v);
+                    if (j + 2 < tiles)
                     {
-                        const int v = take();
-                        product(j & 1, v, j > 1);
-                        free_slot(v);
-                        if (j + 2 < tiles)
-                        {
-                            const int k = take();
-                            after_product(j & 1);
-                            score(j & 1, k);
-                            free_slot(k);
-                        }
+                        const int k = take();
+                        after_product(j & 1);
+                        score(j & 1, k);
+                        free_slot(k);
                     }
                 }
             }
-            if (any)
-            {
-                mma_commit(smem_u32(&tail.drain));
-                volatile int never = 0;
-                bar_wait(smem_u32(&tail.drain), 0, &never);
-            }
+        }
+        if (any)
+        {
+            commit_if(leader, smem_u32(&tail.drain));
+            volatile int never = 0;
+            bar_wait(smem_u32(&tail.drain), 0, &never);
         }
     }
     else
@@ -466,9 +575,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int group = warp >> 2, row = t & (GROUP_THREADS - 1);
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t my_scores = lanes + group * KEYS, my_output = lanes + OUTPUT_COLUMN + group * 128;
-        // A negative scale turns the query's signs, so that the largest product stays the largest score.
-        const uint32_t turn = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
-        const float scale = fabsf(a.scale_log2);
+        // A negative scale turns the query's signs and a zero one clears it, so that the
+        // factor is positive: the largest product is the largest score, and -infinity stays.
+        const uint32_t turn = a.scale_log2 < 0.0f ? 0x80008000u : 0u, keep = a.scale_log2 == 0.0f ? 0u : ~0u;
+        const float scale = a.scale_log2 == 0.0f ? 1.0f : fabsf(a.scale_log2);
         int scores_seen = 0;
         Both<int> products_seen{0, 0};
         for (int segment = 0; cursor.next(a, g); ++segment)
@@ -491,7 +601,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 {
                     const int chunk = first_chunk + c;
                     uint4 v = live ? *reinterpret_cast<const uint4*>(from + 8 * chunk) : make_uint4(0, 0, 0, 0);
-                    v = make_uint4(v.x ^ turn, v.y ^ turn, v.z ^ turn, v.w ^ turn);
+                    v = make_uint4((v.x ^ turn) & keep, (v.y ^ turn) & keep, (v.z ^ turn) & keep, (v.w ^ turn) & keep);
                     *reinterpret_cast<uint4*>(to + (chunk >> 3) * L::panel_bytes + (((chunk & 7) ^ (row & 7)) << 4)) = v;
                 }
                 fence_async_proxy();
@@ -502,105 +612,110 @@ __global__ void __launch_bounds__(THREADS, 1)
                                tail.above, group == 0 && warp < 2 ? a.error_word : nullptr, t, [] { softmax_sync(); });
             const unsigned long long sees = has_draft && live ? tail.masks[node] : 0ull;
 
-            float maximum = -INFINITY, sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            // A warp without a live row has nothing to compute: whatever its lanes of TMEM hold stays there.
+            const bool busy = __any_sync(0xffffffffu, live);
+            float maximum = -INFINITY, sum = 0.0f;
             for (int j = TWO ? 0 : group; j < tiles; j += TWO ? 1 : 2)
             {
                 const int tile = g.tile_begin + j;
-                const bool drafted = tile == g.e.tiles - 1;
-                const int held = drafted ? 0 : g.e.length - tile * KEYS;
-                const bool masked = held < KEYS;
-                // Keys 32 c to 32 c + 31 that this row sees, one bit each.
-                const auto visible = [&](int c) -> uint32_t
+                const bool masked = Work::is_masked(g, tile);
+                // Scores 16 c to 16 c + 15 of this row, those it does not see made -infinity.
+                const auto hide = [&](int c, uint32_t (&s)[16])
                 {
-                    if (drafted)
-                        return c == 0 ? static_cast<uint32_t>(sees) : (c == 1 ? static_cast<uint32_t>(sees >> 32) : 0u);
-                    const int n = held - 32 * c;
-                    return n >= 32 ? ~0u : (n <= 0 ? 0u : (1u << n) - 1u);
+                    const uint32_t bits = Work::visible(g, tile, c >> 1, sees) >> (16 * (c & 1));
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        s[k] = bits >> k & 1u ? s[k] : 0xff800000u;
                 };
                 wait(tail.scores[group], scores_seen++);
                 __syncwarp();
                 tc_fence_after();
-                float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (busy)
+                {
+                    const bool first = TWO ? j == 0 : j < 2;
+                    if (first)
+                    {
+                        float best = -INFINITY;
 #pragma unroll 1
-                for (int c = 0; c < KEYS / 32; ++c)
-                {
-                    uint32_t s[32];
-                    tmem_load32(my_scores + 32 * c, s);
-                    tmem_wait_loads();
-                    if (masked)
-                    {
-                        const uint32_t bits = visible(c);
-#pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            best[k & 3] = fmaxf(best[k & 3], bits >> k & 1u ? __uint_as_float(s[k]) : -INFINITY);
-                    }
-                    else
-                    {
-#pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            best[k & 3] = fmaxf(best[k & 3], __uint_as_float(s[k]));
-                    }
-                }
-                const float highest = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
-                const float top = highest == -INFINITY ? -INFINITY : highest * scale;
-                const bool first = TWO ? j == 0 : j < 2;
-                if (first)
-                {
-                    maximum = top;
-                }
-                else if (__any_sync(0xffffffffu, top > maximum + RESCALE))
-                {
-                    const float raised = fmaxf(maximum, top);
-                    const float shrink = maximum == -INFINITY ? 0.0f : power_of_two(maximum - raised);
-                    maximum = raised;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        sums[k] *= shrink;
-                    // The product before these scores is complete: they were issued after it.
-#pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c)
-                    {
-                        uint32_t o[32];
-                        tmem_load32(my_output + 32 * c, o);
-                        tmem_wait_loads();
-#pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
-                        tmem_store16(my_output + 32 * c, o);
-                        tmem_store16(my_output + 32 * c + 16, o + 16);
-                    }
-                }
-                const float shift = maximum == -INFINITY ? 0.0f : -maximum;
-#pragma unroll 1
-                for (int c = 0; c < KEYS / 32; ++c)
-                {
-                    uint32_t s[32], p[16];
-                    tmem_load32(my_scores + 32 * c, s);
-                    tmem_wait_loads();
-                    const uint32_t bits = masked ? visible(c) : ~0u;
-#pragma unroll
-                    for (int k = 0; k < 32; k += 2)
-                    {
-                        float x = power_of_two(fmaf(__uint_as_float(s[k]), scale, shift));
-                        float y = power_of_two(fmaf(__uint_as_float(s[k + 1]), scale, shift));
-                        if (masked)
+                        for (int c = 0; c < KEYS / 16; ++c)
                         {
-                            x = bits >> k & 1u ? x : 0.0f;
-                            y = bits >> (k + 1) & 1u ? y : 0.0f;
+                            uint32_t s[16];
+                            tmem_load16(my_scores + 16 * c, s);
+                            tmem_wait16(s);
+                            if (masked)
+                                hide(c, s);
+#pragma unroll
+                            for (int k = 0; k < 16; ++k)
+                                best = fmaxf(best, __uint_as_float(s[k]));
                         }
-                        sums[k & 3] += x;
-                        sums[(k & 3) + 1] += y;
-                        p[k / 2] = Half2<T>::pack(x, y);
+                        maximum = best == -INFINITY ? -INFINITY : best * scale;
                     }
-                    tmem_store16(my_scores + 16 * c, p); // over scores that have been read
+                    uint32_t p[KEYS / 2];
+                    float part[2];
+                    // p with the maximum so far; returns the tile's own maximum.
+                    const auto exponentials = [&]
+                    {
+                        const float shift = maximum == -INFINITY ? 0.0f : -maximum;
+                        float best[2] = {-INFINITY, -INFINITY};
+                        part[0] = part[1] = 0.0f;
+                        uint32_t s[2][16];
+                        tmem_load16(my_scores, s[0]);
+#pragma unroll
+                        for (int c = 0; c < KEYS / 16; ++c)
+                        {
+                            uint32_t(&now)[16] = s[c & 1];
+                            tmem_wait16(now);
+                            if (c + 1 < KEYS / 16) // the next scores are on their way while these are used
+                                tmem_load16(my_scores + 16 * (c + 1), s[(c + 1) & 1]);
+                            if (masked)
+                                hide(c, now);
+#pragma unroll
+                            for (int k = 0; k < 16; k += 2)
+                            {
+                                best[0] = fmaxf(best[0], __uint_as_float(now[k]));
+                                best[1] = fmaxf(best[1], __uint_as_float(now[k + 1]));
+                                const float x = power_of_two(fmaf(__uint_as_float(now[k]), scale, shift));
+                                const float y = power_of_two(fmaf(__uint_as_float(now[k + 1]), scale, shift));
+                                part[0] += x;
+                                part[1] += y;
+                                p[8 * c + k / 2] = Half2<T>::pack(x, y);
+                            }
+                        }
+                        const float highest = fmaxf(best[0], best[1]);
+                        return highest == -INFINITY ? -INFINITY : highest * scale;
+                    };
+                    const float top = exponentials();
+                    if (!first && __any_sync(0xffffffffu, top > maximum + RESCALE))
+                    {
+                        const float raised = fmaxf(maximum, top);
+                        const float shrink = maximum == -INFINITY ? 0.0f : power_of_two(maximum - raised);
+                        maximum = raised;
+                        sum *= shrink;
+                        // The product before these scores is complete: they were issued after it.
+#pragma unroll 1
+                        for (int c = 0; c < D / 16; ++c)
+                        {
+                            uint32_t o[16];
+                            tmem_load16(my_output + 16 * c, o);
+                            tmem_wait16(o);
+#pragma unroll
+                            for (int k = 0; k < 16; ++k)
+                                o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
+                            tmem_store16(my_output + 16 * c, o);
+                        }
+                        exponentials();
+                    }
+                    sum += part[0] + part[1];
+#pragma unroll
+                    for (int c = 0; c < KEYS / 32; ++c)
+                        tmem_store16(my_scores + 16 * c, p + 16 * c); // over scores that have been read
+                    tmem_wait_stores();
                 }
-                tmem_wait_stores();
                 tc_fence_before();
                 bar_arrive(smem_u32(&tail.weights[group]));
             }
             // ------------------------------------------------------- epilogue --
             const Both<int> made{TWO ? tiles : (tiles + 1) / 2, TWO ? tiles : tiles / 2};
-            float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
             if (made(group))
                 wait(tail.products[group], products_seen(group) + made(group) - 1);
             Both<float> part{1.0f, 1.0f}; // factors of the groups' outputs
@@ -632,16 +747,16 @@ __global__ void __launch_bounds__(THREADS, 1)
             const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum; // a row that sees nothing gives zeros
             constexpr int columns = TWO ? D : D / 2;                  // of this thread
             const int first_column = TWO ? 0 : group * columns;
-            constexpr int step = TWO ? 32 : 16;
+            constexpr int step = 16;
 #pragma unroll 1
-            for (int c = 0; c < columns; c += step)
+            for (int c = 0; busy && c < columns; c += step)
             {
                 const int column = first_column + c;
                 uint32_t o[step];
                 if constexpr (TWO)
                 {
-                    tmem_load32(my_output + column, o);
-                    tmem_wait_loads();
+                    tmem_load16(my_output + column, o);
+                    tmem_wait16(o);
                 }
                 else
                 {
@@ -649,7 +764,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                     tmem_load16(lanes + OUTPUT_COLUMN + column, o); // the first group always has a tile
                     if (made.second)
                         tmem_load16(lanes + OUTPUT_COLUMN + 128 + column, other);
-                    tmem_wait_loads();
+                    tmem_wait16(o);
+                    if (made.second)
+                        tmem_wait16(other);
 #pragma unroll
                     for (int k = 0; k < step; ++k)
                     {
@@ -662,12 +779,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                 for (unsigned long long rest = tainted; rest; rest &= rest - 1)
                 {
                     const int key = __ffsll(static_cast<long long>(rest)) - 1;
-                    const uint32_t pair = tmem_load1(lanes + draft_group * KEYS + key / 2);
-                    tmem_wait_loads();
-                    const long long offset = sees >> key & 1ull ? Work::key_row(a, g, g.e.tiles - 1, key) : -1;
+                    const int in_tile = g.e.length - g.e.last_base + key;
+                    const uint32_t pair = tmem_load1(lanes + draft_group * KEYS + in_tile / 2);
+                    const long long offset = sees >> key & 1ull ? Work::key_row(a, g, g.e.tiles - 1, in_tile) : -1;
                     if (offset >= 0)
                     {
-                        const float weight = Half2<T>::value(static_cast<std::uint16_t>(key & 1 ? pair >> 16 : pair)) *
+                        const float weight = Half2<T>::value(static_cast<std::uint16_t>(in_tile & 1 ? pair >> 16 : pair)) *
                                              part(TWO ? 0 : draft_group);
                         const auto* values = reinterpret_cast<const std::uint16_t*>(plane + a.cache.plane_bytes + offset) + column;
 #pragma unroll
@@ -730,6 +847,25 @@ __global__ void __launch_bounds__(THREADS, 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLUMNS));
 }
 
+// The layer's two planes as [keys, values][row][head][column], in boxes of
+// `rows` rows of one head and 64 columns.
+bool make_map(CUtensorMap* map, const TreeArgs& a, int rows)
+{
+    const auto fn = encode_fn();
+    const CacheView& c = a.cache;
+    const cuuint64_t plane_rows = static_cast<cuuint64_t>(c.pages) << c.page_shift;
+    if (!fn || plane_rows >= 0x7fffffffull || c.plane_bytes >= 1ll << 40)
+        return false;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(a.heads), plane_rows, 2};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(2 * a.head_dim), static_cast<cuuint64_t>(c.row_bytes),
+                                   static_cast<cuuint64_t>(c.plane_bytes)};
+    const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(rows), 1};
+    const cuuint32_t elem[4] = {1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, c.pool + 2ll * a.layer * c.plane_bytes, dims, strides, box, elem,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <class T, int D, bool TWO>
 void launch(const TreeArgs& a, float* pieces, TreeShared* shared_items, cudaStream_t stream)
 {
@@ -744,8 +880,13 @@ void launch(const TreeArgs& a, float* pieces, TreeShared* shared_items, cudaStre
                            cudaFuncSetAttribute(tree_attention_tc_kernel<T, D, TWO>,
                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem);
                        });
-    launch_pdl(tree_attention_tc_kernel<T, D, TWO>, dim3(sm_count()), dim3(THREADS), L::smem, stream, a, pieces,
-               shared_items);
+    // Boxes of a page, or of the 64 rows that a producer warp fills.
+    CUtensorMap map{};
+    int box_rows = a.cache.page_size() < PRODUCER_ROWS ? a.cache.page_size() : PRODUCER_ROWS;
+    if (box_rows < 8 || !make_map(&map, a, box_rows))
+        box_rows = 0;
+    launch_pdl(tree_attention_tc_kernel<T, D, TWO>, dim3(sm_count()), dim3(THREADS), L::smem, stream, map, a, box_rows,
+               pieces, shared_items);
     note_launch();
 }
 
