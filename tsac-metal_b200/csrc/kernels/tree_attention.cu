@@ -20,6 +20,7 @@
 #include "kernels/pdl.cuh"
 #include "kernels/tree_attention.cuh"
 
+#include <algorithm>
 #include <mutex>
 
 namespace tsacb::dev
@@ -61,10 +62,9 @@ __global__ void __launch_bounds__(THREADS, 2)
 {
     pdl_prologue();
     using L = Layout<D, MT>;
-    using Work = TreeWork<KEYS, L::ROWS>;
+    using Work = TreeWork<KEYS, L::ROWS, 1>;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ unsigned long long masks[DRAFT_MAX_NODES];
-    __shared__ int above[DRAFT_MAX_NODES];
     __shared__ long long warp_sums[WARPS];
     __shared__ typename Work::Start found;
     __shared__ float row_max[WARPS][L::ROWS], row_sum[WARPS][L::ROWS];
@@ -78,16 +78,48 @@ __global__ void __launch_bounds__(THREADS, 2)
     const std::uint32_t ring = static_cast<std::uint32_t>(__cvta_generic_to_shared(smem)) + warp * STAGES * L::stage_bytes;
     const unsigned char* plane = a.cache.pool + 2ll * a.layer * a.cache.plane_bytes;
 
-    typename Work::Cursor cursor(start, cta);
+    typename Work::Cursor cursor(start);
     typename Work::Segment g;
     while (cursor.next(a, g))
     {
         const auto& e = g.e;
         const int head = g.head, first_row = g.first_row, rows = g.rows;
         const int tile_begin = g.tile_begin, tile_end = g.tile_end;
+        // Lane % 16 follows one of the warp's 16 keys.
+        const auto key_row = [&](int tile) { return Work::key_row(a, g, tile, warp * WARP_KEYS + (lane & 15)); };
+        // Rows of L::chunks 16-byte chunks, chunk c of row r at place c ^ (r & 7): conflict-free for ldmatrix.
+        const auto fetch = [&](int stage, long long row_offset)
+        {
+            constexpr int rows_at_once = 32 / L::chunks;
+            const std::uint32_t base = ring + stage * L::stage_bytes;
+#pragma unroll
+            for (int i = 0; i < WARP_KEYS / rows_at_once; ++i)
+            {
+                const int row = i * rows_at_once + lane / L::chunks, chunk = lane % L::chunks;
+                const long long offset = __shfl_sync(0xffffffffu, row_offset, row);
+                const unsigned bytes = offset >= 0 ? 16u : 0u;
+                const unsigned char* from = plane + (offset >= 0 ? offset + 16 * chunk : 0);
+                const std::uint32_t to = base + row * L::row_bytes + ((chunk ^ (row & 7)) << 4);
+                copy_16(to, from, bytes);
+                copy_16(to + WARP_KEYS * L::row_bytes, from + a.cache.plane_bytes, bytes);
+            }
+        };
+        __syncwarp();
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s)
+        {
+            fetch(s, key_row(tile_begin + s));
+            copies_commit();
+        }
+        long long next_row = key_row(tile_begin + STAGES - 1);
+        // While the first keys and values are on their way: the tree's masks and the query.
         if (tile_end == e.tiles)
-            ancestor_masks(a.parents + static_cast<long long>(g.list_entry) * a.max_nodes, e.nodes, masks, above,
-                           a.error_word, t, [] { __syncthreads(); });
+        {
+            if (warp == 0)
+                ancestor_masks(a.parents + static_cast<long long>(g.list_entry) * a.max_nodes, e.nodes, masks,
+                               a.error_word, lane);
+            __syncthreads();
+        }
 
         // Query fragments: row lane / 4 (+ 8), columns 2 (lane % 4) (+ 8) of each 16.
         std::uint32_t q[MT][D / 16][4];
@@ -116,33 +148,6 @@ __global__ void __launch_bounds__(THREADS, 2)
             sum[m][0] = sum[m][1] = 0.0f;
         }
 
-        // Lane % 16 follows one of the warp's 16 keys.
-        const auto key_row = [&](int tile) { return Work::key_row(a, g, tile, warp * WARP_KEYS + (lane & 15)); };
-        // Rows of L::chunks 16-byte chunks, chunk c of row r at place c ^ (r & 7): conflict-free for ldmatrix.
-        const auto fetch = [&](int stage, long long row_offset)
-        {
-            constexpr int rows_at_once = 32 / L::chunks;
-            const std::uint32_t base = ring + stage * L::stage_bytes;
-#pragma unroll
-            for (int i = 0; i < WARP_KEYS / rows_at_once; ++i)
-            {
-                const int row = i * rows_at_once + lane / L::chunks, chunk = lane % L::chunks;
-                const long long offset = __shfl_sync(0xffffffffu, row_offset, row);
-                const unsigned bytes = offset >= 0 ? 16u : 0u;
-                const unsigned char* from = plane + (offset >= 0 ? offset + 16 * chunk : 0);
-                const std::uint32_t to = base + row * L::row_bytes + ((chunk ^ (row & 7)) << 4);
-                copy_16(to, from, bytes);
-                copy_16(to + WARP_KEYS * L::row_bytes, from + a.cache.plane_bytes, bytes);
-            }
-        };
-        __syncwarp();
-#pragma unroll
-        for (int s = 0; s < STAGES - 1; ++s)
-        {
-            fetch(s, key_row(tile_begin + s));
-            copies_commit();
-        }
-        long long next_row = key_row(tile_begin + STAGES - 1);
         int stage = 0;
         for (int tile = tile_begin; tile < tile_end; ++tile)
         {
@@ -387,53 +392,133 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
 }
 
-// Joins the pieces of an item that several CTAs share, in CTA order: one warp
-// per row.  Piece 0 is in the first CTA's second place, the others in their
-// CTAs' first places.
+// Joins the pieces of an item that several CTAs share.  Piece 0 is in the first
+// CTA's second place, the others in their CTAs' first places.  Each CTA lists
+// the shared items, so that the rows spread over the whole grid, and gives each
+// row 1, 4 or 16 warps, as many as the grid has for all rows at once: the warps
+// take the pieces in turn, several in flight, and are joined in shared memory
+// in a fixed order.  Bound by the latency of three dependent reads.
+constexpr int COMBINE_WARPS = 16, COMBINE_THREADS = COMBINE_WARPS * 32;
+
 template <class T, int D>
-__global__ void __launch_bounds__(128)
-    tree_combine_kernel(const TreeArgs a, int rows_per_item, const float* pieces,
-                        const TreeShared* shared_items)
+__global__ void __launch_bounds__(COMBINE_THREADS)
+    tree_combine_kernel(const TreeArgs a, int rows_per_item, int ctas, const float* pieces, const TreeShared* shared_items)
 {
     pdl_prologue();
-    const int cta = blockIdx.x, lane = threadIdx.x & 31;
-    const TreeShared item = shared_items[cta];
-    const int row = blockIdx.y * 4 + (threadIdx.x >> 5);
-    if (item.pieces == 0 || row >= rows_per_item || item.first_row + row >= item.nodes * a.group)
-        return;
-    const long long stride = 2 * tree_piece_floats(rows_per_item, D);
-    const auto piece = [&](int k)
-    { return pieces + (cta + k) * stride + (k == 0 ? stride / 2 : 0) + row * (D + TREE_PIECE_HEAD); };
-    float best = -INFINITY;
-    for (int k = lane; k < item.pieces; k += 32)
-        best = fmaxf(best, piece(k)[0]);
-#pragma unroll
-    for (int d = 16; d; d >>= 1)
-        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
-    constexpr int PER = D / 32;
-    float v[PER] = {}, total = 0.0f;
-    if (best != -INFINITY)
+    constexpr int PER = D / 32; // columns of one lane
+    __shared__ float part[COMBINE_WARPS][D + 2];
+    __shared__ int rows_until[COMBINE_THREADS], warp_sums[COMBINE_WARPS];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    int until = 0; // rows of the shared items up to the thread's
+    if (t < ctas)
     {
-#pragma unroll 4
-        for (int k = 0; k < item.pieces; ++k)
-        {
-            const float* from = piece(k);
-            const float scale = power_of_two(from[0] - best);
-            total = fmaf(from[1], scale, total);
-#pragma unroll
-            for (int j = 0; j < PER; ++j)
-                v[j] = fmaf(from[TREE_PIECE_HEAD + lane * PER + j], scale, v[j]);
-        }
+        const TreeShared s = shared_items[t];
+        until = s.pieces ? min(s.nodes * a.group - s.first_row, rows_per_item) : 0;
     }
-    const int node = (item.first_row + row) / a.group, in_group = item.first_row + row - node * a.group;
-    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-    std::uint16_t* to = a.out + item.entry * a.out_batch + node * a.out_node + (item.head * a.group + in_group) * a.out_head;
 #pragma unroll
-    for (int j = 0; j < PER; j += 2)
-        *reinterpret_cast<std::uint32_t*>(to + lane * PER + j) = Half2<T>::pack(v[j] * inverse, v[j + 1] * inverse);
-    if (a.lse && lane == 0)
-        a.lse[(static_cast<long long>(item.entry) * a.max_nodes + node) * a.heads * a.group + item.head * a.group + in_group] =
-            total == 0.0f ? -INFINITY : (best + log2f(total)) * 0.6931471805599453f;
+    for (int d = 1; d < 32; d <<= 1)
+    {
+        const int up = __shfl_up_sync(0xffffffffu, until, d);
+        until += lane >= d ? up : 0;
+    }
+    if (lane == 31)
+        warp_sums[warp] = until;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w)
+        until += warp_sums[w];
+    rows_until[t] = until;
+    __syncthreads();
+    const int rows = rows_until[COMBINE_THREADS - 1];
+    const int warps = static_cast<int>(gridDim.x) * COMBINE_WARPS;
+    const int shares = rows * 16 <= warps ? 16 : (rows * 4 <= warps ? 4 : 1); // warps of one row
+    const int at_once = COMBINE_WARPS / shares, share = warp & (shares - 1);
+    for (int first = blockIdx.x * at_once; first < rows; first += gridDim.x * at_once)
+    {
+        const int index = first + warp / shares;
+        const bool live = index < rows;
+        int cta = 0; // the first whose running count exceeds the row's
+        for (int step = COMBINE_THREADS / 2; step; step >>= 1)
+            cta += rows_until[cta + step - 1] <= (live ? index : 0) ? step : 0;
+        const TreeShared item = shared_items[cta];
+        const int row = index - (cta ? rows_until[cta - 1] : 0);
+        const long long stride = 2 * tree_piece_floats(rows_per_item, D);
+        const auto piece = [&](int k)
+        { return pieces + (cta + k) * stride + (k == 0 ? stride / 2 : 0) + row * (D + TREE_PIECE_HEAD); };
+        float best = -INFINITY, total = 0.0f, v[PER] = {};
+        constexpr int AHEAD = 4;
+        for (int k0 = share; live && k0 < item.pieces; k0 += AHEAD * shares)
+        {
+            float2 head[AHEAD]; // maximum and sum
+            float x[AHEAD][PER];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j)
+            {
+                const int k = k0 + j * shares;
+                head[j] = make_float2(-INFINITY, 0.0f);
+                if (k < item.pieces)
+                {
+                    const float* from = piece(k);
+                    head[j] = *reinterpret_cast<const float2*>(from);
+                    if constexpr (PER == 4)
+                        *reinterpret_cast<float4*>(x[j]) = *reinterpret_cast<const float4*>(from + TREE_PIECE_HEAD + 4 * lane);
+                    else
+                        *reinterpret_cast<float2*>(x[j]) = *reinterpret_cast<const float2*>(from + TREE_PIECE_HEAD + 2 * lane);
+                }
+                else
+                {
+#pragma unroll
+                    for (int c = 0; c < PER; ++c)
+                        x[j][c] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j)
+            {
+                const float raised = fmaxf(best, head[j].x), zero = raised == -INFINITY ? 0.0f : raised;
+                const float old_scale = power_of_two(best - zero), new_scale = power_of_two(head[j].x - zero);
+                best = raised;
+                total = fmaf(total, old_scale, head[j].y * new_scale);
+#pragma unroll
+                for (int c = 0; c < PER; ++c)
+                    v[c] = fmaf(v[c], old_scale, x[j][c] * new_scale);
+            }
+        }
+        if (shares > 1)
+        {
+            __syncthreads(); // the last rows have been read
+#pragma unroll
+            for (int c = 0; c < PER; ++c)
+                part[warp][lane * PER + c] = v[c];
+            if (lane == 0)
+            {
+                part[warp][D] = best;
+                part[warp][D + 1] = total;
+            }
+            __syncthreads();
+            if (share == 0)
+                for (int w = warp + 1; w < warp + shares; ++w)
+                {
+                    const float raised = fmaxf(best, part[w][D]), zero = raised == -INFINITY ? 0.0f : raised;
+                    const float old_scale = power_of_two(best - zero), new_scale = power_of_two(part[w][D] - zero);
+                    best = raised;
+                    total = fmaf(total, old_scale, part[w][D + 1] * new_scale);
+#pragma unroll
+                    for (int c = 0; c < PER; ++c)
+                        v[c] = fmaf(v[c], old_scale, part[w][lane * PER + c] * new_scale);
+                }
+        }
+        if (!live || share != 0)
+            continue;
+        const int node = (item.first_row + row) / a.group, in_group = item.first_row + row - node * a.group;
+        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+        std::uint16_t* to = a.out + item.entry * a.out_batch + node * a.out_node + (item.head * a.group + in_group) * a.out_head;
+#pragma unroll
+        for (int c = 0; c < PER; c += 2)
+            *reinterpret_cast<std::uint32_t*>(to + lane * PER + c) = Half2<T>::pack(v[c] * inverse, v[c + 1] * inverse);
+        if (a.lse && lane == 0)
+            a.lse[(static_cast<long long>(item.entry) * a.max_nodes + node) * a.heads * a.group + item.head * a.group + in_group] =
+                total == 0.0f ? -INFINITY : (best + log2f(total)) * 0.6931471805599453f;
+    }
 }
 
 int sms()
@@ -449,7 +534,7 @@ struct Shape
 {
     int ctas, rows;
     explicit Shape(int rows_per_head)
-        : ctas(tree_attention_many(rows_per_head) ? sms() : 2 * sms()),
+        : ctas(std::min(COMBINE_THREADS, tree_attention_many(rows_per_head) ? sms() : 2 * sms())),
           rows(tree_attention_many(rows_per_head) ? tree_attention_tc_rows(rows_per_head) : 16)
     {
     }
@@ -481,7 +566,7 @@ template <class T, int D> cudaError_t launch(const TreeArgs& a, ValueType type, 
     auto* items = reinterpret_cast<TreeShared*>(pieces + 2ll * shape.ctas * tree_piece_floats(shape.rows, D));
     if (tree_attention_many(rows))
     {
-        const cudaError_t status = tree_attention_tc(a, type, pieces, items, stream);
+        const cudaError_t status = tree_attention_tc(a, type, shape.ctas, pieces, items, stream);
         if (status != cudaSuccess)
             return status;
     }
@@ -489,7 +574,7 @@ template <class T, int D> cudaError_t launch(const TreeArgs& a, ValueType type, 
     {
         launch_few<T, D>(a, shape, pieces, items, stream);
     }
-    launch_pdl(tree_combine_kernel<T, D>, dim3(shape.ctas, (shape.rows + 3) / 4), dim3(128), 0, stream, a, shape.rows,
+    launch_pdl(tree_combine_kernel<T, D>, dim3(2 * sms()), dim3(COMBINE_THREADS), 0, stream, a, shape.rows, shape.ctas,
                static_cast<const float*>(pieces), static_cast<const TreeShared*>(items));
     note_launch();
     return cudaGetLastError();

@@ -36,7 +36,7 @@ struct TreeArgs
 // takes the units [U c / g, U (c + 1) / g): equal shares, none of them empty,
 // whatever the lengths, with at most two items of each CTA shared with its
 // neighbours.
-template <int KEYS, int ROWS> struct TreeWork
+template <int KEYS, int ROWS, int START> struct TreeWork
 {
     static constexpr int keys_per_tile = KEYS, rows_per_item = ROWS;
 
@@ -76,13 +76,22 @@ template <int KEYS, int ROWS> struct TreeWork
         e.last_base = e.length - (behind + e.nodes <= KEYS ? behind : e.length % (KEYS > 64 ? KEYS - 64 : 1));
         e.tiles = (e.last_base + KEYS - 1) / KEYS + 1;
         e.row_items = (e.nodes * a.group + ROWS - 1) / ROWS;
-        e.units = static_cast<long long>(e.tiles) * e.row_items * a.heads;
+        e.units = static_cast<long long>(START + e.tiles) * e.row_items * a.heads;
         return e;
     }
 
+    // By 32-bit division where it serves: the 64-bit one is a long routine.
+    static __device__ __forceinline__ long long quotient(long long n, long long d)
+    {
+        if (static_cast<unsigned long long>(n | d) >> 32)
+            return n / d;
+        return static_cast<unsigned>(n) / static_cast<unsigned>(d);
+    }
+    // units * cta / ctas
     static __device__ __forceinline__ long long first_unit(long long units, int cta, int ctas)
     {
-        return units * cta / ctas;
+        const long long q = quotient(units, ctas);
+        return q * cta + quotient((units - q * ctas) * cta, ctas);
     }
     // The CTA whose share holds unit u.
     static __device__ __forceinline__ int owner(long long units, long long u, int ctas)
@@ -96,6 +105,7 @@ template <int KEYS, int ROWS> struct TreeWork
         long long before; // units of the list entries before `entry`
         int entry;        // list entry that holds the CTA's first unit
         int ctas;         // CTAs that have a share
+        long long first, last; // the CTA's share
     };
 
     // The CTA's first list entry, by the whole CTA (THREADS threads, a multiple of 32).
@@ -118,7 +128,7 @@ template <int KEYS, int ROWS> struct TreeWork
         if (lane == 31)
             warp_sums[warp] = inclusive;
         if (threadIdx.x == 0)
-            *found = Start{0, 0, a.count, 0};
+            *found = Start{0, 0, a.count, 0, 0, 0};
         __syncthreads();
         long long before = 0, units = 0;
         for (int w = 0; w < THREADS / 32; ++w)
@@ -129,6 +139,7 @@ template <int KEYS, int ROWS> struct TreeWork
         before += inclusive - mine;
         const int sharing = units < ctas ? static_cast<int>(units) : ctas;
         const long long u = cta < sharing ? first_unit(units, cta, sharing) : units;
+        const long long last = cta < sharing ? first_unit(units, cta + 1, sharing) : units;
         if (u >= before && u < before + mine)
         {
             for (int i = begin; i < end; ++i)
@@ -136,7 +147,7 @@ template <int KEYS, int ROWS> struct TreeWork
                 const long long n = entry(a, i).units;
                 if (u < before + n)
                 {
-                    *found = Start{units, before, i, sharing};
+                    *found = Start{units, before, i, sharing, u, last};
                     break;
                 }
                 before += n;
@@ -163,9 +174,8 @@ template <int KEYS, int ROWS> struct TreeWork
         long long unit, last_unit, before;
         int list_entry;
 
-        __device__ __forceinline__ Cursor(const Start& s, int cta)
-            : unit(first_unit(s.units, cta, s.ctas)), last_unit(first_unit(s.units, cta + 1, s.ctas)),
-              before(s.before), list_entry(s.entry)
+        __device__ __forceinline__ explicit Cursor(const Start& s)
+            : unit(s.first), last_unit(s.last), before(s.before), list_entry(s.entry)
         {
         }
         __device__ __forceinline__ bool next(const TreeArgs& a, Segment& s)
@@ -179,15 +189,17 @@ template <int KEYS, int ROWS> struct TreeWork
                     ++list_entry;
                     continue;
                 }
-                const int item = static_cast<int>((unit - before) / s.e.tiles);
+                const int item = static_cast<int>(quotient(unit - before, START + s.e.tiles));
                 s.list_entry = list_entry;
                 s.head = item / s.e.row_items;
                 s.first_row = (item - s.head * s.e.row_items) * ROWS;
                 s.rows = s.e.nodes * a.group;
-                s.item_start = before + static_cast<long long>(item) * s.e.tiles;
-                s.tile_begin = static_cast<int>(unit - s.item_start);
+                s.item_start = before + static_cast<long long>(item) * (START + s.e.tiles) + START; // its first tile's unit
+                s.tile_begin = static_cast<int>(max(unit - s.item_start, 0ll));
                 s.tile_end = static_cast<int>(min(static_cast<long long>(s.e.tiles), last_unit - s.item_start));
-                unit = s.item_start + s.tile_end;
+                unit = s.item_start + max(s.tile_end, 0);
+                if (s.tile_begin >= s.tile_end) // the share ends before the item's first tile
+                    continue;
                 return true;
             }
             return false;
@@ -241,38 +253,49 @@ template <int KEYS, int ROWS> struct TreeWork
     }
 };
 
-// Bit a of masks[n]: node a is node n or one of its ancestors.  Pointer
-// doubling: log2(64) rounds in place of a walk of up to 64 dependent steps.
-// A parent below -1 makes a node that sees no drafted node, not even itself;
-// one that is not before its child is reported and treated as such.
-// Called by at least 64 threads, numbered from 0; `sync` is their barrier.
-template <class Sync>
-__device__ __forceinline__ void ancestor_masks(const int* parents, int nodes, unsigned long long* masks, int* above,
-                                               unsigned* error_word, int t, Sync&& sync)
+// Bit a of masks[n]: node a is node n or one of its ancestors.  By one warp, two
+// nodes per lane, with pointer doubling: log2(64) rounds in place of a walk of
+// up to 64 dependent steps.  A parent below -1 makes a node that sees no
+// drafted node, not even itself; one that is not before its child is reported
+// and treated as such.
+__device__ __forceinline__ void ancestor_masks(const int* parents, int nodes, unsigned long long* masks,
+                                               unsigned* error_word, int lane)
 {
-    if (t < DRAFT_MAX_NODES)
+    unsigned long long mask[2];
+    int above[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
     {
-        const int parent = t < nodes ? parents[t] : -2;
-        const bool wrong = parent >= t;
+        const int n = lane + 32 * k;
+        const int parent = n < nodes ? parents[n] : -2;
+        const bool wrong = parent >= n;
         if (wrong && error_word)
             atomicOr(error_word, error_cache);
-        masks[t] = parent < -1 || wrong ? 0ull : 1ull << t;
-        above[t] = wrong || parent < 0 ? -1 : parent;
+        mask[k] = parent < -1 || wrong ? 0ull : 1ull << n;
+        above[k] = wrong || parent < 0 ? -1 : parent;
     }
-    sync();
     for (int round = 0; round < 6; ++round)
     {
-        const int up = t < DRAFT_MAX_NODES ? above[t] : -1;
-        const unsigned long long mask = up >= 0 ? masks[up] : 0ull;
-        const int next = up >= 0 ? above[up] : -1;
-        sync();
-        if (t < DRAFT_MAX_NODES)
+        unsigned long long more[2];
+        int next[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
         {
-            masks[t] |= mask;
-            above[t] = next;
+            const int from = above[k] & 31;
+            const unsigned long long low = __shfl_sync(0xffffffffu, mask[0], from), high = __shfl_sync(0xffffffffu, mask[1], from);
+            const int low_above = __shfl_sync(0xffffffffu, above[0], from), high_above = __shfl_sync(0xffffffffu, above[1], from);
+            more[k] = above[k] < 0 ? 0ull : (above[k] < 32 ? low : high);
+            next[k] = above[k] < 0 ? -1 : (above[k] < 32 ? low_above : high_above);
         }
-        sync();
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+        {
+            mask[k] |= more[k];
+            above[k] = next[k];
+        }
     }
+    masks[lane] = mask[0];
+    masks[lane + 32] = mask[1];
 }
 
 // What a CTA leaves for the combining launch: the item it began and did not finish.
@@ -294,7 +317,7 @@ inline __host__ __device__ long long tree_piece_floats(int rows, int head_dim)
 bool tree_attention_many(int rows);
 size_t tree_attention_scratch(int head_dim, int rows);
 cudaError_t tree_attention(const TreeArgs& a, ValueType type, void* scratch, cudaStream_t stream);
-cudaError_t tree_attention_tc(const TreeArgs& a, ValueType type, float* pieces, TreeShared* shared_items,
+cudaError_t tree_attention_tc(const TreeArgs& a, ValueType type, int ctas, float* pieces, TreeShared* shared_items,
                               cudaStream_t stream);
 int tree_attention_tc_rows(int rows); // rows of one of its items
 } // namespace tsacb::dev

@@ -10,7 +10,7 @@
 // keys and values cross HBM once, and the kernel is bound by HBM as long as
 // products, exponentials and loads overlap.
 //
-// One CTA per SM, 11 warps:
+// One CTA per SM, 12 warps:
 //   warps 0-3, 4-7  two softmax groups, one query row per thread.  Each has its
 //                   own scores S and output O in TMEM.  With 256 rows each
 //                   group has 128 of them and sees every tile; with 128 rows
@@ -29,6 +29,8 @@
 //                   fewer than 8 rows (a swizzle atom), or 2^31 rows in a plane.  Copies of every tile by the two warps
 //                   bound the kernel by their address arithmetic (290 against
 //                   BATCH_TREES us for 64 x 16 nodes over up to 4,096 positions).
+//   warp 11         the query rows of the next segment, as soon as the last
+//                   scores of this one are made, and its tree's masks.
 // The running maximum moves only when a row's tile exceeds it by more than 8
 // (in powers of two): p then stays below 256, which bf16, fp16 and the 32-bit
 // sums hold as well as 1, and the output in TMEM is rescaled rarely.  So a tile
@@ -53,10 +55,11 @@ using namespace tc;
 
 constexpr int KEYS = 128;
 constexpr int GROUP_THREADS = 128, SOFTMAX_THREADS = 2 * GROUP_THREADS;
-// Eleven warps leave each thread 168 registers; a 13th warp would leave 128,
-// and the softmax threads would spill.
+// Twelve warps leave each thread 168 registers; a 13th would leave 128, and the
+// softmax threads would spill.
 constexpr int MMA_WARP = 8, PRODUCER_WARP = 9, PRODUCERS = 64, PRODUCER_ROWS = KEYS / 2;
-constexpr int THREADS = PRODUCER_WARP * 32 + PRODUCERS;
+constexpr int QUERY_WARP = PRODUCER_WARP + PRODUCERS / 32;
+constexpr int THREADS = (QUERY_WARP + 1) * 32;
 constexpr int TMEM_COLUMNS = 512, OUTPUT_COLUMN = 256; // S of the groups at 0 and 128, O at 256 and 384
 constexpr float RESCALE = 8.0f;                        // powers of two
 constexpr int TAINT_SLOTS = 16; // segments that the producers can be ahead of the epilogue, and more
@@ -71,26 +74,24 @@ template <int D, bool TWO> struct Tiles
     static constexpr int chunks = D / 8;
     static constexpr int ring_offset = query_bytes;
     static constexpr int tail_offset = ring_offset + SLOTS * operand_bytes;
-    static constexpr int tail_bytes = TWO ? 2048 : 4096; // barriers and small arrays
+    static constexpr int tail_bytes = TWO && D == 128 ? 2048 : 5120; // barriers and small arrays
     static constexpr int smem = tail_offset + tail_bytes + 1024; // the rest: alignment
     static_assert(smem <= 227 * 1024, "shared memory of one SM");
 };
 
-template <bool TWO> struct Tail
+template <int SLOTS, bool TWO> struct Tail
 {
-    uint64_t full[10], empty[10];
-    uint64_t scores[2], weights[2], products[2], query, drain;
-    unsigned long long masks[DRAFT_MAX_NODES];
+    uint64_t full[SLOTS], empty[SLOTS];
+    uint64_t scores[2], weights[2], products[2], query, query_free, done, drain;
+    // The softmax threads read the masks of a segment at its start; the query warp may be two ahead.
+    unsigned long long masks[3][DRAFT_MAX_NODES];
     unsigned long long tainted[TAINT_SLOTS];
     long long warp_sums[THREADS / 32];
     float maximum[2][TWO ? 1 : GROUP_THREADS], sum[2][TWO ? 1 : GROUP_THREADS]; // of the groups' shares of a row
-    int above[DRAFT_MAX_NODES];
-    long long start[4]; // TreeWork::Start
+    long long start[6]; // TreeWork::Start
     uint32_t tmem;
     int abort;
 };
-static_assert(sizeof(Tail<true>) <= 2048 && sizeof(Tail<false>) <= 4096, "tail of the shared memory");
-
 __device__ __forceinline__ uint32_t tmem_load1(uint32_t address)
 {
     uint32_t r;
@@ -250,11 +251,13 @@ __global__ void __launch_bounds__(THREADS, 1)
 {
     pdl_prologue();
     using L = Tiles<D, TWO>;
-    using Work = TreeWork<KEYS, L::ROWS>;
+    using Work = TreeWork<KEYS, L::ROWS, 3>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                            ~static_cast<uintptr_t>(1023));
-    Tail<TWO>& tail = *reinterpret_cast<Tail<TWO>*>(smem + L::tail_offset);
+    using TailOf = Tail<L::SLOTS, TWO>;
+    static_assert(sizeof(TailOf) <= L::tail_bytes, "tail of the shared memory");
+    TailOf& tail = *reinterpret_cast<TailOf*>(smem + L::tail_offset);
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
     const int cta = blockIdx.x;
     static_assert(sizeof(typename Work::Start) <= sizeof(tail.start));
@@ -277,7 +280,9 @@ __global__ void __launch_bounds__(THREADS, 1)
             bar_init(smem_u32(&tail.weights[g]), GROUP_THREADS);
             bar_init(smem_u32(&tail.products[g]), 1);
         }
-        bar_init(smem_u32(&tail.query), SOFTMAX_THREADS);
+        bar_init(smem_u32(&tail.query), 1);
+        bar_init(smem_u32(&tail.query_free), SOFTMAX_THREADS + 1);
+        bar_init(smem_u32(&tail.done), SOFTMAX_THREADS);
         bar_init(smem_u32(&tail.drain), 1);
         for (int k = 0; k < TAINT_SLOTS; ++k)
             tail.tainted[k] = 0;
@@ -308,10 +313,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         return ok;
     };
-    typename Work::Cursor cursor(start, cta);
+    typename Work::Cursor cursor(start);
     typename Work::Segment g;
 
-    if (warp >= PRODUCER_WARP)
+    if (warp >= PRODUCER_WARP && warp < QUERY_WARP)
     {
         // ------------------------------------------------------------ producers --
         const int first_row = (warp - PRODUCER_WARP) * PRODUCER_ROWS; // this warp's rows of each tile
@@ -319,7 +324,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int boxes = box_rows ? PRODUCER_ROWS / box_rows * panels : 0; // of this warp's half tile
         int slot = 0, round = 0; // uses of the slot so far
         int copied = -1, copied_segment = 0; // a slot whose copies have been issued and not yet announced
-        int copied_nodes = -1; // its first drafted row; -1: none
+        int copied_draft = -1, copied_nodes = 0; // its first drafted row, -1: none; drafted rows
         // Announces the copied slot, once its copies have landed: all but the newest `behind` group.
         const auto announce = [&](bool behind)
         {
@@ -329,23 +334,25 @@ __global__ void __launch_bounds__(THREADS, 1)
                 asm volatile("cp.async.wait_group 1;" ::: "memory");
             else
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
-            if (copied_nodes >= 0)
+            if (copied_draft >= 0)
             {
                 // 0 x NaN would reach rows that do not see the node: values that are not
                 // finite leave the product and are added where they are seen.
-                for (int i = 0; i < PRODUCER_ROWS / rows_at_once; ++i)
+                const int chunk = lane % L::chunks;
+                const int end = min(first_row + PRODUCER_ROWS, copied_draft + copied_nodes);
+#pragma unroll 2
+                for (int row = max(first_row, copied_draft) + lane / L::chunks; row < end; row += rows_at_once)
                 {
-                    const int row = first_row + i * rows_at_once + lane / L::chunks, chunk = lane % L::chunks;
                     auto* at = reinterpret_cast<uint4*>(smem + L::ring_offset + copied * L::operand_bytes +
                                                         (chunk >> 3) * L::panel_bytes + row * 128 +
                                                         (((chunk & 7) ^ (row & 7)) << 4));
                     const uint4 v = *at;
                     const uint32_t odd[4] = {nonfinite_mask<T>(v.x), nonfinite_mask<T>(v.y), nonfinite_mask<T>(v.z),
                                              nonfinite_mask<T>(v.w)};
-                    if (row >= copied_nodes && (odd[0] | odd[1] | odd[2] | odd[3]))
+                    if (odd[0] | odd[1] | odd[2] | odd[3])
                     {
                         *at = make_uint4(v.x & ~odd[0], v.y & ~odd[1], v.z & ~odd[2], v.w & ~odd[3]);
-                        atomicOr(&tail.tainted[copied_segment % TAINT_SLOTS], 1ull << ((row - copied_nodes) & 63));
+                        atomicOr(&tail.tainted[copied_segment % TAINT_SLOTS], 1ull << ((row - copied_draft) & 63));
                     }
                 }
             }
@@ -424,7 +431,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                     asm volatile("cp.async.commit_group;" ::: "memory");
                     announce(true);
                     copied = slot;
-                    copied_nodes = Work::is_last(g, tile) && value ? g.e.length - g.e.last_base : -1;
+                    copied_draft = Work::is_last(g, tile) && value ? g.e.length - g.e.last_base : -1;
+                    copied_nodes = g.e.nodes;
                     copied_segment = segment;
                 }
                 if (++slot == L::SLOTS)
@@ -442,6 +450,64 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int used = round * L::SLOTS + slot; // operands issued; every earlier use of a slot was waited for
             for (int n = used > L::SLOTS ? used - L::SLOTS : 0; n < used; ++n)
                 bar_wait(smem_u32(&tail.full[n % L::SLOTS]), static_cast<uint32_t>(n / L::SLOTS & 1), &never);
+        }
+    }
+    else if (warp == QUERY_WARP)
+    {
+        // -------------------------------------------------------------- queries --
+        // A negative scale turns the query's signs and a zero one clears it, so that the
+        // softmax's factor is positive: the largest product is the largest score.
+        const uint32_t turn = a.scale_log2 < 0.0f ? 0x80008000u : 0u, keep = a.scale_log2 == 0.0f ? 0u : ~0u;
+        constexpr int rows_at_once = 32 / L::chunks;
+        const int chunk = lane % L::chunks;
+        for (int segment = 0; ok && cursor.next(a, g); ++segment)
+        {
+            const bool has_draft = g.tile_end == g.e.tiles;
+            if (has_draft)
+                ancestor_masks(a.parents + static_cast<long long>(g.list_entry) * a.max_nodes, g.e.nodes,
+                               tail.masks[segment % 3], a.error_word, lane);
+            wait(tail.query_free, segment + 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok)
+                break;
+            const auto place = [&](int row) // of the item
+            {
+                return (chunk >> 3) * L::panel_bytes + (row >> 7) * L::operand_bytes + (row & 127) * 128 +
+                       (((chunk & 7) ^ (row & 7)) << 4);
+            };
+            // A lane finds the place of one row in 32; the copies take it by shuffle.
+            const std::uint16_t* from = a.query + g.list_entry * a.query_batch + 8 * chunk;
+            for (int block = 0; block < L::ROWS; block += 32)
+            {
+                const int mine = g.first_row + block + lane, node = mine / a.group;
+                const long long offset = node * a.query_node + (g.head * a.group + mine - node * a.group) * a.query_head;
+                if (g.first_row + block >= g.rows) // nothing but zeros from here on
+                {
+                    for (int row = block + lane / L::chunks; row < L::ROWS; row += rows_at_once)
+                        *reinterpret_cast<uint4*>(smem + place(row)) = make_uint4(0, 0, 0, 0);
+                    break;
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i += rows_at_once)
+                {
+                    const int in_block = i + lane / L::chunks;
+                    const bool live = g.first_row + block + in_block < g.rows;
+                    const long long at = __shfl_sync(0xffffffffu, offset, in_block);
+                    copy_16(smem_u32(smem) + place(block + in_block), live ? from + at : a.query, live ? 16u : 0u);
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (a.scale_log2 <= 0.0f)
+                for (int row = lane / L::chunks; row < L::ROWS; row += rows_at_once)
+                {
+                    auto* at = reinterpret_cast<uint4*>(smem + place(row));
+                    const uint4 v = *at;
+                    *at = make_uint4((v.x ^ turn) & keep, (v.y ^ turn) & keep, (v.z ^ turn) & keep, (v.w ^ turn) & keep);
+                }
+            fence_async_proxy();
+            __syncwarp();
+            if (lane == 0)
+                bar_arrive(smem_u32(&tail.query));
         }
     }
     else if (warp == MMA_WARP)
@@ -508,16 +574,25 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (ok)
                 commit_if(leader, smem_u32(&tail.empty[s]));
         };
+        const auto free_query = [&]
+        {
+            if (ok)
+                commit_if(leader, smem_u32(&tail.query_free));
+        };
         for (int segment = 0; ok && uniform(cursor.next(a, g)); ++segment)
         {
             const int tiles = uniform(g.tile_end - g.tile_begin);
             wait_all(tail.query, segment);
+            if (segment) // the softmax threads have read the last segment's P and O
+                wait_all(tail.done, segment - 1);
             if constexpr (TWO)
             {
                 int k = take();
                 score(0, k);
                 score(1, k);
                 free_slot(k);
+                if (tiles == 1)
+                    free_query();
                 for (int j = 0; j < tiles && ok; ++j)
                 {
                     const int v = take();
@@ -536,6 +611,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                         after_product(1);
                         score(1, k);
                         free_slot(k);
+                        if (j + 2 == tiles)
+                            free_query();
                     }
                 }
             }
@@ -547,6 +624,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                     score(j, k);
                     free_slot(k);
                 }
+                if (tiles <= 2)
+                    free_query();
                 for (int j = 0; j < tiles && ok; ++j)
                 {
                     const int v = take();
@@ -558,6 +637,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                         after_product(j & 1);
                         score(j & 1, k);
                         free_slot(k);
+                        if (j + 3 == tiles)
+                            free_query();
                     }
                 }
             }
@@ -575,10 +656,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int group = warp >> 2, row = t & (GROUP_THREADS - 1);
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t my_scores = lanes + group * KEYS, my_output = lanes + OUTPUT_COLUMN + group * 128;
-        // A negative scale turns the query's signs and a zero one clears it, so that the
-        // factor is positive: the largest product is the largest score, and -infinity stays.
-        const uint32_t turn = a.scale_log2 < 0.0f ? 0x80008000u : 0u, keep = a.scale_log2 == 0.0f ? 0u : ~0u;
-        const float scale = a.scale_log2 == 0.0f ? 1.0f : fabsf(a.scale_log2);
+        const float scale = a.scale_log2 == 0.0f ? 1.0f : fabsf(a.scale_log2); // the query has its sign
         int scores_seen = 0;
         Both<int> products_seen{0, 0};
         for (int segment = 0; cursor.next(a, g); ++segment)
@@ -589,28 +667,9 @@ __global__ void __launch_bounds__(THREADS, 1)
             const bool live = g.first_row + item_row < g.rows;
             const int node = live ? (g.first_row + item_row) / a.group : 0;
             const int query_head = g.head * a.group + (g.first_row + item_row - node * a.group);
-            {
-                // With 128 rows the groups load half a row each.
-                constexpr int mine = TWO ? L::chunks : L::chunks / 2;
-                const int first_chunk = TWO ? 0 : group * mine;
-                const std::uint16_t* from = a.query + g.list_entry * a.query_batch + node * a.query_node +
-                                            query_head * a.query_head;
-                unsigned char* to = smem + (TWO ? group * L::operand_bytes : 0) + row * 128;
-#pragma unroll 4
-                for (int c = 0; c < mine; ++c)
-                {
-                    const int chunk = first_chunk + c;
-                    uint4 v = live ? *reinterpret_cast<const uint4*>(from + 8 * chunk) : make_uint4(0, 0, 0, 0);
-                    v = make_uint4((v.x ^ turn) & keep, (v.y ^ turn) & keep, (v.z ^ turn) & keep, (v.w ^ turn) & keep);
-                    *reinterpret_cast<uint4*>(to + (chunk >> 3) * L::panel_bytes + (((chunk & 7) ^ (row & 7)) << 4)) = v;
-                }
-                fence_async_proxy();
-                bar_arrive(smem_u32(&tail.query));
-            }
-            if (has_draft)
-                ancestor_masks(a.parents + static_cast<long long>(g.list_entry) * a.max_nodes, g.e.nodes, tail.masks,
-                               tail.above, group == 0 && warp < 2 ? a.error_word : nullptr, t, [] { softmax_sync(); });
-            const unsigned long long sees = has_draft && live ? tail.masks[node] : 0ull;
+            wait(tail.query, segment); // the masks are there
+            const unsigned long long sees = has_draft && live ? tail.masks[segment % 3][node] : 0ull;
+            bar_arrive(smem_u32(&tail.query_free)); // the masks are read; the MMA warp adds that the rows are
 
             // A warp without a live row has nothing to compute: whatever its lanes of TMEM hold stays there.
             const bool busy = __any_sync(0xffffffffu, live);
@@ -833,10 +892,14 @@ __global__ void __launch_bounds__(THREADS, 1)
                 shared_items[cta] = TreeShared{g.list_entry, g.head, g.first_row,
                                                Work::owner(start.units, g.item_start + g.e.tiles - 1, start.ctas) - cta + 1,
                                                g.e.nodes};
-            tc_fence_before();
-            softmax_sync(); // outputs, masks and statistics of this segment are done with
-            if (t == 0)
+            if constexpr (!TWO)
+                softmax_sync(); // the groups' statistics and the tainted nodes have been read
+            else if (tainted)
+                softmax_sync();
+            if (t == 0 && tainted)
                 tail.tainted[segment % TAINT_SLOTS] = 0;
+            tc_fence_before();
+            bar_arrive(smem_u32(&tail.done));
         }
     }
 
@@ -867,7 +930,7 @@ bool make_map(CUtensorMap* map, const TreeArgs& a, int rows)
 }
 
 template <class T, int D, bool TWO>
-void launch(const TreeArgs& a, float* pieces, TreeShared* shared_items, cudaStream_t stream)
+void launch(const TreeArgs& a, int ctas, float* pieces, TreeShared* shared_items, cudaStream_t stream)
 {
     using L = Tiles<D, TWO>;
     static std::once_flag once[64];
@@ -885,19 +948,19 @@ void launch(const TreeArgs& a, float* pieces, TreeShared* shared_items, cudaStre
     int box_rows = a.cache.page_size() < PRODUCER_ROWS ? a.cache.page_size() : PRODUCER_ROWS;
     if (box_rows < 8 || !make_map(&map, a, box_rows))
         box_rows = 0;
-    launch_pdl(tree_attention_tc_kernel<T, D, TWO>, dim3(sm_count()), dim3(THREADS), L::smem, stream, map, a, box_rows,
+    launch_pdl(tree_attention_tc_kernel<T, D, TWO>, dim3(ctas), dim3(THREADS), L::smem, stream, map, a, box_rows,
                pieces, shared_items);
     note_launch();
 }
 
 template <class T>
-void launch_shape(const TreeArgs& a, float* pieces, TreeShared* shared_items, cudaStream_t stream)
+void launch_shape(const TreeArgs& a, int ctas, float* pieces, TreeShared* shared_items, cudaStream_t stream)
 {
     const bool two = tree_attention_tc_rows(a.max_nodes * a.group) == 256;
     if (a.head_dim == 64)
-        two ? launch<T, 64, true>(a, pieces, shared_items, stream) : launch<T, 64, false>(a, pieces, shared_items, stream);
+        two ? launch<T, 64, true>(a, ctas, pieces, shared_items, stream) : launch<T, 64, false>(a, ctas, pieces, shared_items, stream);
     else
-        two ? launch<T, 128, true>(a, pieces, shared_items, stream) : launch<T, 128, false>(a, pieces, shared_items, stream);
+        two ? launch<T, 128, true>(a, ctas, pieces, shared_items, stream) : launch<T, 128, false>(a, ctas, pieces, shared_items, stream);
 }
 } // namespace
 
@@ -906,13 +969,13 @@ int tree_attention_tc_rows(int rows)
     return rows > 128 ? 256 : 128;
 }
 
-cudaError_t tree_attention_tc(const TreeArgs& a, ValueType type, float* pieces, TreeShared* shared_items,
+cudaError_t tree_attention_tc(const TreeArgs& a, ValueType type, int ctas, float* pieces, TreeShared* shared_items,
                               cudaStream_t stream)
 {
     if (type == ValueType::bf16)
-        launch_shape<__nv_bfloat16>(a, pieces, shared_items, stream);
+        launch_shape<__nv_bfloat16>(a, ctas, pieces, shared_items, stream);
     else
-        launch_shape<__half>(a, pieces, shared_items, stream);
+        launch_shape<__half>(a, ctas, pieces, shared_items, stream);
     return cudaGetLastError();
 }
 } // namespace tsacb::dev
