@@ -70,16 +70,16 @@ template <int D, bool TWO> struct Tiles
     static constexpr int panel_bytes = KEYS * 128;           // 64 columns of 128 rows
     static constexpr int operand_bytes = panel_bytes * (D / 64);
     static constexpr int query_bytes = operand_bytes * (ROWS / 128);
-    static constexpr int SLOTS = D == 128 ? 5 : 10;
+    static constexpr int SLOTS = (TWO ? 160 : 192) * 1024 / operand_bytes;
     static constexpr int chunks = D / 8;
     static constexpr int ring_offset = query_bytes;
     static constexpr int tail_offset = ring_offset + SLOTS * operand_bytes;
-    static constexpr int tail_bytes = TWO && D == 128 ? 2048 : 5120; // barriers and small arrays
+    static constexpr int tail_bytes = D == 128 ? 2048 : 4096; // barriers and small arrays
     static constexpr int smem = tail_offset + tail_bytes + 1024; // the rest: alignment
     static_assert(smem <= 227 * 1024, "shared memory of one SM");
 };
 
-template <int SLOTS, bool TWO> struct Tail
+template <int SLOTS> struct Tail
 {
     uint64_t full[SLOTS], empty[SLOTS];
     uint64_t scores[2], weights[2], products[2], query, query_free, done, drain;
@@ -87,7 +87,6 @@ template <int SLOTS, bool TWO> struct Tail
     unsigned long long masks[3][DRAFT_MAX_NODES];
     unsigned long long tainted[TAINT_SLOTS];
     long long warp_sums[THREADS / 32];
-    float maximum[2][TWO ? 1 : GROUP_THREADS], sum[2][TWO ? 1 : GROUP_THREADS]; // of the groups' shares of a row
     long long start[6]; // TreeWork::Start
     uint32_t tmem;
     int abort;
@@ -120,6 +119,11 @@ __device__ __forceinline__ void tmem_store16(uint32_t address, const uint32_t* r
                  "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
                  "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
+}
+
+__device__ __forceinline__ void tmem_store2(uint32_t address, uint32_t a, uint32_t b)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};" ::"r"(address), "r"(a), "r"(b) : "memory");
 }
 
 __device__ __forceinline__ void tmem_wait_stores()
@@ -255,7 +259,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                            ~static_cast<uintptr_t>(1023));
-    using TailOf = Tail<L::SLOTS, TWO>;
+    using TailOf = Tail<L::SLOTS>;
     static_assert(sizeof(TailOf) <= L::tail_bytes, "tail of the shared memory");
     TailOf& tail = *reinterpret_cast<TailOf*>(smem + L::tail_offset);
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
@@ -780,17 +784,22 @@ __global__ void __launch_bounds__(THREADS, 1)
             Both<float> part{1.0f, 1.0f}; // factors of the groups' outputs
             if constexpr (!TWO)
             {
-                tail.maximum[group][row] = maximum;
-                tail.sum[group][row] = sum;
+                // The groups exchange their statistics in TMEM, in columns of S that P leaves free.
+                tmem_store2(my_scores + KEYS / 2, __float_as_uint(maximum), __float_as_uint(sum));
+                tmem_wait_stores();
+                tc_fence_before();
                 softmax_sync();
                 // The other group has seen its product complete; this makes it visible here.
                 if (made(1 - group))
                     wait(tail.products[1 - group], products_seen(1 - group) + made(1 - group) - 1);
-                const float m0 = tail.maximum[0][row], m1 = tail.maximum[1][row];
+                __syncwarp();
+                tc_fence_after();
+                const float m0 = __uint_as_float(tmem_load1(lanes + KEYS / 2)), m1 = __uint_as_float(tmem_load1(lanes + KEYS + KEYS / 2));
+                const float sum0 = __uint_as_float(tmem_load1(lanes + KEYS / 2 + 1)), sum1 = __uint_as_float(tmem_load1(lanes + KEYS + KEYS / 2 + 1));
                 maximum = fmaxf(m0, m1);
                 part.first = m0 == -INFINITY ? 0.0f : power_of_two(m0 - maximum);
                 part.second = m1 == -INFINITY ? 0.0f : power_of_two(m1 - maximum);
-                sum = tail.sum[0][row] * part.first + tail.sum[1][row] * part.second;
+                sum = sum0 * part.first + sum1 * part.second;
             }
             __syncwarp();
             tc_fence_after();
