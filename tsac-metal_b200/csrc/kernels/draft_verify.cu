@@ -15,12 +15,13 @@
 // B200 mapping.  Only the last node's rows are read whole, so a call is bound
 // by one row of p (and one of q) per sequence: latency for small vocabularies,
 // HBM for large ones.  The gathers p(x), q(x) of every node are loaded at once
-// before the walk, which then runs redundantly in every thread from shared
-// memory.  A whole-row pass is spread over a cluster of CTAs: each warp owns a
-// contiguous range of the row and sums it with 16-byte loads, the ranges' sums
-// are exchanged through distributed shared memory (one cluster barrier per
-// pass), and the CTA that owns the crossing range reads it once more, from
-// cache, to find the token.
+// before the walk.  Each warp then walks for itself: its lanes hold two nodes
+// each, a ballot finds the children of the current node, and nothing waits for
+// another warp.  A whole-row pass is spread over a cluster of CTAs: each warp
+// owns a contiguous range of the row and sums it with 16-byte loads, the
+// ranges' sums are exchanged through distributed shared memory (one cluster
+// barrier per pass), and the CTA that owns the crossing range reads it once
+// more, from cache, to find the token.
 //
 // All sums and the excess are in 64 bits: the token is an integer that one
 // rounding near a border would change, and 32-bit partial sums over 10^5
@@ -31,9 +32,12 @@
 #include "kernels/launch_count.hpp"
 #include "kernels/pdl.cuh"
 
+#include <algorithm>
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 namespace tsacb::dev
 {
@@ -41,8 +45,7 @@ namespace
 {
 namespace cg = cooperative_groups;
 
-constexpr int THREADS = 256, WARPS = THREADS / 32;
-constexpr int WIDE = 8; // CTAs of a cluster for a large vocabulary
+constexpr int MAX_RANGES = 128; // warps of a cluster, at most: 8 CTAs of 512 threads
 
 __device__ __forceinline__ double to_double(float v) { return v; }
 __device__ __forceinline__ double to_double(__half v) { return __half2float(v); }
@@ -54,27 +57,57 @@ template <class T> struct alignas(16) Vector
     T v[N];
 };
 
+// The same 16 bytes as words.
+struct Words
+{
+    std::uint32_t w[4];
+    __device__ __forceinline__ Words() : w{0, 0, 0, 0} {}
+    __device__ __forceinline__ explicit Words(const uint4& v) : w{v.x, v.y, v.z, v.w} {}
+    template <class T> __device__ __forceinline__ double value(int j) const
+    {
+        if constexpr (sizeof(T) == 4)
+            return __uint_as_float(w[j]);
+        else if constexpr (std::is_same_v<T, __half>)
+            return to_double(__ushort_as_half(static_cast<unsigned short>(j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu)));
+        else // a bf16 value is the upper half of a 32-bit one
+            return __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+    }
+};
+
 struct Shared
 {
     int parents[DRAFT_MAX_NODES], tokens[DRAFT_MAX_NODES], path[DRAFT_MAX_NODES];
     float coins[DRAFT_MAX_NODES];
     double p[DRAFT_MAX_NODES], q[DRAFT_MAX_NODES];
-    double scale[DRAFT_MAX_NODES];           // 1 / Z of each round of rejections
-    int rejected[DRAFT_MAX_NODES];           // tokens rejected at the current node
-    double sums[2][WIDE * WARPS];            // sums of the warps' ranges, by pass parity
-    double scan[WARPS];
+    double scale[DRAFT_MAX_NODES]; // 1 / Z of each round of rejections
+    double sums[2][MAX_RANGES];    // sums of the warps' ranges, by pass parity
+    double scan[16];               // of a CTA's warps
     int first;
 };
 
-// The weights at the current node: the target's row, reduced once per round.
+// The weights at the current node.  With a draft: the target's row after
+// `rounds` applications of max(w / Z - q, 0); else: without the tokens of the
+// rejected nodes, of which a warp keeps those that lie in its range.
 template <class T, bool DRAFT> struct Weights
 {
     const T* p;
     const T* q;
-    int rounds; // with a draft: applications of max(w / Z - q, 0); else: rejected tokens
+    int rounds;
     const double* scale;
-    const int* rejected;
+    unsigned long long rejected; // nodes
+    const int* tokens;           // of the nodes
 
+    __device__ __forceinline__ void keep(int first, int last)
+    {
+        if constexpr (!DRAFT)
+        {
+            const int lane = threadIdx.x & 31;
+            const auto inside = [&](int n)
+            { return (rejected >> n & 1ull) && tokens[n] >= first && tokens[n] < last; };
+            const unsigned low = __ballot_sync(0xffffffffu, inside(lane)), high = __ballot_sync(0xffffffffu, inside(lane + 32));
+            rejected = static_cast<unsigned long long>(high) << 32 | low;
+        }
+    }
     __device__ __forceinline__ double excess(double w, double q_value) const
     {
         if (rounds > 0)
@@ -93,8 +126,8 @@ template <class T, bool DRAFT> struct Weights
         else
         {
 #pragma unroll 1
-            for (int i = 0; i < rounds; ++i)
-                p_value = rejected[i] == token ? 0.0 : p_value;
+            for (unsigned long long rest = rejected; rest; rest &= rest - 1)
+                p_value = tokens[__ffsll(static_cast<long long>(rest)) - 1] == token ? 0.0 : p_value;
             return p_value;
         }
     }
@@ -120,6 +153,10 @@ template <class T, bool DRAFT> struct Row
         vectors = !DRAFT || skew_of(q) == skew;
         blocks = (vocab + skew + N - 1) / N;
     }
+    __device__ __forceinline__ int first_token(int block) const { return block * N - skew; }
+    // Blocks [whole_begin, whole_end) lie in the row and may be read at once.
+    __device__ __forceinline__ int whole_begin() const { return vectors ? (skew ? 1 : 0) : blocks; }
+    __device__ __forceinline__ int whole_end() const { return vectors ? (vocab + skew) / N : blocks; }
     __device__ __forceinline__ void load(const T* x, int block, Vector<T>& out) const
     {
         const int token = block * N - skew;
@@ -142,6 +179,7 @@ __device__ __forceinline__ double warp_sum(double v)
     return v;
 }
 
+// The sum of a block's weights, token by token compared with the rejected ones.
 template <class T, bool DRAFT>
 __device__ __forceinline__ double block_weight(const Weights<T, DRAFT>& w, const Row<T, DRAFT>& row, int block,
                                                const Vector<T>& p, const Vector<T>& q)
@@ -149,37 +187,142 @@ __device__ __forceinline__ double block_weight(const Weights<T, DRAFT>& w, const
     double sum = 0.0;
 #pragma unroll
     for (int k = 0; k < Row<T, DRAFT>::N; ++k)
-        sum += w.at(block * Row<T, DRAFT>::N - row.skew + k, to_double(p.v[k]), DRAFT ? to_double(q.v[k]) : 0.0);
+        sum += w.at(row.first_token(block) + k, to_double(p.v[k]), DRAFT ? to_double(q.v[k]) : 0.0);
     return sum;
+}
+
+// Running sums of the warps' ranges, by each warp for itself: lane l gets those
+// of ranges l, l + 32, ..., by the same additions everywhere.
+template <int RANGES> struct RangeSums
+{
+    static constexpr int EACH = (RANGES + 31) / 32;
+    double own[EACH], until[EACH], total;
+
+    __device__ __forceinline__ explicit RangeSums(const double* sums)
+    {
+        const int lane = threadIdx.x & 31;
+        double before = 0.0;
+#pragma unroll
+        for (int k = 0; k < EACH; ++k)
+        {
+            own[k] = 32 * k + lane < RANGES ? sums[32 * k + lane] : 0.0;
+            double v = own[k];
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1)
+            {
+                const double up = __shfl_up_sync(0xffffffffu, v, d);
+                v = lane >= d ? v + up : v;
+            }
+            until[k] = before + v;
+            before = __shfl_sync(0xffffffffu, until[k], 31);
+        }
+        total = before;
+    }
+};
+
+template <int CLUSTER> __device__ __forceinline__ int cluster_rank()
+{
+    return CLUSTER > 1 ? static_cast<int>(cg::this_cluster().block_rank()) : 0;
 }
 
 // Sums the weights of the whole row; every thread of the cluster returns the
 // total, and sums holds each warp range's sum.
-template <class T, bool DRAFT, int CLUSTER>
-__device__ double whole_row(const Weights<T, DRAFT>& w, const Row<T, DRAFT>& row, int per, double* sums)
+template <class T, bool DRAFT, int CLUSTER, int THREADS>
+__device__ double whole_row(Weights<T, DRAFT> w, const Row<T, DRAFT>& row, int per, double* sums)
 {
+    constexpr int WARPS = THREADS / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int rank = CLUSTER > 1 ? static_cast<int>(cg::this_cluster().block_rank()) : 0;
-    const int mine = rank * WARPS + warp;
+    const int mine = cluster_rank<CLUSTER>() * WARPS + warp;
     const int end = min(row.blocks, (mine + 1) * per);
+    w.keep(row.first_token(mine * per), row.first_token(end));
+    constexpr int UNROLL = DRAFT ? 4 : 8; // 16-byte loads in flight per row and lane
+    constexpr int N = Row<T, DRAFT>::N;
     double sum = 0.0;
-    constexpr int UNROLL = 4;
-    for (int b = mine * per + lane; b < end; b += 32 * UNROLL)
+    // Blocks that are not whole, and all of rows that cannot be read in vectors.
+    const int low = min(end, max(mine * per, row.whole_begin())), high = max(low, min(end, row.whole_end()));
+    for (int b = mine * per + lane; b < end; b += 32)
     {
-        Vector<T> p[UNROLL], q[UNROLL];
+        if (b >= low && b < high)
+        {
+            b += (high - b + 31) / 32 * 32 - 32; // to the first of this lane's blocks from `high` on
+            continue;
+        }
+        Vector<T> p, q;
+        row.load(w.p, b, p);
+        if constexpr (DRAFT)
+            row.load(w.q, b, q);
+        sum += block_weight<T, DRAFT>(w, row, b, p, q);
+    }
+    // Whole blocks, with nothing in the loop but loads, conversions and sums by a tree (a
+    // chain of 64-bit additions would wait for each).
+    double parts[4] = {};
+    bool undefined = false;
+    const auto* from_p = reinterpret_cast<const uint4*>(w.p - row.skew);
+    const auto* from_q = reinterpret_cast<const uint4*>(DRAFT ? w.q - row.skew : w.p);
+    const bool subtract = w.rounds > 0;
+    for (int first = low; first < high; first += 32 * UNROLL)
+    {
+        Words p[UNROLL], q[DRAFT ? UNROLL : 1];
 #pragma unroll
         for (int k = 0; k < UNROLL; ++k)
-            if (b + 32 * k < end)
+        {
+            const int b = first + lane + 32 * k;
+            p[k] = b < high ? Words(from_p[b]) : Words();
+            if constexpr (DRAFT)
+                q[k] = b < high && subtract ? Words(from_q[b]) : Words();
+        }
+        if constexpr (!DRAFT)
+        {
+            // A rejected token of these blocks is cleared where it was loaded.
+            for (unsigned long long rest = w.rejected; rest; rest &= rest - 1)
             {
-                row.load(w.p, b + 32 * k, p[k]);
+                const int token = w.tokens[__ffsll(static_cast<long long>(rest)) - 1] + row.skew;
+                const int away = token / N - first, byte = token % N * static_cast<int>(sizeof(T));
+                if (away >= 0 && away < 32 * UNROLL && (away & 31) == lane)
+                {
+                    const std::uint32_t stays = sizeof(T) == 4 ? 0u : (byte & 2 ? 0x0000ffffu : 0xffff0000u);
+#pragma unroll
+                    for (int k = 0; k < UNROLL; ++k)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            p[k].w[j] &= k == away / 32 && j == byte / 4 ? stays : ~0u;
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < UNROLL; ++k)
+        {
+            double sums[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+            {
+                sums[j] = p[k].template value<T>(j);
                 if constexpr (DRAFT)
-                    row.load(w.q, b + 32 * k, q[k]);
+                {
+                    sums[j] -= q[k].template value<T>(j);
+                    undefined |= sums[j] != sums[j];
+                    sums[j] = sums[j] > 0.0 ? sums[j] : 0.0;
+                }
+            }
+            if (DRAFT && w.rounds > 1)
+            {
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+#pragma unroll 1
+                    for (int i = 1; i < w.rounds; ++i)
+                        sums[j] = Weights<T, DRAFT>::above(sums[j] * w.scale[i] - q[DRAFT ? k : 0].template value<T>(j));
             }
 #pragma unroll
-        for (int k = 0; k < UNROLL; ++k)
-            if (b + 32 * k < end)
-                sum += block_weight<T, DRAFT>(w, row, b + 32 * k, p[k], q[k]);
+            for (int n = N / 2; n; n /= 2)
+#pragma unroll
+                for (int j = 0; j < n; ++j)
+                    sums[j] += sums[j + n];
+            parts[k & 3] += sums[0];
+        }
     }
+    sum += (parts[0] + parts[1]) + (parts[2] + parts[3]);
+    if (undefined)
+        sum = NAN;
     sum = warp_sum(sum);
     if constexpr (CLUSTER > 1)
     {
@@ -194,37 +337,35 @@ __device__ double whole_row(const Weights<T, DRAFT>& w, const Row<T, DRAFT>& row
             sums[mine] = sum;
         __syncthreads();
     }
-    double total = 0.0;
-#pragma unroll 8
-    for (int k = 0; k < CLUSTER * WARPS; ++k)
-        total += sums[k];
-    return total;
+    return RangeSums<CLUSTER * WARPS>(sums).total;
 }
 
 // The first token whose cumulative weight exceeds `threshold`, by the CTA that
 // owns its range; the last token of positive weight if rounding leaves none.
-template <class T, bool DRAFT, int CLUSTER>
-__device__ void pick(const Weights<T, DRAFT>& w, const Row<T, DRAFT>& row, int per, const double* sums,
-                     double threshold, Shared& sh, int* token)
+template <class T, bool DRAFT, int CLUSTER, int THREADS>
+__device__ void pick(Weights<T, DRAFT> w, const Row<T, DRAFT>& row, int per, const double* sums, double threshold,
+                     Shared& sh, int* token)
 {
+    constexpr int WARPS = THREADS / 32;
+    // The last range with weight that starts at or below the threshold.
+    const RangeSums<CLUSTER * WARPS> scan(sums);
     int range = -1;
-    double before = 0.0, running = 0.0;
-#pragma unroll 8
-    for (int k = 0; k < CLUSTER * WARPS; ++k)
+    double before = 0.0;
+#pragma unroll
+    for (int k = 0; k < RangeSums<CLUSTER * WARPS>::EACH; ++k)
     {
-        const double next = running + sums[k];
-        if (sums[k] > 0.0 && !(running > threshold))
-        {
-            range = k;
-            before = running;
-        }
-        running = next;
+        const double start = scan.until[k] - scan.own[k];
+        const unsigned found = __ballot_sync(0xffffffffu, scan.own[k] > 0.0 && !(start > threshold));
+        const int last = 31 - __clz(found);
+        const double there = __shfl_sync(0xffffffffu, start, found ? last : 0);
+        range = found ? 32 * k + last : range;
+        before = found ? there : before;
     }
-    const int rank = CLUSTER > 1 ? static_cast<int>(cg::this_cluster().block_rank()) : 0;
-    if (range / WARPS != rank || range < 0)
+    if (range < 0 || range / WARPS != cluster_rank<CLUSTER>())
         return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int begin = range * per, end = min(row.blocks, begin + per);
+    w.keep(row.first_token(begin), row.first_token(end));
     const int each = (per + THREADS - 1) / THREADS;
     const int b0 = min(end, begin + static_cast<int>(threadIdx.x) * each), b1 = min(end, b0 + each);
     double sum = 0.0;
@@ -270,7 +411,7 @@ __device__ void pick(const Weights<T, DRAFT>& w, const Row<T, DRAFT>& row, int p
 #pragma unroll
         for (int k = 0; k < Row<T, DRAFT>::N; ++k)
         {
-            const int candidate = b * Row<T, DRAFT>::N - row.skew + k;
+            const int candidate = row.first_token(b) + k;
             const double weight = w.at(candidate, to_double(p.v[k]), DRAFT ? to_double(q.v[k]) : 0.0);
             cumulative += weight;
             if (!crossed && weight > 0.0)
@@ -283,69 +424,78 @@ __device__ void pick(const Weights<T, DRAFT>& w, const Row<T, DRAFT>& row, int p
     *token = found;
 }
 
-template <class T, bool DRAFT, int CLUSTER>
-__global__ void __launch_bounds__(THREADS, 2) draft_verify_kernel(const VerifyArgs a)
+template <class T, bool DRAFT, int CLUSTER, int THREADS>
+__global__ void __launch_bounds__(THREADS, (DRAFT ? 512 : 1024) / THREADS) draft_verify_kernel(const VerifyArgs a)
 {
+    if constexpr (CLUSTER > 1)
+        cg::this_cluster().barrier_arrive();
     pdl_prologue();
     __shared__ Shared sh;
+    constexpr int RANGES = CLUSTER * THREADS / 32;
     const int sequence = blockIdx.x / CLUSTER;
-    const bool leader = blockIdx.x % CLUSTER == 0;
-    const int t = threadIdx.x;
+    const int t = threadIdx.x, lane = t & 31;
     const long long list = static_cast<long long>(sequence) * a.max_nodes;
     int nodes = a.nodes ? a.nodes[sequence] : a.max_nodes;
     nodes = nodes < 0 ? 0 : (nodes < a.max_nodes ? nodes : a.max_nodes);
     const T* target = static_cast<const T*>(a.target) + sequence * a.target_batch;
     const T* draft = DRAFT ? static_cast<const T*>(a.draft) + sequence * a.draft_batch : nullptr;
-    if (t < nodes)
+    const float draw = a.draws[sequence];
+    if (t < DRAFT_MAX_NODES)
     {
-        const int parent = a.parents[list + t], token = a.tokens[list + t];
+        const bool there = t < nodes;
+        const int parent = there ? a.parents[list + t] : -1, token = there ? a.tokens[list + t] : -1;
         const bool real = t > 0 && parent >= 0 && parent < t;
         const bool known = static_cast<unsigned>(token) < static_cast<unsigned>(a.vocab);
         sh.parents[t] = real ? parent : -1;
         sh.tokens[t] = token;
-        sh.coins[t] = a.coins[list + t];
+        sh.coins[t] = there ? a.coins[list + t] : 0.0f;
         // A token outside the vocabulary has probability 0 and is never accepted.
         sh.p[t] = real && known ? to_double(target[parent * a.target_node + token]) : 0.0;
         if constexpr (DRAFT)
             sh.q[t] = real && known ? to_double(draft[parent * a.draft_node + token]) : 0.0;
     }
     if constexpr (CLUSTER > 1)
-        cg::this_cluster().sync(); // every CTA runs before its shared memory is written to
-    else
-        __syncthreads();
+        cg::this_cluster().barrier_wait(); // every CTA runs before its shared memory is written to
+    __syncthreads();
     int accepted = 0, passes = 0;
     bool failed = false;
     if (nodes > 0)
     {
+        const int parents[2] = {sh.parents[lane], sh.parents[lane + 32]};
+        const auto children_of = [&](int node)
+        {
+            const unsigned low = __ballot_sync(0xffffffffu, parents[0] == node), high = __ballot_sync(0xffffffffu, parents[1] == node);
+            return static_cast<unsigned long long>(high) << 32 | low;
+        };
         int node = 0, rounds = 0;
         bool summed = false; // the last pass summed the current weights
         double total = 0.0, left = 1.0;
+        unsigned long long rejected = 0;
         accepted = 1;
         if (t == 0)
             sh.path[0] = 0;
-        const auto weights = [&](int at, int n)
+        const auto weights = [&](int n, unsigned long long without)
         {
-            return Weights<T, DRAFT>{target + at * a.target_node, DRAFT ? draft + at * a.draft_node : nullptr, n, sh.scale,
-                                     sh.rejected};
+            return Weights<T, DRAFT>{target + node * a.target_node, DRAFT ? draft + node * a.draft_node : nullptr, n,
+                                     sh.scale, without, sh.tokens};
         };
-        const int ranges = CLUSTER * WARPS;
-        for (int n = 1; n < nodes && !failed; ++n)
+        unsigned long long children = children_of(0);
+        while (children && !failed)
         {
-            if (sh.parents[n] != node)
-                continue;
+            const int n = __ffsll(static_cast<long long>(children)) - 1;
+            children &= children - 1;
             double p = sh.p[n];
             bool pass;
             if constexpr (DRAFT)
             {
-                const Weights<T, DRAFT> w = weights(node, rounds);
-                p = w.excess(p, sh.q[n]);
+                p = weights(rounds, 0).excess(p, sh.q[n]);
                 p = rounds ? p * sh.scale[rounds] : p;
                 pass = sh.coins[n] * sh.q[n] < p;
             }
             else
             {
-                for (int i = 0; i < rounds; ++i)
-                    p = sh.rejected[i] == sh.tokens[n] ? 0.0 : p;
+                for (unsigned long long rest = rejected; rest; rest &= rest - 1)
+                    p = sh.tokens[__ffsll(static_cast<long long>(rest)) - 1] == sh.tokens[n] ? 0.0 : p;
                 pass = sh.coins[n] * left < p;
             }
             if (pass)
@@ -357,20 +507,22 @@ __global__ void __launch_bounds__(THREADS, 2) draft_verify_kernel(const VerifyAr
                 rounds = 0;
                 summed = false;
                 left = 1.0;
-                __syncthreads(); // the rejected tokens have been read
+                rejected = 0;
+                children = children_of(n);
                 continue;
             }
             if constexpr (DRAFT)
             {
-                const Weights<T, DRAFT> w = weights(node, rounds + 1);
+                const Weights<T, DRAFT> w = weights(rounds + 1, 0);
                 const Row<T, DRAFT> row(w.p, w.q, a.vocab);
-                const double z = whole_row<T, DRAFT, CLUSTER>(w, row, (row.blocks + ranges - 1) / ranges, sh.sums[passes & 1]);
-                if (z > 0.0 && z < INFINITY)
+                const double z = whole_row<T, DRAFT, CLUSTER, THREADS>(w, row, (row.blocks + RANGES - 1) / RANGES,
+                                                                      sh.sums[passes & 1]);
+                ++passes;
+                summed = z > 0.0 && z < INFINITY;
+                if (summed)
                 {
                     total = z;
-                    summed = true;
                     ++rounds;
-                    ++passes;
                     if (t == 0)
                         sh.scale[rounds] = 1.0 / z;
                     __syncthreads();
@@ -378,42 +530,37 @@ __global__ void __launch_bounds__(THREADS, 2) draft_verify_kernel(const VerifyAr
                 else // no excess: the weights stay; a NaN or an infinity ends the walk
                 {
                     failed = !(z == 0.0);
-                    summed = false;
-                    ++passes;
                 }
             }
             else
             {
-                if (t == 0)
-                    sh.rejected[rounds] = sh.tokens[n];
+                rejected |= 1ull << n;
                 left -= p;
-                ++rounds;
-                __syncthreads();
             }
         }
-        const auto finish = [&](int n)
+        const auto finish = [&](unsigned long long without)
         {
-            const Weights<T, DRAFT> w = weights(node, n);
+            const Weights<T, DRAFT> w = weights(rounds, without);
             const Row<T, DRAFT> row(w.p, w.q, a.vocab);
-            const int per = (row.blocks + ranges - 1) / ranges;
+            const int per = (row.blocks + RANGES - 1) / RANGES;
             if (!summed)
-                total = whole_row<T, DRAFT, CLUSTER>(w, row, per, sh.sums[passes++ & 1]);
+                total = whole_row<T, DRAFT, CLUSTER, THREADS>(w, row, per, sh.sums[passes++ & 1]);
             if (!(total > 0.0 && total < INFINITY))
                 return false;
-            pick<T, DRAFT, CLUSTER>(w, row, per, sh.sums[(passes - 1) & 1],
-                                    static_cast<double>(a.draws[sequence]) * total, sh, a.token + sequence);
+            pick<T, DRAFT, CLUSTER, THREADS>(w, row, per, sh.sums[(passes - 1) & 1], static_cast<double>(draw) * total, sh,
+                                             a.token + sequence);
             return true;
         };
         if (!failed)
         {
-            bool done = finish(rounds);
+            bool done = finish(rejected);
             if constexpr (!DRAFT)
-                if (!done && rounds && total == 0.0) // nothing left beside the rejected tokens
+                if (!done && rejected && total == 0.0) // nothing left beside the rejected tokens
                     done = finish(0);
             failed = !done;
         }
     }
-    if (leader)
+    if (blockIdx.x % CLUSTER == 0)
     {
         __syncthreads();
         for (int n = t; n < a.max_nodes; n += THREADS)
@@ -429,7 +576,7 @@ __global__ void __launch_bounds__(THREADS, 2) draft_verify_kernel(const VerifyAr
     }
 }
 
-template <class T, bool DRAFT, int CLUSTER> cudaError_t launch(const VerifyArgs& a, int batch, cudaStream_t stream)
+template <class T, bool DRAFT, int CLUSTER, int THREADS> cudaError_t launch(const VerifyArgs& a, int batch, cudaStream_t stream)
 {
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(batch * CLUSTER);
@@ -444,16 +591,38 @@ template <class T, bool DRAFT, int CLUSTER> cudaError_t launch(const VerifyArgs&
     attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
     config.numAttrs = 2;
-    const cudaError_t status = cudaLaunchKernelEx(&config, draft_verify_kernel<T, DRAFT, CLUSTER>, a);
+    const cudaError_t status = cudaLaunchKernelEx(&config, draft_verify_kernel<T, DRAFT, CLUSTER, THREADS>, a);
     note_launch();
     return status;
 }
 
+// CTAs for one sequence.  Small vocabularies are latency alone: one CTA of 128
+// threads.  Others: CTAs of 512 threads (256 with a draft, whose pass needs
+// twice the registers), as many as leave each thread 16 tokens or more.  All of
+// them on the GPU at once, two per SM, serve best (160 rows of 131,072 tokens:
+// 24.6 us, with three waves 71); the smaller ones of a draft up to five per SM
+// (41 us in clusters of 4, 86 without a cluster).
+template <class T, bool DRAFT> cudaError_t launch_cluster(const VerifyArgs& a, int batch, cudaStream_t stream)
+{
+    constexpr int THREADS = DRAFT ? 256 : 512;
+    int device = 0, sms = 148;
+    if (cudaGetDevice(&device) == cudaSuccess)
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    const int most = std::min((DRAFT ? 5 : 2) * sms / batch, a.vocab / (16 * THREADS));
+    if (a.vocab <= 8192)
+        return launch<T, DRAFT, 1, 128>(a, batch, stream);
+    if (most >= 8)
+        return launch<T, DRAFT, 8, THREADS>(a, batch, stream);
+    if (most >= 4)
+        return launch<T, DRAFT, 4, THREADS>(a, batch, stream);
+    if (most >= 2)
+        return launch<T, DRAFT, 2, THREADS>(a, batch, stream);
+    return launch<T, DRAFT, 1, THREADS>(a, batch, stream);
+}
+
 template <class T> cudaError_t launch_type(const VerifyArgs& a, int batch, cudaStream_t stream)
 {
-    if (a.vocab >= 16384)
-        return a.draft ? launch<T, true, WIDE>(a, batch, stream) : launch<T, false, WIDE>(a, batch, stream);
-    return a.draft ? launch<T, true, 1>(a, batch, stream) : launch<T, false, 1>(a, batch, stream);
+    return a.draft ? launch_cluster<T, true>(a, batch, stream) : launch_cluster<T, false>(a, batch, stream);
 }
 } // namespace
 
