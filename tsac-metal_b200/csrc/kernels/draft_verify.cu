@@ -32,7 +32,6 @@
 #include "kernels/launch_count.hpp"
 #include "kernels/pdl.cuh"
 
-#include <algorithm>
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -598,26 +597,40 @@ template <class T, bool DRAFT, int CLUSTER, int THREADS> cudaError_t launch(cons
 
 // CTAs for one sequence.  Small vocabularies are latency alone: one CTA of 128
 // threads.  Others: CTAs of 512 threads (256 with a draft, whose pass needs
-// twice the registers), as many as leave each thread 16 tokens or more.  All of
-// them on the GPU at once, two per SM, serve best (160 rows of 131,072 tokens:
-// 24.6 us, with three waves 71); the smaller ones of a draft up to five per SM
-// (41 us in clusters of 4, 86 without a cluster).
+// twice the registers), two per SM; of 1, 2, 4 or 8 the number that costs
+// least, where a wave of CTAs costs its start (about 6 us, in which a CTA reads
+// 240 KB, or 72 KB with a draft) and its part of the rows.  Measured in us:
+// 160 x 131,072 fp32, 1 CTA 24.6, 4 in three waves 71; 48 x 50,001 bf16 with a
+// draft, 4 CTAs 10.3, 8 in two waves 14.4.
 template <class T, bool DRAFT> cudaError_t launch_cluster(const VerifyArgs& a, int batch, cudaStream_t stream)
 {
     constexpr int THREADS = DRAFT ? 256 : 512;
+    constexpr long long start_bytes = DRAFT ? 72 << 10 : 240 << 10;
+    if (a.vocab <= 8192)
+        return launch<T, DRAFT, 1, 128>(a, batch, stream);
     int device = 0, sms = 148;
     if (cudaGetDevice(&device) == cudaSuccess)
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    const int most = std::min((DRAFT ? 5 : 2) * sms / batch, a.vocab / (16 * THREADS));
-    if (a.vocab <= 8192)
-        return launch<T, DRAFT, 1, 128>(a, batch, stream);
-    if (most >= 8)
+    const long long row_bytes = static_cast<long long>(a.vocab) * sizeof(T) * (DRAFT ? 2 : 1);
+    const auto cost = [&](int cluster)
+    {
+        const long long waves = (static_cast<long long>(batch) * cluster + 2 * sms - 1) / (2 * sms);
+        return waves * (start_bytes + row_bytes / cluster);
+    };
+    int best = 1;
+    for (int cluster = 2; cluster <= 8; cluster *= 2)
+        best = cost(cluster) < cost(best) ? cluster : best;
+    switch (best)
+    {
+    case 8:
         return launch<T, DRAFT, 8, THREADS>(a, batch, stream);
-    if (most >= 4)
+    case 4:
         return launch<T, DRAFT, 4, THREADS>(a, batch, stream);
-    if (most >= 2)
+    case 2:
         return launch<T, DRAFT, 2, THREADS>(a, batch, stream);
-    return launch<T, DRAFT, 1, THREADS>(a, batch, stream);
+    default:
+        return launch<T, DRAFT, 1, THREADS>(a, batch, stream);
+    }
 }
 
 template <class T> cudaError_t launch_type(const VerifyArgs& a, int batch, cudaStream_t stream)
