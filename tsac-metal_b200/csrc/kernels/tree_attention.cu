@@ -11,10 +11,12 @@
 // Bound: the keys and values cross HBM once per key head, M / 2 multiply-adds
 // per byte for M query rows; up to 32 rows that is below what mma.sync
 // sustains, so the layout is chosen for bytes in flight: each warp streams its
-// own 16 keys of a 64-key tile through a private three-stage ring (16-byte
-// asynchronous copies, any page size), so no barrier couples the warps before
-// the end of an item, and two CTAs of four warps keep up to 128 KiB in flight
-// per SM.
+// own keys of a tile (16 of 64 at 128 columns, 32 of 128 at 64) through a
+// private three-stage ring (16-byte asynchronous copies, any page size), so no
+// barrier couples the warps before the end of an item, and two CTAs of four
+// warps keep up to 128 KiB in flight per SM.  (16 keys of 64 columns a stage,
+// half of that, took 133 us for 96 single tokens over up to 8,191 positions;
+// 32 take 112.)
 #include "kernels/half_types.cuh"
 #include "kernels/launch_count.hpp"
 #include "kernels/pdl.cuh"
@@ -27,7 +29,7 @@ namespace tsacb::dev
 {
 namespace
 {
-constexpr int WARPS = 4, THREADS = WARPS * 32, STAGES = 3, WARP_KEYS = 16, KEYS = WARPS * WARP_KEYS;
+constexpr int WARPS = 4, THREADS = WARPS * 32, STAGES = 3;
 
 __device__ __forceinline__ void load_matrices(std::uint32_t address, std::uint32_t (&r)[4])
 {
@@ -49,6 +51,7 @@ template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("c
 template <int D, int MT> struct Layout
 {
     static constexpr int ROWS = 16 * MT;
+    static constexpr int WARP_KEYS = D == 128 ? 16 : 32, KEYS = WARPS * WARP_KEYS;
     static constexpr int row_bytes = 2 * D, chunks = D / 8;
     static constexpr int stage_bytes = 2 * WARP_KEYS * row_bytes; // keys, then values
     static constexpr int ring_bytes = WARPS * STAGES * stage_bytes;
@@ -62,7 +65,8 @@ __global__ void __launch_bounds__(THREADS, 2)
 {
     pdl_prologue();
     using L = Layout<D, MT>;
-    using Work = TreeWork<KEYS, L::ROWS, 1>;
+    using Work = TreeWork<L::KEYS, L::ROWS, 1>;
+    constexpr int WARP_KEYS = L::WARP_KEYS, NT = WARP_KEYS / 8; // keys of a warp, and their groups of 8
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ unsigned long long masks[DRAFT_MAX_NODES];
     __shared__ long long warp_sums[WARPS];
@@ -85,8 +89,9 @@ __global__ void __launch_bounds__(THREADS, 2)
         const auto& e = g.e;
         const int head = g.head, first_row = g.first_row, rows = g.rows;
         const int tile_begin = g.tile_begin, tile_end = g.tile_end;
-        // Lane % 16 follows one of the warp's 16 keys.
-        const auto key_row = [&](int tile) { return Work::key_row(a, g, tile, warp * WARP_KEYS + (lane & 15)); };
+        // Each lane follows one of the warp's keys.
+        const auto key_row = [&](int tile)
+        { return Work::key_row(a, g, tile, warp * WARP_KEYS + (lane & (WARP_KEYS - 1))); };
         // Rows of L::chunks 16-byte chunks, chunk c of row r at place c ^ (r & 7): conflict-free for ldmatrix.
         const auto fetch = [&](int stage, long long row_offset)
         {
@@ -160,24 +165,26 @@ __global__ void __launch_bounds__(THREADS, 2)
             const std::uint32_t keys = ring + stage * L::stage_bytes, values = keys + WARP_KEYS * L::row_bytes;
             stage = stage + 1 == STAGES ? 0 : stage + 1;
 
-            float s[MT][2][4] = {};
+            float s[MT][NT][4] = {};
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
-            {
-                // Matrices: keys 0-7 and 8-15 by the two halves of the 16 columns.
-                const int row = (lane & 7) + ((lane >> 4) << 3), chunk = 2 * k + ((lane >> 3) & 1);
-                std::uint32_t b[4];
-                load_matrices(keys + row * L::row_bytes + ((chunk ^ (row & 7)) << 4), b);
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
+                for (int half = 0; half < NT / 2; ++half) // 16 keys each
                 {
-                    Half2<T>::mma(s[m][0], q[m][k], b[0], b[1]);
-                    Half2<T>::mma(s[m][1], q[m][k], b[2], b[3]);
+                    // Matrices: keys 0-7 and 8-15 by the two halves of the 16 columns.
+                    const int row = 16 * half + (lane & 7) + ((lane >> 4) << 3), chunk = 2 * k + ((lane >> 3) & 1);
+                    std::uint32_t b[4];
+                    load_matrices(keys + row * L::row_bytes + ((chunk ^ (row & 7)) << 4), b);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+                    {
+                        Half2<T>::mma(s[m][2 * half], q[m][k], b[0], b[1]);
+                        Half2<T>::mma(s[m][2 * half + 1], q[m][k], b[2], b[3]);
+                    }
                 }
-            }
             const bool last = Work::is_last(g, tile);
             const bool masked = Work::is_masked(g, tile);
-            // The warp's keys are bits `first_bit` to + 15 of the 32 that `visible` gives.
+            // The warp's keys are bits `first_bit` and on of the 32 that `visible` gives.
             const int first_bit = (warp * WARP_KEYS) & 31;
             const int first_node = Work::base(g, tile) + warp * WARP_KEYS - e.length; // of the warp's first key, if drafted
             unsigned tainted = 0; // drafted rows with a value that is not finite
@@ -199,8 +206,8 @@ __global__ void __launch_bounds__(THREADS, 2)
                     tainted |= __any_sync(0xffffffffu, odd) ? 1u << row : 0u;
                 }
             }
-            std::uint32_t p[MT][4];
-            float exact_p[MT][2][4];
+            std::uint32_t p[MT][NT / 2][4];
+            float exact_p[MT][2][2 * NT];
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -211,11 +218,11 @@ __global__ void __launch_bounds__(THREADS, 2)
                     {
                         const int row = first_row + 16 * m + 8 * r + (lane >> 2);
                         sees = Work::visible(g, tile, warp * WARP_KEYS / 32, last && row < rows ? masks[row / a.group] : 0ull) >>
-                               (first_bit + 2 * (lane & 3)); // this lane's keys: bits 0, 1, 8, 9
+                               (first_bit + 2 * (lane & 3)); // this lane's keys: bits 0 and 1 of each 8
                     }
-                    float z[4], best = top[m][r];
+                    float z[2 * NT], best = top[m][r];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
+                    for (int k = 0; k < 2 * NT; ++k)
                     {
                         z[k] = s[m][k >> 1][2 * r + (k & 1)] * a.scale_log2;
                         if (!(sees >> ((k & 1) + 8 * (k >> 1)) & 1u))
@@ -229,15 +236,19 @@ __global__ void __launch_bounds__(THREADS, 2)
                     top[m][r] = best;
                     float partial = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
+                    for (int k = 0; k < 2 * NT; ++k)
                     {
                         z[k] = power_of_two(z[k] - shift);
                         partial += z[k];
                         exact_p[m][r][k] = z[k];
                     }
                     sum[m][r] = fmaf(sum[m][r], scale, partial);
-                    p[m][r] = Half2<T>::pack(z[0], z[1]);
-                    p[m][r + 2] = Half2<T>::pack(z[2], z[3]);
+#pragma unroll
+                    for (int half = 0; half < NT / 2; ++half)
+                    {
+                        p[m][half][r] = Half2<T>::pack(z[4 * half], z[4 * half + 1]);
+                        p[m][half][r + 2] = Half2<T>::pack(z[4 * half + 2], z[4 * half + 3]);
+                    }
                     if (__any_sync(0xffffffffu, scale != 1.0f))
                     {
 #pragma unroll
@@ -267,7 +278,7 @@ __global__ void __launch_bounds__(THREADS, 2)
                             const bool seen = row < rows && (masks[row / a.group] >> (first_node + key) & 1ull);
                             float weight = 0.0f;
 #pragma unroll
-                            for (int kk = 0; kk < 4; ++kk)
+                            for (int kk = 0; kk < 2 * NT; ++kk)
                             {
                                 const float w = __shfl_sync(0xffffffffu, exact_p[m][r][kk], from);
                                 weight = kk == k ? w : weight;
@@ -292,19 +303,21 @@ __global__ void __launch_bounds__(THREADS, 2)
                 __syncwarp();
             }
 #pragma unroll
-            for (int n = 0; n < D / 16; ++n)
-            {
-                // Matrices: keys 0-7 and 8-15 by the two halves of 16 output columns.
-                const int row = (lane & 7) + (((lane >> 3) & 1) << 3), chunk = 2 * n + (lane >> 4);
-                std::uint32_t b[4];
-                load_matrices_transposed(values + row * L::row_bytes + ((chunk ^ (row & 7)) << 4), b);
+            for (int half = 0; half < NT / 2; ++half)
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
+                for (int n = 0; n < D / 16; ++n)
                 {
-                    Half2<T>::mma(o[m][2 * n], p[m], b[0], b[1]);
-                    Half2<T>::mma(o[m][2 * n + 1], p[m], b[2], b[3]);
+                    // Matrices: keys 0-7 and 8-15 by the two halves of 16 output columns.
+                    const int row = 16 * half + (lane & 7) + (((lane >> 3) & 1) << 3), chunk = 2 * n + (lane >> 4);
+                    std::uint32_t b[4];
+                    load_matrices_transposed(values + row * L::row_bytes + ((chunk ^ (row & 7)) << 4), b);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+                    {
+                        Half2<T>::mma(o[m][2 * n], p[m][half], b[0], b[1]);
+                        Half2<T>::mma(o[m][2 * n + 1], p[m][half], b[2], b[3]);
+                    }
                 }
-            }
             __syncwarp(); // the stage may be refilled
         }
         copies_wait<0>();
