@@ -429,3 +429,22 @@ def test_captured_step_replays():
         for b in (0, 1):
             pair.book.release(b, pair.book.lengths[b])
         pair.check()
+
+
+def test_captured_reservation_outlives_larger_ones():
+    """A graph's temporary memory stays its own when later calls need more."""
+    cache = tsac_cuda.PagedCache.empty(1, 600, 4, 1, 8, 300, 4)
+    first = ints([0])
+    positions = ints([3])
+    cache.reserve(positions, sequences=first, slots=1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.release(sequences=first)
+        cache.reserve(positions, sequences=first, slots=1)
+    cache.reserve(torch.ones(300, dtype=torch.int32, device="cuda"))
+    guards = [torch.full((n,), 17, dtype=torch.uint8, device="cuda") for n in (16, 64, 512, 4096, 8192, 20000) for _ in range(8)]
+    want = cache.refs.clone(), cache.tables.clone()
+    for _ in range(3):
+        graph.replay()
+    assert all((guard == 17).all() for guard in guards)
+    assert torch.equal(cache.refs, want[0]) and torch.equal(cache.tables, want[1])

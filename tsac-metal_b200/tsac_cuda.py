@@ -283,6 +283,7 @@ class PagedCache:
         s.type = 0 if pool.dtype == torch.bfloat16 else 1
         self._struct, self._lib, self._on = s, _drafting(), _Device.of(self.index)
         self._cache = ctypes.addressof(s)
+        self._scratches = []
 
     @classmethod
     def empty(cls, layers, pages, page_size, kv_heads, head_dim, sequences, max_pages, dtype=None, device="cuda"):
@@ -303,18 +304,26 @@ class PagedCache:
             raise TsacError("error_word must hold a 32-bit word")
         return _whole(error_word, "error_word", error_word.dtype, self.index)
 
-    def _scratch(self, nbytes):
+    def _temporary(self, nbytes):
         return self._torch.empty(max(nbytes, 16), dtype=self._torch.uint8, device=self.device)
+
+    def _kept(self, nbytes):
+        """Temporary memory of the calls that change the cache, which must not overlap: kept from one to the next.
+        A larger one is added, not exchanged: a captured graph goes on using the one that it was captured with."""
+        if not self._scratches or self._scratches[-1].numel() < nbytes:
+            last = self._scratches[-1].numel() if self._scratches else 0
+            self._scratches.append(self._temporary(max(nbytes, 2 * last)))
+        return self._scratches[-1]
 
     def reserve(self, positions, sequences=None, slots=None, error_word=None):
         """Makes positions[i] further positions of each sequence writable (all or nothing)."""
         count = positions.shape[0]
         slots = slots or self.max_pages
         nbytes = self._lib.tsac_cuda_cache_reserve_scratch_bytes(count, slots)
-        scratch = self._scratch(nbytes)
+        scratch = self._kept(nbytes)
         self._on.call(self._lib.tsac_cuda_cache_reserve, self._cache, self._list(sequences, count),
                       _whole(positions, "positions", self._int, self.index, (count,)), count, slots,
-                      scratch.data_ptr(), scratch.numel(), self._word(error_word), self._on.stream())
+                      scratch.data_ptr(), nbytes, self._word(error_word), self._on.stream())
 
     def fork(self, parents, children, error_word=None):
         """children[i], empty so far, shares the committed pages of parents[i]."""
@@ -333,14 +342,15 @@ class PagedCache:
 
     def append(self, layer, keys, values, nodes=None, sequences=None, starts=None, error_word=None):
         """Stores [entry][node][kv_heads][head_dim] rows of one layer behind each sequence's length (or at starts)."""
-        count, most = keys.shape[:2]
-        shape = (count, most, self.kv_heads, self.head_dim)
-        k, key_strides = _rows(keys, "keys", self.dtype, self.index, shape)
-        v, value_strides = _rows(values, "values", self.dtype, self.index, shape)
+        count, most, _, _ = keys.shape
+        shape, index, ints = (count, most, self.kv_heads, self.head_dim), self.index, self._int
+        k, key_strides = _rows(keys, "keys", self.dtype, index, shape)
+        v, value_strides = _rows(values, "values", self.dtype, index, shape)
         self._on.call(self._lib.tsac_cuda_cache_append, self._cache, layer, k, key_strides, v, value_strides,
-                      self._list(sequences, count), _whole(nodes, "nodes", self._int, self.index, (count,)),
-                      _whole(starts, "starts", self._int, self.index, (count,)), count, most,
-                      self._word(error_word), self._on.stream())
+                      sequences if sequences is None else _whole(sequences, "sequences", ints, index, (count,)),
+                      nodes if nodes is None else _whole(nodes, "nodes", ints, index, (count,)),
+                      starts if starts is None else _whole(starts, "starts", ints, index, (count,)), count, most,
+                      error_word if error_word is None else self._word(error_word), self._on.stream())
 
     def keep(self, path, accepted, starts=None, lengths_out=None, sequences=None, error_word=None):
         """Keeps rows start + path[i][:accepted[i]], in every layer, as the next positions."""
@@ -356,7 +366,7 @@ class PagedCache:
     def compact(self, tables_out=None, refs_out=None, live=None, error_word=None):
         """Moves the pages in use to the lower end of the pool; returns their number (device int32 [1])."""
         live = self._torch.empty(1, dtype=self._int, device=self.device) if live is None else live
-        scratch = self._scratch(self._lib.tsac_cuda_cache_compact_scratch_bytes(self.pages))
+        scratch = self._kept(self._lib.tsac_cuda_cache_compact_scratch_bytes(self.pages))
         self._on.call(self._lib.tsac_cuda_cache_compact, self._cache,
                       _whole(self.tables if tables_out is None else tables_out, "tables_out", self._int, self.index,
                              self.tables.shape),
@@ -376,7 +386,7 @@ class PagedCache:
         out = torch.empty(shape, dtype=self.dtype, device=self.device) if out is None else out
         q, query_strides = _rows(query, "query", self.dtype, self.index, shape)
         o, out_strides = _rows(out, "out", self.dtype, self.index, shape)
-        scratch = self._scratch(self._lib.tsac_cuda_tree_attention_scratch_bytes(self._cache, heads, most))
+        scratch = self._temporary(self._lib.tsac_cuda_tree_attention_scratch_bytes(self._cache, heads, most))
         self._on.call(self._lib.tsac_cuda_tree_attention, self._cache, layer, self._list(sequences, count),
                       _whole(parents, "parents", self._int, self.index, (count, most)),
                       _whole(nodes, "nodes", self._int, self.index, (count,)), q, query_strides, o, out_strides,
@@ -407,19 +417,19 @@ def draft_verify(target, tokens, parents, coins, draws, draft=None, nodes=None, 
             raise TsacError(f"{name} must be bf16, fp16 or fp32 [batch][nodes][vocab], the vocabulary contiguous")
     ints, floats, rows, ones = torch.int32, torch.float32, (batch, most), (batch,)
     if out is None:
-        device = target.device
-        out = (torch.empty(batch, dtype=ints, device=device), torch.empty(rows, dtype=ints, device=device),
-               torch.empty(batch, dtype=ints, device=device))
-    accepted, path, token = out
+        accepted, path, token = draws.new_empty(batch, dtype=ints), parents.new_empty(rows), draws.new_empty(batch, dtype=ints)
+        places = accepted.data_ptr(), path.data_ptr(), token.data_ptr()
+    else:
+        accepted, path, token = out
+        places = (_whole(accepted, "accepted", ints, index, ones), _whole(path, "path", ints, index, rows),
+                  _whole(token, "token", ints, index, ones))
     word = None if error_word is None else _whole(error_word, "error_word", error_word.dtype, index)
     on = _Device.of(index)
     on.call(lib.tsac_cuda_draft_verify, target.data_ptr(), _strides(target.stride()[:2]),
             None if draft is None else draft.data_ptr(), None if draft is None else _strides(draft.stride()[:2]), types[kind],
             _whole(tokens, "tokens", ints, index, rows), _whole(parents, "parents", ints, index, rows),
             _whole(coins, "coins", floats, index, rows), _whole(draws, "draws", floats, index, ones),
-            _whole(nodes, "nodes", ints, index, ones), batch, most, vocab,
-            _whole(accepted, "accepted", ints, index, ones), _whole(path, "path", ints, index, rows),
-            _whole(token, "token", ints, index, ones), word, on.stream())
+            _whole(nodes, "nodes", ints, index, ones), batch, most, vocab, *places, word, on.stream())
     return accepted, path, token
 
 
