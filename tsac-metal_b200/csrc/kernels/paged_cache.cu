@@ -19,7 +19,8 @@ namespace
 {
 constexpr int PLAN_THREADS = 1024;
 constexpr int COPY_THREADS = 256;
-constexpr int COPY_CHUNKS = 4 * COPY_THREADS; // 16-byte chunks of one copy unit: four loads in flight per thread
+constexpr int COPY_AHEAD = 8;                          // loads in flight per thread
+constexpr int COPY_CHUNKS = COPY_AHEAD * COPY_THREADS; // 16-byte chunks of one copy unit
 
 __device__ __forceinline__ void raise(unsigned* error_word, unsigned bit)
 {
@@ -267,32 +268,34 @@ __global__ void __launch_bounds__(PLAN_THREADS)
         *s.copies_count = copies;
 }
 
-// Copies whole pages of every plane, HBM-bound: one unit is 16 KiB of one
-// page of one plane, four 16-byte loads in flight per thread.  Sources and
+// Copies whole pages of every plane, HBM-bound: one unit is 32 KiB of one
+// page of one plane, eight 16-byte loads in flight per thread.  Sources and
 // destinations are distinct pages, so units are independent.
 __device__ __forceinline__ void copy_pages(const CacheView& c, const int2* pairs, long long count)
 {
     const int page_chunks = static_cast<int>(c.page_bytes() >> 4);
     const int parts = (page_chunks + COPY_CHUNKS - 1) / COPY_CHUNKS;
     const long long units = count * c.planes * parts;
+    const bool small = units <= 0x7fffffff; // 32-bit division serves
     for (long long u = blockIdx.x; u < units; u += gridDim.x)
     {
-        const int part = static_cast<int>(u % parts);
-        const long long rest = u / parts;
-        const int2 pair = pairs[rest / c.planes];
-        unsigned char* plane = c.pool + (rest % c.planes) * c.plane_bytes;
+        const long long rest = small ? static_cast<unsigned>(u) / static_cast<unsigned>(parts) : u / parts;
+        const int part = static_cast<int>(u - rest * parts);
+        const long long index = small ? static_cast<unsigned>(rest) / static_cast<unsigned>(c.planes) : rest / c.planes;
+        const int2 pair = pairs[index];
+        unsigned char* plane = c.pool + (rest - index * c.planes) * c.plane_bytes;
         const auto* from = reinterpret_cast<const uint4*>(plane + pair.x * c.page_bytes());
         auto* to = reinterpret_cast<uint4*>(plane + pair.y * c.page_bytes());
-        uint4 v[4];
+        uint4 v[COPY_AHEAD];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < COPY_AHEAD; ++k)
         {
             const int at = part * COPY_CHUNKS + k * COPY_THREADS + threadIdx.x;
             if (at < page_chunks)
                 v[k] = __ldcs(from + at);
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < COPY_AHEAD; ++k)
         {
             const int at = part * COPY_CHUNKS + k * COPY_THREADS + threadIdx.x;
             if (at < page_chunks)
