@@ -28,14 +28,17 @@
 //                   zeros, as does everything where TMA does not serve: pages of
 //                   fewer than 8 rows (a swizzle atom), or 2^31 rows in a plane.  Copies of every tile by the two warps
 //                   bound the kernel by their address arithmetic (290 against
-//                   BATCH_TREES us for 64 x 16 nodes over up to 4,096 positions).
+//                   209 us for 64 x 16 nodes over up to 4,096 positions).
 //   warp 11         the query rows of the next segment, as soon as the last
 //                   scores of this one are made, and its tree's masks.
-// The running maximum moves only when a row's tile exceeds it by more than 8
-// (in powers of two): p then stays below 256, which bf16, fp16 and the 32-bit
-// sums hold as well as 1, and the output in TMEM is rescaled rarely.  So a tile
-// is read once: p is computed with the maximum so far while the tile's own is
-// found, and computed again only when that has moved.
+// The running maximum is a whole number and moves only when a row's scores
+// exceed it by more than 8 (in powers of two): p then stays below 256, which
+// bf16, fp16 and the 32-bit sums hold as well as 1, scores are read once, and
+// what has been computed with the old maximum, p of the same tile included, is
+// rescaled rarely and by powers of two.  The loop over a tile's scores is kept
+// small: unrolled over the whole tile it delayed the MMA warp (64 x 16 nodes 172
+// against 162 us), and exponentials of some pairs by a polynomial on the FMA
+// pipes gained nothing over the special function units' 16 per clock.
 //
 // Every wait is bounded (tc_common.cuh).  One that gives up raises
 // error_timeout and the CTA's abort flag; softmax threads then run through
@@ -91,6 +94,21 @@ template <int SLOTS> struct Tail
     uint32_t tmem;
     int abort;
 };
+__device__ __forceinline__ void tmem_load32(uint32_t address, uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32"
+                 " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
+                 " %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+                   "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+                   "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+                   "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(address)
+                 : "memory");
+}
+
 __device__ __forceinline__ uint32_t tmem_load1(uint32_t address)
 {
     uint32_t r;
@@ -236,6 +254,43 @@ template <bool TWO> __device__ __forceinline__ void operand(int op, int tiles, b
     tile = k < 0 ? op : (k >= steady ? tiles - 2 + (k - steady) : (k & 1 ? (k >> 1) + 2 : k >> 1));
 }
 
+// ------------------------------------------------- pairs of 32-bit numbers --
+using Pair = unsigned long long;
+
+__device__ __forceinline__ Pair make_pair(float a, float b)
+{
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ void split(Pair p, float& a, float& b)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ Pair fma_pair(Pair a, Pair b, Pair c)
+{
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ Pair add_pair(Pair a, Pair b)
+{
+    Pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Pair mul_pair(Pair a, Pair b)
+{
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 // One number for each softmax group, selected without an array in memory.
 template <class N> struct Both
 {
@@ -682,96 +737,83 @@ __global__ void __launch_bounds__(THREADS, 1)
             {
                 const int tile = g.tile_begin + j;
                 const bool masked = Work::is_masked(g, tile);
-                // Scores 16 c to 16 c + 15 of this row, those it does not see made -infinity.
-                const auto hide = [&](int c, uint32_t (&s)[16])
-                {
-                    const uint32_t bits = Work::visible(g, tile, c >> 1, sees) >> (16 * (c & 1));
-#pragma unroll
-                    for (int k = 0; k < 16; ++k)
-                        s[k] = bits >> k & 1u ? s[k] : 0xff800000u;
-                };
                 wait(tail.scores[group], scores_seen++);
                 __syncwarp();
                 tc_fence_after();
                 if (busy)
                 {
-                    const bool first = TWO ? j == 0 : j < 2;
-                    if (first)
-                    {
-                        float best = -INFINITY;
+                    Pair part = make_pair(0.0f, 0.0f);
 #pragma unroll 1
-                        for (int c = 0; c < KEYS / 16; ++c)
-                        {
-                            uint32_t s[16];
-                            tmem_load16(my_scores + 16 * c, s);
-                            tmem_wait16(s);
-                            if (masked)
-                                hide(c, s);
-#pragma unroll
-                            for (int k = 0; k < 16; ++k)
-                                best = fmaxf(best, __uint_as_float(s[k]));
-                        }
-                        maximum = best == -INFINITY ? -INFINITY : best * scale;
-                    }
-                    uint32_t p[KEYS / 2];
-                    float part[2];
-                    // p with the maximum so far; returns the tile's own maximum.
-                    const auto exponentials = [&]
+                    for (int c = 0; c < KEYS / 32; ++c)
                     {
-                        const float shift = maximum == -INFINITY ? 0.0f : -maximum;
-                        float best[2] = {-INFINITY, -INFINITY};
-                        part[0] = part[1] = 0.0f;
-                        uint32_t s[2][16];
-                        tmem_load16(my_scores, s[0]);
-#pragma unroll
-                        for (int c = 0; c < KEYS / 16; ++c)
+                        uint32_t s[32];
+                        tmem_load32(my_scores + 32 * c, s);
+                        if (masked)
                         {
-                            uint32_t(&now)[16] = s[c & 1];
-                            tmem_wait16(now);
-                            if (c + 1 < KEYS / 16) // the next scores are on their way while these are used
-                                tmem_load16(my_scores + 16 * (c + 1), s[(c + 1) & 1]);
-                            if (masked)
-                                hide(c, now);
+                            const uint32_t bits = Work::visible(g, tile, c, sees);
 #pragma unroll
-                            for (int k = 0; k < 16; k += 2)
+                            for (int k = 0; k < 32; ++k)
+                                s[k] = bits >> k & 1u ? s[k] : 0xff800000u; // -infinity
+                        }
+                        float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (int k = 0; k < 32; k += 2)
+                            best[k >> 1 & 3] = max3(best[k >> 1 & 3], __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
+                        const float highest = max3(best[0], best[1], fmaxf(best[2], best[3]));
+                        const float top = highest == -INFINITY ? -INFINITY : highest * scale;
+                        if (__any_sync(0xffffffffu, top > maximum + RESCALE))
+                        {
+                            const float raised = fmaxf(maximum, ceilf(top));
+                            const float shrink = maximum == -INFINITY ? 0.0f : power_of_two(maximum - raised);
+                            maximum = raised;
+                            sum *= shrink;
+                            part = mul_pair(part, make_pair(shrink, shrink));
+                            // P of this tile's earlier scores, then the output; its last product is
+                            // complete, these scores were issued after it.
+                            tmem_wait_stores();
+#pragma unroll 1
+                            for (int b = 0; b < c; ++b)
                             {
-                                best[0] = fmaxf(best[0], __uint_as_float(now[k]));
-                                best[1] = fmaxf(best[1], __uint_as_float(now[k + 1]));
-                                const float x = power_of_two(fmaf(__uint_as_float(now[k]), scale, shift));
-                                const float y = power_of_two(fmaf(__uint_as_float(now[k + 1]), scale, shift));
-                                part[0] += x;
-                                part[1] += y;
-                                p[8 * c + k / 2] = Half2<T>::pack(x, y);
+                                uint32_t w[16];
+                                tmem_load16(my_scores + 16 * b, w);
+                                tmem_wait16(w);
+#pragma unroll
+                                for (int k = 0; k < 16; ++k)
+                                    w[k] = Half2<T>::pack(Half2<T>::value(static_cast<std::uint16_t>(w[k])) * shrink,
+                                                          Half2<T>::value(static_cast<std::uint16_t>(w[k] >> 16)) * shrink);
+                                tmem_store16(my_scores + 16 * b, w);
+                            }
+#pragma unroll 1
+                            for (int b = 0; b < D / 16 && (TWO ? j > 0 : j > 1); ++b)
+                            {
+                                uint32_t w[16];
+                                tmem_load16(my_output + 16 * b, w);
+                                tmem_wait16(w);
+#pragma unroll
+                                for (int k = 0; k < 16; ++k)
+                                    w[k] = __float_as_uint(__uint_as_float(w[k]) * shrink);
+                                tmem_store16(my_output + 16 * b, w);
                             }
                         }
-                        const float highest = fmaxf(best[0], best[1]);
-                        return highest == -INFINITY ? -INFINITY : highest * scale;
-                    };
-                    const float top = exponentials();
-                    if (!first && __any_sync(0xffffffffu, top > maximum + RESCALE))
-                    {
-                        const float raised = fmaxf(maximum, top);
-                        const float shrink = maximum == -INFINITY ? 0.0f : power_of_two(maximum - raised);
-                        maximum = raised;
-                        sum *= shrink;
-                        // The product before these scores is complete: they were issued after it.
-#pragma unroll 1
-                        for (int c = 0; c < D / 16; ++c)
+                        const float shift = maximum == -INFINITY ? 0.0f : -maximum;
+                        uint32_t p[16];
+#pragma unroll
+                        for (int k = 0; k < 32; k += 2)
                         {
-                            uint32_t o[16];
-                            tmem_load16(my_output + 16 * c, o);
-                            tmem_wait16(o);
-#pragma unroll
-                            for (int k = 0; k < 16; ++k)
-                                o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
-                            tmem_store16(my_output + 16 * c, o);
+                            float x, y;
+                            split(fma_pair(make_pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])),
+                                           make_pair(scale, scale), make_pair(shift, shift)),
+                                  x, y);
+                            x = power_of_two(x);
+                            y = power_of_two(y);
+                            part = add_pair(part, make_pair(x, y));
+                            p[k / 2] = Half2<T>::pack(x, y);
                         }
-                        exponentials();
+                        tmem_store16(my_scores + 16 * c, p); // over scores that have been read
                     }
-                    sum += part[0] + part[1];
-#pragma unroll
-                    for (int c = 0; c < KEYS / 32; ++c)
-                        tmem_store16(my_scores + 16 * c, p + 16 * c); // over scores that have been read
+                    float even, odd;
+                    split(part, even, odd);
+                    sum += even + odd;
                     tmem_wait_stores();
                 }
                 tc_fence_before();
