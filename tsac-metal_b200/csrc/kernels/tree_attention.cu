@@ -48,9 +48,9 @@ __device__ __forceinline__ void load_matrices_transposed(std::uint32_t address, 
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <int D, int MT> struct Layout
+template <int D> struct Layout
 {
-    static constexpr int ROWS = 16 * MT;
+    static constexpr int ROWS = 16; // of an item: the rows of an mma.sync tile
     static constexpr int WARP_KEYS = D == 128 ? 16 : 32, KEYS = WARPS * WARP_KEYS;
     static constexpr int row_bytes = 2 * D, chunks = D / 8;
     static constexpr int stage_bytes = 2 * WARP_KEYS * row_bytes; // keys, then values
@@ -59,12 +59,12 @@ template <int D, int MT> struct Layout
     static constexpr int smem = ring_bytes > merge_bytes ? ring_bytes : merge_bytes;
 };
 
-template <class T, int D, int MT>
+template <class T, int D>
 __global__ void __launch_bounds__(THREADS, 2)
     tree_attention_kernel(const TreeArgs a, float* pieces, TreeShared* shared_items)
 {
     pdl_prologue();
-    using L = Layout<D, MT>;
+    using L = Layout<D>;
     using Work = TreeWork<L::KEYS, L::ROWS, 1>;
     constexpr int WARP_KEYS = L::WARP_KEYS, NT = WARP_KEYS / 8; // keys of a warp, and their groups of 8
     extern __shared__ __align__(128) unsigned char smem[];
@@ -127,31 +127,23 @@ __global__ void __launch_bounds__(THREADS, 2)
         }
 
         // Query fragments: row lane / 4 (+ 8), columns 2 (lane % 4) (+ 8) of each 16.
-        std::uint32_t q[MT][D / 16][4];
+        std::uint32_t q[D / 16][4];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-            {
-                const int row = first_row + 16 * m + 8 * r + (lane >> 2);
-                const int node = row / a.group, in_group = row - node * a.group;
-                const std::uint16_t* from = a.query + g.list_entry * a.query_batch + node * a.query_node +
-                                            (head * a.group + in_group) * a.query_head + 2 * (lane & 3);
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k)
-                {
-                    q[m][k][r] = row < rows ? *reinterpret_cast<const std::uint32_t*>(from + 16 * k) : 0u;
-                    q[m][k][r + 2] = row < rows ? *reinterpret_cast<const std::uint32_t*>(from + 16 * k + 8) : 0u;
-                }
-            }
-        float o[MT][D / 8][4] = {};
-        float top[MT][2], sum[MT][2];
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int r = 0; r < 2; ++r)
         {
-            top[m][0] = top[m][1] = -INFINITY;
-            sum[m][0] = sum[m][1] = 0.0f;
+            const int row = first_row + 8 * r + (lane >> 2);
+            const int node = row / a.group, in_group = row - node * a.group;
+            const std::uint16_t* from = a.query + g.list_entry * a.query_batch + node * a.query_node +
+                                        (head * a.group + in_group) * a.query_head + 2 * (lane & 3);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+            {
+                q[k][r] = row < rows ? *reinterpret_cast<const std::uint32_t*>(from + 16 * k) : 0u;
+                q[k][r + 2] = row < rows ? *reinterpret_cast<const std::uint32_t*>(from + 16 * k + 8) : 0u;
+            }
         }
+        float o[D / 8][4] = {};
+        float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
 
         int stage = 0;
         for (int tile = tile_begin; tile < tile_end; ++tile)
@@ -165,7 +157,7 @@ __global__ void __launch_bounds__(THREADS, 2)
             const std::uint32_t keys = ring + stage * L::stage_bytes, values = keys + WARP_KEYS * L::row_bytes;
             stage = stage + 1 == STAGES ? 0 : stage + 1;
 
-            float s[MT][NT][4] = {};
+            float s[NT][4] = {};
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
 #pragma unroll
@@ -175,12 +167,8 @@ __global__ void __launch_bounds__(THREADS, 2)
                     const int row = 16 * half + (lane & 7) + ((lane >> 4) << 3), chunk = 2 * k + ((lane >> 3) & 1);
                     std::uint32_t b[4];
                     load_matrices(keys + row * L::row_bytes + ((chunk ^ (row & 7)) << 4), b);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m)
-                    {
-                        Half2<T>::mma(s[m][2 * half], q[m][k], b[0], b[1]);
-                        Half2<T>::mma(s[m][2 * half + 1], q[m][k], b[2], b[3]);
-                    }
+                    Half2<T>::mma(s[2 * half], q[k], b[0], b[1]);
+                    Half2<T>::mma(s[2 * half + 1], q[k], b[2], b[3]);
                 }
             const bool last = Work::is_last(g, tile);
             const bool masked = Work::is_masked(g, tile);
@@ -206,59 +194,57 @@ __global__ void __launch_bounds__(THREADS, 2)
                     tainted |= __any_sync(0xffffffffu, odd) ? 1u << row : 0u;
                 }
             }
-            std::uint32_t p[MT][NT / 2][4];
-            float exact_p[MT][2][2 * NT];
+            std::uint32_t p[NT / 2][4];
+            float exact_p[2][2 * NT];
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int r = 0; r < 2; ++r)
+            for (int r = 0; r < 2; ++r)
+            {
+                std::uint32_t sees = ~0u;
+                if (masked)
                 {
-                    std::uint32_t sees = ~0u;
-                    if (masked)
-                    {
-                        const int row = first_row + 16 * m + 8 * r + (lane >> 2);
-                        sees = Work::visible(g, tile, warp * WARP_KEYS / 32, last && row < rows ? masks[row / a.group] : 0ull) >>
-                               (first_bit + 2 * (lane & 3)); // this lane's keys: bits 0 and 1 of each 8
-                    }
-                    float z[2 * NT], best = top[m][r];
+                    const int row = first_row + 8 * r + (lane >> 2);
+                    sees = Work::visible(g, tile, warp * WARP_KEYS / 32, last && row < rows ? masks[row / a.group] : 0ull) >>
+                           (first_bit + 2 * (lane & 3)); // this lane's keys: bits 0 and 1 of each 8
+                }
+                float z[2 * NT], best = top[r];
 #pragma unroll
-                    for (int k = 0; k < 2 * NT; ++k)
-                    {
-                        z[k] = s[m][k >> 1][2 * r + (k & 1)] * a.scale_log2;
-                        if (!(sees >> ((k & 1) + 8 * (k >> 1)) & 1u))
-                            z[k] = -INFINITY;
-                        best = fmaxf(best, z[k]);
-                    }
-                    best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
-                    best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
-                    const float shift = best == -INFINITY ? 0.0f : best; // rows that have seen nothing yet
-                    const float scale = power_of_two(top[m][r] - shift);
-                    top[m][r] = best;
-                    float partial = 0.0f;
+                for (int k = 0; k < 2 * NT; ++k)
+                {
+                    z[k] = s[k >> 1][2 * r + (k & 1)] * a.scale_log2;
+                    if (!(sees >> ((k & 1) + 8 * (k >> 1)) & 1u))
+                        z[k] = -INFINITY;
+                    best = fmaxf(best, z[k]);
+                }
+                best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
+                best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
+                const float shift = best == -INFINITY ? 0.0f : best; // rows that have seen nothing yet
+                const float scale = power_of_two(top[r] - shift);
+                top[r] = best;
+                float partial = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < 2 * NT; ++k)
-                    {
-                        z[k] = power_of_two(z[k] - shift);
-                        partial += z[k];
-                        exact_p[m][r][k] = z[k];
-                    }
-                    sum[m][r] = fmaf(sum[m][r], scale, partial);
+                for (int k = 0; k < 2 * NT; ++k)
+                {
+                    z[k] = power_of_two(z[k] - shift);
+                    partial += z[k];
+                    exact_p[r][k] = z[k];
+                }
+                sum[r] = fmaf(sum[r], scale, partial);
 #pragma unroll
-                    for (int half = 0; half < NT / 2; ++half)
-                    {
-                        p[m][half][r] = Half2<T>::pack(z[4 * half], z[4 * half + 1]);
-                        p[m][half][r + 2] = Half2<T>::pack(z[4 * half + 2], z[4 * half + 3]);
-                    }
-                    if (__any_sync(0xffffffffu, scale != 1.0f))
-                    {
+                for (int half = 0; half < NT / 2; ++half)
+                {
+                    p[half][r] = Half2<T>::pack(z[4 * half], z[4 * half + 1]);
+                    p[half][r + 2] = Half2<T>::pack(z[4 * half + 2], z[4 * half + 3]);
+                }
+                if (__any_sync(0xffffffffu, scale != 1.0f))
+                {
 #pragma unroll
-                        for (int n = 0; n < D / 8; ++n)
-                        {
-                            o[m][n][2 * r] *= scale;
-                            o[m][n][2 * r + 1] *= scale;
-                        }
+                    for (int n = 0; n < D / 8; ++n)
+                    {
+                        o[n][2 * r] *= scale;
+                        o[n][2 * r + 1] *= scale;
                     }
                 }
+            }
             if (tainted)
             {
                 // 0 x NaN would reach rows that do not see the node: take such
@@ -270,31 +256,29 @@ __global__ void __launch_bounds__(THREADS, 2)
                         continue;
                     const int k = (key & 1) + 2 * (key >> 3), from = (lane & ~3) | ((key & 7) >> 1);
 #pragma unroll
-                    for (int m = 0; m < MT; ++m)
+                    for (int r = 0; r < 2; ++r)
+                    {
+                        const int row = first_row + 8 * r + (lane >> 2);
+                        const bool seen = row < rows && (masks[row / a.group] >> (first_node + key) & 1ull);
+                        float weight = 0.0f;
 #pragma unroll
-                        for (int r = 0; r < 2; ++r)
+                        for (int kk = 0; kk < 2 * NT; ++kk)
                         {
-                            const int row = first_row + 16 * m + 8 * r + (lane >> 2);
-                            const bool seen = row < rows && (masks[row / a.group] >> (first_node + key) & 1ull);
-                            float weight = 0.0f;
+                            const float w = __shfl_sync(0xffffffffu, exact_p[r][kk], from);
+                            weight = kk == k ? w : weight;
+                        }
 #pragma unroll
-                            for (int kk = 0; kk < 2 * NT; ++kk)
+                        for (int n = 0; n < D / 8; ++n)
+                        {
+                            const std::uint32_t v = *reinterpret_cast<const std::uint32_t*>(
+                                smem + base + key * L::row_bytes + ((n ^ (key & 7)) << 4) + 4 * (lane & 3));
+                            if (seen)
                             {
-                                const float w = __shfl_sync(0xffffffffu, exact_p[m][r][kk], from);
-                                weight = kk == k ? w : weight;
-                            }
-#pragma unroll
-                            for (int n = 0; n < D / 8; ++n)
-                            {
-                                const std::uint32_t v = *reinterpret_cast<const std::uint32_t*>(
-                                    smem + base + key * L::row_bytes + ((n ^ (key & 7)) << 4) + 4 * (lane & 3));
-                                if (seen)
-                                {
-                                    o[m][n][2 * r] = fmaf(weight, Half2<T>::value(v & 0xffffu), o[m][n][2 * r]);
-                                    o[m][n][2 * r + 1] = fmaf(weight, Half2<T>::value(v >> 16), o[m][n][2 * r + 1]);
-                                }
+                                o[n][2 * r] = fmaf(weight, Half2<T>::value(v & 0xffffu), o[n][2 * r]);
+                                o[n][2 * r + 1] = fmaf(weight, Half2<T>::value(v >> 16), o[n][2 * r + 1]);
                             }
                         }
+                    }
                 }
                 __syncwarp();
                 for (int key = 0; key < WARP_KEYS; ++key)
@@ -311,48 +295,40 @@ __global__ void __launch_bounds__(THREADS, 2)
                     const int row = 16 * half + (lane & 7) + (((lane >> 3) & 1) << 3), chunk = 2 * n + (lane >> 4);
                     std::uint32_t b[4];
                     load_matrices_transposed(values + row * L::row_bytes + ((chunk ^ (row & 7)) << 4), b);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m)
-                    {
-                        Half2<T>::mma(o[m][2 * n], p[m][half], b[0], b[1]);
-                        Half2<T>::mma(o[m][2 * n + 1], p[m][half], b[2], b[3]);
-                    }
+                    Half2<T>::mma(o[2 * n], p[half], b[0], b[1]);
+                    Half2<T>::mma(o[2 * n + 1], p[half], b[2], b[3]);
                 }
             __syncwarp(); // the stage may be refilled
         }
         copies_wait<0>();
         // Join the warps: common maximum, scaled outputs through shared memory.
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
+        for (int r = 0; r < 2; ++r)
+        {
+            sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+            sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+            if ((lane & 3) == 0)
             {
-                sum[m][r] += __shfl_xor_sync(0xffffffffu, sum[m][r], 1);
-                sum[m][r] += __shfl_xor_sync(0xffffffffu, sum[m][r], 2);
-                if ((lane & 3) == 0)
-                {
-                    row_max[warp][16 * m + 8 * r + (lane >> 2)] = top[m][r];
-                    row_sum[warp][16 * m + 8 * r + (lane >> 2)] = sum[m][r];
-                }
+                row_max[warp][8 * r + (lane >> 2)] = top[r];
+                row_sum[warp][8 * r + (lane >> 2)] = sum[r];
             }
+        }
         __syncthreads();
         float* merge = reinterpret_cast<float*>(smem);
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int r = 0; r < 2; ++r)
+        {
+            const int row = 8 * r + (lane >> 2);
+            float best = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
-            {
-                const int row = 16 * m + 8 * r + (lane >> 2);
-                float best = -INFINITY;
+            for (int w = 0; w < WARPS; ++w)
+                best = fmaxf(best, row_max[w][row]);
+            const float scale = best == -INFINITY ? 0.0f : power_of_two(top[r] - best);
 #pragma unroll
-                for (int w = 0; w < WARPS; ++w)
-                    best = fmaxf(best, row_max[w][row]);
-                const float scale = best == -INFINITY ? 0.0f : power_of_two(top[m][r] - best);
-#pragma unroll
-                for (int n = 0; n < D / 8; ++n)
-                    *reinterpret_cast<float2*>(merge + (warp * L::ROWS + row) * D + 8 * n + 2 * (lane & 3)) =
-                        make_float2(o[m][n][2 * r] * scale, o[m][n][2 * r + 1] * scale);
-            }
+            for (int n = 0; n < D / 8; ++n)
+                *reinterpret_cast<float2*>(merge + (warp * L::ROWS + row) * D + 8 * n + 2 * (lane & 3)) =
+                    make_float2(o[n][2 * r] * scale, o[n][2 * r + 1] * scale);
+        }
         __syncthreads();
         const bool whole = tile_begin == 0 && tile_end == e.tiles;
         // A piece that begins its item goes to the CTA's second place, any other to its first.
@@ -556,7 +532,7 @@ struct Shape
 template <class T, int D>
 void launch_few(const TreeArgs& a, const Shape& shape, float* pieces, TreeShared* items, cudaStream_t stream)
 {
-    using L = Layout<D, 1>;
+    using L = Layout<D>;
     static std::once_flag once[64];
     int device = 0;
     cudaGetDevice(&device);
@@ -564,10 +540,10 @@ void launch_few(const TreeArgs& a, const Shape& shape, float* pieces, TreeShared
         std::call_once(once[device],
                        []
                        {
-                           cudaFuncSetAttribute(tree_attention_kernel<T, D, 1>,
+                           cudaFuncSetAttribute(tree_attention_kernel<T, D>,
                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem);
                        });
-    launch_pdl(tree_attention_kernel<T, D, 1>, dim3(shape.ctas), dim3(THREADS), L::smem, stream, a, pieces, items);
+    launch_pdl(tree_attention_kernel<T, D>, dim3(shape.ctas), dim3(THREADS), L::smem, stream, a, pieces, items);
     note_launch();
 }
 
@@ -599,6 +575,9 @@ template <class T> cudaError_t launch_type(const TreeArgs& a, ValueType type, vo
 }
 } // namespace
 
+// 16 rows are one mma.sync tile of each warp.  Two tiles would spill at 128
+// columns, and at 64 took 188 us for 96 sequences of up to 8,191 positions with
+// 32 rows, the tensor cores 158.
 bool tree_attention_many(int rows)
 {
     return rows > 16;

@@ -26,9 +26,10 @@
 //                   a lane each.  Value tiles with rows behind the last position
 //                   come by 16-byte asynchronous copies that make those rows
 //                   zeros, as does everything where TMA does not serve: pages of
-//                   fewer than 8 rows (a swizzle atom), or 2^31 rows in a plane.  Copies of every tile by the two warps
-//                   bound the kernel by their address arithmetic (290 against
-//                   209 us for 64 x 16 nodes over up to 4,096 positions).
+//                   fewer than 8 rows (a swizzle atom), or 2^31 rows in a plane.
+//                   Copies of every tile by the two warps bound the kernel by
+//                   their address arithmetic (290 against 209 us for 64 x 16
+//                   nodes over up to 4,096 positions).
 //   warp 11         the query rows of the next segment, as soon as the last
 //                   scores of this one are made, and its tree's masks.
 // The running maximum is a whole number and moves only when a row's scores
