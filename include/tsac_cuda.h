@@ -418,10 +418,11 @@ int tsac_cuda_range_decode_tree(const uint8_t* bytes, size_t size, const float* 
  * allocate nothing, never read the device from the host, and may be captured
  * into a CUDA graph.  The device that holds the buffers must be current.
  * Faults that only the device can see (an invalid sequence, page or position,
- * a sequence named twice) skip the entry concerned, leave its outputs as they
- * were, and OR bit 16 into *error_word (nullable); none reads or writes
- * outside the buffers as long as the counts given here are true.  Two calls
- * on one cache must not overlap unless both only read it. */
+ * a sequence named twice where it must not be) skip the entry concerned, leave
+ * its outputs as they were where not stated otherwise, and OR bit 16 into
+ * *error_word (nullable); none reads or writes outside the buffers as long as
+ * the counts given here are true.  Calls on one cache must not overlap unless
+ * all of them only read it, as tsac_cuda_tree_attention does. */
 
 enum tsac_cuda_value_type
 {
@@ -494,7 +495,9 @@ int tsac_cuda_cache_release(const tsac_cuda_paged_cache* cache, const int32_t* s
  *                 type with the given strides in elements (multiples of 8; the
  *                 last dimension is contiguous), 16-byte aligned
  *   nodes         device int32 [count] or NULL: max_nodes each
- * max_nodes may be any length here (a prompt, for instance). */
+ * max_nodes may be any length here (a prompt, for instance).  A row whose page
+ * is missing or shared is skipped (bit 16).  A sequence may be listed more than
+ * once with starts whose rows do not overlap. */
 int tsac_cuda_cache_append(const tsac_cuda_paged_cache* cache, size_t layer, const void* keys,
                            const ptrdiff_t key_strides[3], const void* values,
                            const ptrdiff_t value_strides[3], const int32_t* sequences,
@@ -541,8 +544,12 @@ int tsac_cuda_cache_compact(const tsac_cuda_paged_cache* cache, int32_t* tables_
  *   scratch  device, >= tsac_cuda_tree_attention_scratch_bytes(cache, heads,
  *            max_nodes), 16-byte aligned; calls that overlap need their own
  * A row that sees nothing gives zeros and -infinity.  A value that is not
- * finite reaches the rows that see it and no others.  max_nodes 1 is plain
- * decoding.  head_dim 64 or 128; max_nodes <= TSAC_CUDA_MAX_NODES. */
+ * finite reaches the rows that see it and no others.  An entry whose length
+ * and nodes exceed its pages is skipped (bit 16); a table entry that is no page
+ * of the pool is reported likewise and read as zeros.  The same sequence may be
+ * listed more than once.  The order of the sums depends on all lengths and
+ * nodes of the call, and on nothing else.  max_nodes 1 is plain decoding.
+ * head_dim 64 or 128; max_nodes <= TSAC_CUDA_MAX_NODES. */
 size_t tsac_cuda_tree_attention_scratch_bytes(const tsac_cuda_paged_cache* cache, size_t heads,
                                               size_t max_nodes);
 int tsac_cuda_tree_attention(const tsac_cuda_paged_cache* cache, size_t layer, const int32_t* sequences,

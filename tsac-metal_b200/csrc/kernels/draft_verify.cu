@@ -590,9 +590,9 @@ template <class T, bool DRAFT, int CLUSTER, int THREADS> cudaError_t launch(cons
     attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
     config.numAttrs = 2;
-    const cudaError_t status = cudaLaunchKernelEx(&config, draft_verify_kernel<T, DRAFT, CLUSTER, THREADS>, a);
+    cudaLaunchKernelEx(&config, draft_verify_kernel<T, DRAFT, CLUSTER, THREADS>, a);
     note_launch();
-    return status;
+    return cudaGetLastError();
 }
 
 // CTAs for one sequence.  Small vocabularies are latency alone: one CTA of 128
