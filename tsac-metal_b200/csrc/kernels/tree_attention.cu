@@ -384,9 +384,10 @@ __global__ void __launch_bounds__(THREADS, 2)
 // Joins the pieces of an item that several CTAs share.  Piece 0 is in the first
 // CTA's second place, the others in their CTAs' first places.  Each CTA lists
 // the shared items, so that the rows spread over the whole grid, and gives each
-// row 1, 4 or 16 warps, as many as the grid has for all rows at once: the warps
-// take the pieces in turn, several in flight, and are joined in shared memory
-// in a fixed order.  Bound by the latency of three dependent reads.
+// row up to 16 warps, one for four pieces as far as the grid has warps for all
+// rows at once: the warps take the pieces in turn, four in flight, and are
+// joined in shared memory in a fixed order.  Bound by the latency of three
+// dependent reads.
 constexpr int COMBINE_WARPS = 16, COMBINE_THREADS = COMBINE_WARPS * 32;
 
 template <class T, int D>
@@ -396,13 +397,18 @@ __global__ void __launch_bounds__(COMBINE_THREADS)
     pdl_prologue();
     constexpr int PER = D / 32; // columns of one lane
     __shared__ float part[COMBINE_WARPS][D + 2];
-    __shared__ int rows_until[COMBINE_THREADS], warp_sums[COMBINE_WARPS];
+    __shared__ int rows_until[COMBINE_THREADS], warp_sums[COMBINE_WARPS], most_pieces;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     int until = 0; // rows of the shared items up to the thread's
+    if (t == 0)
+        most_pieces = 0;
+    __syncthreads();
     if (t < ctas)
     {
         const TreeShared s = shared_items[t];
         until = s.pieces ? min(s.nodes * a.group - s.first_row, rows_per_item) : 0;
+        if (s.pieces)
+            atomicMax(&most_pieces, s.pieces);
     }
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1)
@@ -419,7 +425,9 @@ __global__ void __launch_bounds__(COMBINE_THREADS)
     __syncthreads();
     const int rows = rows_until[COMBINE_THREADS - 1];
     const int warps = static_cast<int>(gridDim.x) * COMBINE_WARPS;
-    const int shares = rows * 16 <= warps ? 16 : (rows * 4 <= warps ? 4 : 1); // warps of one row
+    int shares = 1; // warps of one row, a power of two
+    while (shares < COMBINE_WARPS && 4 * shares < most_pieces && 2 * shares * rows <= warps)
+        shares *= 2;
     const int at_once = COMBINE_WARPS / shares, share = warp & (shares - 1);
     for (int first = blockIdx.x * at_once; first < rows; first += gridDim.x * at_once)
     {

@@ -52,22 +52,18 @@ template <int KEYS, int ROWS, int START> struct TreeWork
     {
         Entry e;
         e.sequence = cache_sequence(a.cache, a.sequences, i);
+        // All reads at once: a caller waits for one round trip.
+        const int s = e.sequence < 0 ? 0 : e.sequence;
         e.nodes = a.nodes ? a.nodes[i] : a.max_nodes;
+        e.held = cache_held(a.cache, s);
+        e.length = a.cache.lengths[s];
         e.nodes = e.nodes < a.max_nodes ? e.nodes : a.max_nodes;
-        e.units = e.tiles = e.row_items = e.length = e.held = e.last_base = 0;
-        if (e.nodes <= 0)
-            return e;
-        bool valid = e.sequence >= 0;
-        if (valid)
+        e.tiles = e.row_items = e.last_base = 0;
+        e.units = 0;
+        const bool valid = e.sequence >= 0 && e.length >= 0 && static_cast<long long>(e.length) + e.nodes <= static_cast<long long>(e.held) << a.cache.page_shift;
+        if (e.nodes <= 0 || !valid)
         {
-            e.held = cache_held(a.cache, e.sequence);
-            e.length = a.cache.lengths[e.sequence];
-            valid = e.length >= 0 &&
-                    static_cast<long long>(e.length) + e.nodes <= static_cast<long long>(e.held) << a.cache.page_shift;
-        }
-        if (!valid)
-        {
-            if (a.error_word)
+            if (e.nodes > 0 && a.error_word)
                 atomicOr(a.error_word, error_cache);
             return e;
         }
@@ -108,23 +104,42 @@ template <int KEYS, int ROWS, int START> struct TreeWork
         long long first, last; // the CTA's share
     };
 
+    static __device__ __forceinline__ long long warp_inclusive(long long v)
+    {
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1)
+        {
+            const long long up = __shfl_up_sync(0xffffffffu, v, d);
+            v += (threadIdx.x & 31) >= d ? up : 0;
+        }
+        return v;
+    }
+
     // The CTA's first list entry, by the whole CTA (THREADS threads, a multiple of 32).
     template <int THREADS>
     static __device__ Start find(const TreeArgs& a, int cta, int ctas, long long* warp_sums, Start* found)
     {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        if (a.count <= 32) // each warp for itself, without a barrier
+        {
+            const long long mine = lane < a.count ? entry(a, lane).units : 0;
+            const long long until = warp_inclusive(mine);
+            Start s;
+            s.units = __shfl_sync(0xffffffffu, until, 31);
+            s.ctas = s.units < ctas ? static_cast<int>(s.units) : ctas;
+            s.first = cta < s.ctas ? first_unit(s.units, cta, s.ctas) : s.units;
+            s.last = cta < s.ctas ? first_unit(s.units, cta + 1, s.ctas) : s.units;
+            const unsigned behind = __ballot_sync(0xffffffffu, until > s.first); // entries that end behind the first unit
+            s.entry = behind ? __ffs(static_cast<int>(behind)) - 1 : a.count;
+            s.before = __shfl_sync(0xffffffffu, until - mine, s.entry & 31);
+            return s;
+        }
         const int each = (a.count + THREADS - 1) / THREADS;
         const int begin = min(a.count, static_cast<int>(threadIdx.x) * each), end = min(a.count, begin + each);
         long long mine = 0;
         for (int i = begin; i < end; ++i)
             mine += entry(a, i).units;
-        long long inclusive = mine;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1)
-        {
-            const long long up = __shfl_up_sync(0xffffffffu, inclusive, d);
-            inclusive += lane >= d ? up : 0;
-        }
+        const long long inclusive = warp_inclusive(mine);
         if (lane == 31)
             warp_sums[warp] = inclusive;
         if (threadIdx.x == 0)
