@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 // the shared items, so that the rows spread over the whole grid, and gives each
 // row up to 16 warps, one for four pieces as far as the grid has warps for all
 // rows at once: the warps take the pieces in turn, four in flight, and are
-// joined in shared memory in a fixed order.  Bound by the latency of three
+// joined in shared memory in a fixed order.  Bound by the latency of two
 // dependent reads.
 constexpr int COMBINE_WARPS = 16, COMBINE_THREADS = COMBINE_WARPS * 32;
 
@@ -398,6 +398,7 @@ __global__ void __launch_bounds__(COMBINE_THREADS)
     constexpr int PER = D / 32; // columns of one lane
     __shared__ float part[COMBINE_WARPS][D + 2];
     __shared__ int rows_until[COMBINE_THREADS], warp_sums[COMBINE_WARPS], most_pieces;
+    __shared__ TreeShared items[COMBINE_THREADS];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     int until = 0; // rows of the shared items up to the thread's
     if (t == 0)
@@ -406,6 +407,7 @@ __global__ void __launch_bounds__(COMBINE_THREADS)
     if (t < ctas)
     {
         const TreeShared s = shared_items[t];
+        items[t] = s;
         until = s.pieces ? min(s.nodes * a.group - s.first_row, rows_per_item) : 0;
         if (s.pieces)
             atomicMax(&most_pieces, s.pieces);
@@ -436,7 +438,7 @@ __global__ void __launch_bounds__(COMBINE_THREADS)
         int cta = 0; // the first whose running count exceeds the row's
         for (int step = COMBINE_THREADS / 2; step; step >>= 1)
             cta += rows_until[cta + step - 1] <= (live ? index : 0) ? step : 0;
-        const TreeShared item = shared_items[cta];
+        const TreeShared item = items[cta];
         const int row = index - (cta ? rows_until[cta - 1] : 0);
         const long long stride = 2 * tree_piece_floats(rows_per_item, D);
         const auto piece = [&](int k)
