@@ -182,13 +182,6 @@ def _drafting():
     return _drafting_lib
 
 
-def _raw_stream(index):
-    """Handle of the current stream of device `index`, by torch's direct query where it has one."""
-    import torch
-    query = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return query or (lambda i: torch.cuda.current_stream(i).cuda_stream)
-
-
 class _Device:
     """Makes a tensor's device current for a call, and gives its current stream."""
 
@@ -196,7 +189,11 @@ class _Device:
 
     def __init__(self, index):
         import torch
-        self.index, self._cuda, self._stream = index, torch.cuda, _raw_stream(index)
+        self.index, self._cuda = index, torch.cuda
+        # torch's direct queries where it has them: a call asks both, and is itself a few microseconds.
+        self._current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+        self._stream = (getattr(torch._C, "_cuda_getCurrentRawStream", None)
+                        or (lambda i: torch.cuda.current_stream(i).cuda_stream))
 
     @classmethod
     def of(cls, index):
@@ -209,7 +206,7 @@ class _Device:
         return self._stream(self.index)
 
     def call(self, fn, *arguments) -> None:
-        if self._cuda.current_device() == self.index:
+        if self._current() == self.index:
             status = fn(*arguments)
         else:
             with self._cuda.device(self.index):
@@ -222,10 +219,10 @@ def _whole(t, name, dtype, index, shape=None):
     """Address of a contiguous tensor of the given kind on device `index`; None gives a null pointer."""
     if t is None:
         return None
-    if t.dtype is not dtype or t.get_device() != index or not t.is_contiguous() or (shape is not None and t.shape != shape):
-        raise TsacError(f"{name} must be a contiguous {dtype} tensor on cuda:{index}"
-                        + (f" of shape {tuple(shape)}" if shape is not None else ""))
-    return t.data_ptr()
+    if t.dtype is dtype and t.get_device() == index and t.is_contiguous() and (shape is None or t.shape == shape):
+        return t.data_ptr()
+    raise TsacError(f"{name} must be a contiguous {dtype} tensor on cuda:{index}"
+                    + (f" of shape {tuple(shape)}" if shape is not None else ""))
 
 
 _stride_arrays = {}
@@ -246,10 +243,13 @@ def _rows(t, name, dtype, index, shape):
     strides = t.stride()
     if t.dtype is not dtype or t.get_device() != index or t.shape != shape or (strides[-1] != 1 and shape[-1] > 1):
         raise TsacError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on cuda:{index}, its last dimension contiguous")
-    strides = strides[:3]
-    if 1 in shape:  # a dimension of size one is never stepped over: its stride says nothing
-        strides = tuple(0 if n == 1 else s for n, s in zip(shape, strides))
-    return t.data_ptr(), _strides(strides)
+    array = _stride_arrays.get((strides, shape))
+    if array is None:
+        if len(_stride_arrays) >= 1024:
+            _stride_arrays.clear()
+        # A dimension of size one is never stepped over: its stride says nothing.
+        array = _stride_arrays[strides, shape] = (ctypes.c_ssize_t * 3)(*[0 if n == 1 else s for n, s in zip(shape[:3], strides)])
+    return t.data_ptr(), array
 
 
 class PagedCache:
