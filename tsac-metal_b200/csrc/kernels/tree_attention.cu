@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 constexpr int COMBINE_WARPS = 16, COMBINE_THREADS = COMBINE_WARPS * 32;
 
 template <class T, int D>
-__global__ void __launch_bounds__(COMBINE_THREADS)
+__global__ void __launch_bounds__(COMBINE_THREADS, 1)
     tree_combine_kernel(const TreeArgs a, int rows_per_item, int ctas, const float* pieces, const TreeShared* shared_items)
 {
     pdl_prologue();
