@@ -478,7 +478,8 @@ int tsac_cuda_cache_reserve(const tsac_cuda_paged_cache* cache, const int32_t* s
 
 /* children[i], which must hold no page, becomes a copy of parents[i] that
  * shares the pages of its committed positions (device int32 [count] each).
- * A pair whose child is named twice, or is some pair's parent, is refused. */
+ * A pair is refused (bit 16) when an earlier one names its child, or when its
+ * parent is some pair's child. */
 int tsac_cuda_cache_fork(const tsac_cuda_paged_cache* cache, const int32_t* parents,
                          const int32_t* children, size_t count, unsigned* error_word, void* stream);
 
@@ -538,7 +539,8 @@ int tsac_cuda_cache_compact(const tsac_cuda_paged_cache* cache, int32_t* tables_
  *   query, out  device [count][max_nodes][heads][head_dim] of the cache's type
  *            with the given strides in elements (multiples of 8; the last
  *            dimension is contiguous), 16-byte aligned.  heads is a multiple
- *            of kv_heads: query head h reads key head h / (heads / kv_heads)
+ *            of kv_heads: query head h reads key head h / (heads / kv_heads).
+ *            out may be query itself (the same strides), but not overlap it otherwise
  *   lse      device f32 [count][max_nodes][heads] or NULL: log of the sum of
  *            exponentials
  *   scratch  device, >= tsac_cuda_tree_attention_scratch_bytes(cache, heads,

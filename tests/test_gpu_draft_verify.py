@@ -205,3 +205,11 @@ def test_binding_refusals():
         tsac_cuda.draft_verify(target, tokens, parents, coins[:, :2], draws)
     with pytest.raises(tsac_cuda.TsacError, match="draws must be"):
         tsac_cuda.draft_verify(target, tokens, parents, coins, draws.cpu())
+
+
+def test_binding_refuses_error_words_of_other_sizes():
+    target, tokens, parents, coins, draws, _ = (None if t is None else t.cuda() for t in case(2, 3, 16, "fp32", False, 9))
+    for word in (torch.zeros(4, dtype=torch.uint8, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda"),
+                 torch.zeros(0, dtype=torch.int32, device="cuda")):
+        with pytest.raises(tsac_cuda.TsacError, match="32-bit word"):
+            tsac_cuda.draft_verify(target, tokens, parents, coins, draws, error_word=word)

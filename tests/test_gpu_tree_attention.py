@@ -368,3 +368,34 @@ def test_a_whole_drafted_step():
             assert torch.equal(cache.pool[:, :, table[s][i // 8], i % 8], embed[:, :, token])
     cache.release()
     assert cache.refs.sum().item() == 0
+
+
+@pytest.mark.parametrize("kind,dim,group,nodes", [("bf16", 128, 1, 9), ("fp16", 64, 2, 8), ("bf16", 64, 4, 17), ("fp16", 128, 8, 33)])
+def test_output_in_place_of_the_query(kind, dim, group, nodes):
+    """One buffer for query and output, items split over CTAs and whole ones alike."""
+    s = Setup(kind, dim, 2, group, 16, [4000, 3, 90, 700], [nodes, nodes, 2, nodes], seed=17)
+    buffer = s.query.cuda()
+    lse = torch.full((4, nodes, 2 * group), 77.0, device="cuda")
+    out = s.cache.attention(0, buffer, ints(s.parents), buffer, nodes=ints(s.nodes), lse=lse)
+    assert out is buffer
+    got = out.cpu().double()
+    assert torch.equal(got[2, 2:], s.query[2, 2:].double())
+    got[2, 2:] = 77.0
+    s.check(got, lse.cpu().double())
+
+
+@pytest.mark.parametrize("kind,dim,group,nodes", [("bf16", 128, 2, 7), ("fp16", 64, 1, 16), ("fp16", 128, 4, 20), ("bf16", 64, 8, 30)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_queries_that_are_not_finite_stay_in_their_rows(kind, dim, group, nodes, bad):
+    s = Setup(kind, dim, 2, group, 16, [300, 20], [nodes, nodes], seed=18)
+    clean, clean_lse = s.run()
+    finite = s.query.clone()
+    spoiled = [(0, 0, 0), (0, nodes - 1, 2 * group - 1), (1, nodes // 2, group)]
+    for b, n, h in spoiled:
+        s.query[b, n, h, 5] = bad
+    out, lse = s.run()
+    s.query = finite
+    for b, n, h in spoiled:
+        assert not torch.isfinite(out[b, n, h]).any()
+        out[b, n, h], lse[b, n, h] = clean[b, n, h], clean_lse[b, n, h]
+    s.check(out, lse)

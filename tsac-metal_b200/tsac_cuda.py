@@ -225,6 +225,14 @@ def _whole(t, name, dtype, index, shape=None):
                     + (f" of shape {tuple(shape)}" if shape is not None else ""))
 
 
+def _error_word(word, index):
+    if word is None:
+        return None
+    if word.numel() < 1 or word.element_size() != 4:
+        raise TsacError("error_word must hold a 32-bit word")
+    return _whole(word, "error_word", word.dtype, index)
+
+
 _stride_arrays = {}
 
 
@@ -258,7 +266,8 @@ class PagedCache:
     pool: [layers][2: keys, values][pages][page_size][kv_heads][head_dim], bf16
     or fp16; tables int32 [sequences][max_pages]; counts, lengths int32
     [sequences]; refs int32 [pages].  The tensors stay the caller's: reading,
-    saving or replacing their contents between calls is fine.
+    saving or replacing their contents between calls is fine.  Keep the object
+    as long as a CUDA graph that was captured from its calls.
     """
 
     def __init__(self, pool, tables, counts, lengths, refs):
@@ -298,11 +307,7 @@ class PagedCache:
         return _whole(sequences, "sequences", self._int, self.index, (count,))
 
     def _word(self, error_word):
-        if error_word is None:
-            return None
-        if error_word.numel() < 1 or error_word.element_size() != 4:
-            raise TsacError("error_word must hold a 32-bit word")
-        return _whole(error_word, "error_word", error_word.dtype, self.index)
+        return _error_word(error_word, self.index)
 
     def _temporary(self, nbytes):
         return self._torch.empty(max(nbytes, 16), dtype=self._torch.uint8, device=self.device)
@@ -310,13 +315,19 @@ class PagedCache:
     def _kept(self, nbytes):
         """Temporary memory of the calls that change the cache, which must not overlap: kept from one to the next.
         A larger one is added, not exchanged: a captured graph goes on using the one that it was captured with."""
-        if not self._scratches or self._scratches[-1].numel() < nbytes:
-            last = self._scratches[-1].numel() if self._scratches else 0
-            self._scratches.append(self._temporary(max(nbytes, 2 * last)))
-        return self._scratches[-1]
+        stream = self._on.stream()
+        if not self._scratches or self._scratches[-1][0].numel() < nbytes:
+            last = self._scratches[-1][0].numel() if self._scratches else 0
+            self._scratches.append((self._temporary(max(nbytes, 2 * last)), stream))
+        scratch, owner = self._scratches[-1]
+        if owner != stream:  # the allocator must not hand it out again before this stream is done with it
+            scratch.record_stream(self._torch.cuda.current_stream(self.index))
+        return scratch
 
     def reserve(self, positions, sequences=None, slots=None, error_word=None):
         """Makes positions[i] further positions of each sequence writable (all or nothing)."""
+        if positions.dim() != 1:
+            raise TsacError("positions must be [entry]")
         count = positions.shape[0]
         slots = slots or self.max_pages
         nbytes = self._lib.tsac_cuda_cache_reserve_scratch_bytes(count, slots)
@@ -327,6 +338,8 @@ class PagedCache:
 
     def fork(self, parents, children, error_word=None):
         """children[i], empty so far, shares the committed pages of parents[i]."""
+        if parents.dim() != 1:
+            raise TsacError("parents must be [entry]")
         count = parents.shape[0]
         self._on.call(self._lib.tsac_cuda_cache_fork, self._cache,
                       _whole(parents, "parents", self._int, self.index, (count,)),
@@ -335,6 +348,8 @@ class PagedCache:
 
     def release(self, sequences=None, positions=None, error_word=None):
         """Gives back the pages behind positions[i] (None: all) of each sequence."""
+        if sequences is not None and sequences.dim() != 1:
+            raise TsacError("sequences must be [entry]")
         count = sequences.shape[0] if sequences is not None else self.sequences
         self._on.call(self._lib.tsac_cuda_cache_release, self._cache, self._list(sequences, count),
                       _whole(positions, "positions", self._int, self.index, (count,)), count,
@@ -342,6 +357,8 @@ class PagedCache:
 
     def append(self, layer, keys, values, nodes=None, sequences=None, starts=None, error_word=None):
         """Stores [entry][node][kv_heads][head_dim] rows of one layer behind each sequence's length (or at starts)."""
+        if keys.dim() != 4:
+            raise TsacError("keys must be [entry][node][kv_heads][head_dim]")
         count, most, _, _ = keys.shape
         shape, index, ints = (count, most, self.kv_heads, self.head_dim), self.index, self._int
         k, key_strides = _rows(keys, "keys", self.dtype, index, shape)
@@ -354,6 +371,8 @@ class PagedCache:
 
     def keep(self, path, accepted, starts=None, lengths_out=None, sequences=None, error_word=None):
         """Keeps rows start + path[i][:accepted[i]], in every layer, as the next positions."""
+        if path.dim() != 2:
+            raise TsacError("path must be [entry][width]")
         count, width = path.shape
         out = self.lengths if lengths_out is None else lengths_out
         self._on.call(self._lib.tsac_cuda_cache_keep, self._cache, self._list(sequences, count),
@@ -423,7 +442,7 @@ def draft_verify(target, tokens, parents, coins, draws, draft=None, nodes=None, 
         accepted, path, token = out
         places = (_whole(accepted, "accepted", ints, index, ones), _whole(path, "path", ints, index, rows),
                   _whole(token, "token", ints, index, ones))
-    word = None if error_word is None else _whole(error_word, "error_word", error_word.dtype, index)
+    word = None if error_word is None else _error_word(error_word, index)
     on = _Device.of(index)
     on.call(lib.tsac_cuda_draft_verify, target.data_ptr(), _strides(target.stride()[:2]),
             None if draft is None else draft.data_ptr(), None if draft is None else _strides(draft.stride()[:2]), types[kind],
