@@ -448,3 +448,89 @@ def test_captured_reservation_outlives_larger_ones():
         graph.replay()
     assert all((guard == 17).all() for guard in guards)
     assert torch.equal(cache.refs, want[0]) and torch.equal(cache.tables, want[1])
+
+
+def test_long_reservation_among_short_ones():
+    """A prompt's pages in one call with entries of none, one and two pages, taken in list order."""
+    pair = Pair(pages=6000, page_size=4, sequences=6, max_pages=5000, layers=1)
+    pair.grow([(4, 3), (0, 8)])
+    assert pair.reserve([(1, 1), (3, 0), (0, 19800), (4, 1), (2, 8), (5, 2900)])
+    pair.check()
+    assert not pair.reserve([(2, 4000)])
+    assert pair.word() == 8
+    pair.check()
+
+
+@pytest.mark.parametrize("outside", [True, False])
+def test_several_shared_pages_in_a_range(outside):
+    """Lengths taken back into shared pages: each writer copies each of them, but the last where no other holds it."""
+    pair = Pair(pages=60, page_size=8, sequences=6, max_pages=8)
+    pair.grow([(0, 40)])
+    pair.fork([(0, s) for s in (1, 2, 3, 4)])
+    if not outside:
+        pair.release([(0, 0)])
+    for s, length in ((1, 3), (2, 17), (3, 9), (4, 0)):
+        pair.gpu.lengths[s] = length
+        pair.book.lengths[s] = length
+    assert pair.reserve([(2, 10), (4, 30), (1, 20), (5, 9), (3, 20)])
+    pair.check()
+    assert pair.reserve([(4, 3), (2, 30)])
+    pair.check()
+
+
+def test_many_sequences_share_many_pages():
+    """4,095 sequences that hold the same 24 pages part from all of them in one call, one keeping them."""
+    count, shared = 4095, 24
+    cache = tsac_cuda.PagedCache.empty(1, count * shared + 3, 1, 1, 8, count, shared)
+    cache.reserve(ints([shared] + [0] * (count - 1)))
+    cache.lengths[0] = shared
+    cache.pool[:, :, :shared] = torch.arange(shared, device="cuda", dtype=torch.bfloat16)[:, None, None, None]
+    children = torch.arange(1, count, dtype=torch.int32, device="cuda")
+    cache.fork(torch.zeros_like(children), children)
+    assert (cache.refs[:shared] == count).all()
+    cache.lengths.zero_()
+    errors = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cache.reserve(torch.full((count,), shared, dtype=torch.int32, device="cuda"), error_word=errors)
+    assert errors.item() == 0
+    want = torch.arange(shared, shared * count, dtype=torch.int32, device="cuda").view(count - 1, shared)
+    assert torch.equal(cache.tables[:-1], want) and torch.equal(cache.tables[-1], torch.arange(shared, dtype=torch.int32, device="cuda"))
+    assert (cache.refs[:shared * count] == 1).all() and (cache.refs[shared * count:] == 0).all()
+    rows = cache.pool[0, :, :shared * count, 0, 0, 0].view(2, count, shared)
+    assert (rows == torch.arange(shared, device="cuda", dtype=torch.bfloat16)).all()
+
+
+def test_temporary_memory_used_on_another_stream_is_not_handed_out():
+    """A cache given up while another stream still works for it leaves its temporary memory alone."""
+    cache = tsac_cuda.PagedCache.empty(1, 600, 4, 1, 8, 300, 4)
+    positions = torch.ones(300, dtype=torch.int32, device="cuda")
+    cache.reserve(positions, slots=1)
+    place, size = cache._scratches[-1][0].data_ptr(), cache._scratches[-1][0].numel()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)
+        cache.release()
+        cache.reserve(positions, slots=1)
+    buffers = cache.pool, cache.tables, cache.counts, cache.lengths, cache.refs  # the caller's
+    del cache
+    again = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(16)]
+    assert not side.query() and all(block.data_ptr() != place for block in again)
+    torch.cuda.synchronize()
+    assert buffers[4].sum().item() == 300
+
+
+def test_binding_refuses_other_dimensions():
+    pair = Pair()
+    with pytest.raises(tsac_cuda.TsacError, match="keys must be"):
+        pair.gpu.append(0, torch.zeros(2, 1, ROW, device="cuda", dtype=torch.bfloat16), torch.zeros(2, 1, ROW, device="cuda", dtype=torch.bfloat16))
+    with pytest.raises(tsac_cuda.TsacError, match="path must be"):
+        pair.gpu.keep(ints([0]), ints([1]))
+    with pytest.raises(tsac_cuda.TsacError, match="positions must be"):
+        pair.gpu.reserve(ints([[1]]))
+    with pytest.raises(tsac_cuda.TsacError, match="parents must be"):
+        pair.gpu.fork(ints([[0]]), ints([[1]]))
+    with pytest.raises(tsac_cuda.TsacError, match="sequences must be"):
+        pair.gpu.release(sequences=ints([[0]]))
+    with pytest.raises(tsac_cuda.TsacError, match="32-bit word"):
+        pair.gpu.release(error_word=torch.zeros(4, dtype=torch.uint8, device="cuda"))
+    pair.check()

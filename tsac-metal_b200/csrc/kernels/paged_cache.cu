@@ -145,11 +145,54 @@ __device__ __forceinline__ bool write_range(const CacheView& c, const int* seque
     return w.last - w.first < slots;
 }
 
+// A shared page is copied for each list entry that writes to it, except for
+// the last of them when no other sequence holds it.  With r table entries on a
+// page and g of them in this call's ranges, that is: all copy when r > g, all
+// but the last when r = g.  Found in time linear in the shared entries by
+// lending the page's own count: g is taken off it, then where nothing is left
+// the lowest -(item + 1) names the last, then the count is put back.
+__device__ void mark_copies(int* refs, const ReserveScratch& s, int shared, int slots, int* needs)
+{
+    const int t = threadIdx.x;
+    const auto copy = [&](int item)
+    {
+        s.flags[item] = 1;
+        atomicAdd(&needs[item / slots], 1);
+    };
+    for (int a = t; a < shared; a += PLAN_THREADS)
+        atomicSub(&refs[s.shared[a].x], 1);
+    __syncthreads();
+    for (int a = t; a < shared; a += PLAN_THREADS)
+    {
+        const int2 mine = s.shared[a];
+        if (__ldcg(&refs[mine.x]) > 0)
+            copy(mine.y);
+        else
+            atomicMin(&refs[mine.x], -(mine.y + 1));
+    }
+    __syncthreads();
+    for (int a = t; a < shared; a += PLAN_THREADS)
+    {
+        const int2 mine = s.shared[a];
+        const int left = __ldcg(&refs[mine.x]);
+        if (left <= 0 && left != -(mine.y + 1))
+            copy(mine.y);
+    }
+    __syncthreads();
+    for (int a = t; a < shared; a += PLAN_THREADS)
+    {
+        const int2 mine = s.shared[a];
+        if (__ldcg(&refs[mine.x]) == -(mine.y + 1))
+            atomicExch(&refs[mine.x], 0);
+    }
+    __syncthreads();
+    for (int a = t; a < shared; a += PLAN_THREADS)
+        atomicAdd(&refs[s.shared[a].x], 1);
+    __syncthreads();
+}
+
 // One CTA plans the whole call.  It is bound by a few dependent round trips to
 // L2 (lengths, tables, reference counts, then the free pages), not by bytes.
-// A shared page is copied for each list entry that writes to it, except for
-// the last when no other sequence holds it: an entry copies when the page's
-// count exceeds one plus the entries before it that hold the same page.
 __global__ void __launch_bounds__(PLAN_THREADS)
     cache_reserve_kernel(CacheView c, const int* sequences, const int* positions, int count,
                          int slots, ReserveScratch s, unsigned* error_word)
@@ -198,23 +241,8 @@ __global__ void __launch_bounds__(PLAN_THREADS)
             raise(error_word, error_cache);
         return;
     }
-    const int together = shared_count;
-    for (int a = t; a < together; a += PLAN_THREADS)
-    {
-        const int2 mine = s.shared[a];
-        int before = 0;
-        for (int b = 0; b < together; ++b)
-        {
-            const int2 other = s.shared[b];
-            before += other.x == mine.x && other.y < mine.y;
-        }
-        if (c.refs[mine.x] - before > 1)
-        {
-            s.flags[mine.y] = 1;
-            atomicAdd(&needs[mine.y / slots], 1);
-        }
-    }
-    __syncthreads();
+    if (shared_count)
+        mark_copies(c.refs, s, shared_count, slots, needs);
     // Exclusive sums of the needs, four consecutive list entries per thread.
     int four[4], sum = 0, total;
 #pragma unroll
@@ -239,24 +267,41 @@ __global__ void __launch_bounds__(PLAN_THREADS)
             raise(error_word, error_pages);
         return;
     }
+    // The pages behind the held ones, one thread per page whichever sequence
+    // takes it: a prompt's thousands must not wait for one thread (one sequence
+    // of 2,048 pages, the whole call: 18 us, by one thread 157 us).
+    for (int k = t; k < total; k += PLAN_THREADS)
+    {
+        int i = 0, behind = count; // the entry whose pages hold the k-th
+        while (behind - i > 1)
+        {
+            const int middle = (i + behind) >> 1;
+            (needs[middle] <= k ? i : behind) = middle;
+        }
+        WriteRange w;
+        write_range(c, sequences, positions, i, slots, w);
+        const int end = i + 1 < count ? needs[i + 1] : total; // the entry's copies come first
+        const int j = w.last - (end - 1 - k);
+        if (j < w.first || j < w.held)
+            continue;
+        const int page = s.free_pages[k];
+        c.refs[page] = 1;
+        c.tables[static_cast<size_t>(w.sequence) * c.max_pages + j] = page;
+    }
+    __syncthreads(); // the counts have been read
     for (int i = t; i < count; i += PLAN_THREADS)
     {
         WriteRange w;
         write_range(c, sequences, positions, i, slots, w);
         int next = needs[i];
         int* table = c.tables + static_cast<size_t>(w.sequence) * c.max_pages;
-        for (int j = w.first; j <= w.last; ++j)
+        for (int j = w.first; j <= w.last && j < w.held; ++j)
         {
-            const bool held = j < w.held;
-            if (held && !s.flags[i * slots + j - w.first])
+            if (!s.flags[i * slots + j - w.first])
                 continue;
-            const int page = s.free_pages[next++];
-            if (held)
-            {
-                const int old = table[j];
-                s.copies[atomicAdd(&copies, 1)] = make_int2(old, page);
-                atomicSub(&c.refs[old], 1);
-            }
+            const int page = s.free_pages[next++], old = table[j];
+            s.copies[atomicAdd(&copies, 1)] = make_int2(old, page);
+            atomicSub(&c.refs[old], 1);
             c.refs[page] = 1;
             table[j] = page;
         }
