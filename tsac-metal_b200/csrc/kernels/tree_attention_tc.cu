@@ -22,8 +22,7 @@
 //                   exponentials overlap the other's products.
 //   warps 9, 10     producers, half of each key or value tile each, into a ring
 //                   of shared-memory slots in the 128-byte swizzle that the MMA
-//                   reads, by TMA: one box per page (or 64 rows) and 64 columns,
-//                   a lane each.  Value tiles with rows behind the last position
+//                   reads, by TMA: one box per page (or 64 rows), a lane each.  Value tiles with rows behind the last position
 //                   come by 16-byte asynchronous copies that make those rows
 //                   zeros, as does everything where TMA does not serve: pages of
 //                   fewer than 8 rows (a swizzle atom), or 2^31 rows in a plane.
@@ -40,6 +39,13 @@
 // small: unrolled over the whole tile it delayed the MMA warp (64 x 16 nodes 172
 // against 162 us), and exponentials of some pairs by a polynomial on the FMA
 // pipes gained nothing over the special function units' 16 per clock.
+//
+// What bounds it now.  128 rows: the loads (64 x 16 nodes 154 us, the same with
+// products and softmax left out).  256 rows: power.  2 x 64 nodes over 131,072
+// positions take 238 us, at 1.6 GHz under the 1,000 W limit, where loads alone
+// take 160, products and loads 168 to 193, softmax and loads 184 to 200; issuing
+// a group's next scores without waiting for its product, or handing P on in two
+// parts, gained 7 to 16 us in those and nothing in the whole.
 //
 // Every wait is bounded (tc_common.cuh).  One that gives up raises
 // error_timeout and the CTA's abort flag; softmax threads then run through
@@ -71,11 +77,18 @@ constexpr int TAINT_SLOTS = 16; // segments that the producers can be ahead of t
 template <int D, bool TWO> struct Tiles
 {
     static constexpr int ROWS = TWO ? 256 : 128;
-    static constexpr int panel_bytes = KEYS * 128;           // 64 columns of 128 rows
-    static constexpr int operand_bytes = panel_bytes * (D / 64);
+    static constexpr int panels = D / 64;
+    static constexpr int operand_bytes = KEYS * 2 * D;
+    static constexpr int panel_bytes = KEYS * 128; // queries: 64 columns of 128 rows
+    static constexpr int group_bytes = 1024 * panels; // keys and values: 8 rows, the panels' atoms side by side
     static constexpr int query_bytes = operand_bytes * (ROWS / 128);
     static constexpr int SLOTS = (TWO ? 160 : 192) * 1024 / operand_bytes;
     static constexpr int chunks = D / 8;
+    // Byte of a 16-byte chunk of a key or value row within its slot.
+    static __device__ __forceinline__ int place(int row, int chunk)
+    {
+        return (row >> 3) * group_bytes + (chunk >> 3) * 1024 + (row & 7) * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+    }
     static constexpr int ring_offset = query_bytes;
     static constexpr int tail_offset = ring_offset + SLOTS * operand_bytes;
     static constexpr int tail_bytes = D == 128 ? 2048 : 4096; // barriers and small arrays
@@ -155,11 +168,12 @@ __device__ __forceinline__ void fence_async_proxy()
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-__device__ __forceinline__ void tma_4d(uint32_t to, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar)
+__device__ __forceinline__ void tma_5d(uint32_t to, const CUtensorMap* map, int c0, int c1, int c2, int c3, int c4,
+                                       uint32_t bar)
 {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-                 " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to),
-                 "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+    asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+                 " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(to),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar)
                  : "memory");
 }
 
@@ -169,13 +183,26 @@ __device__ __forceinline__ void softmax_sync()
     asm volatile("bar.sync 1, %0;" ::"n"(SOFTMAX_THREADS) : "memory");
 }
 
-// MN-major operand, 128-byte swizzle: 64 columns x 8 rows of k per 1024-byte
-// atom; the next 64 columns one panel further, the next 8 rows one atom.
-__device__ __forceinline__ uint64_t value_desc(uint32_t address, uint32_t panel_bytes)
+// Key and value tiles are atoms of 8 rows x 64 columns (1,024 bytes, 128-byte
+// swizzle), the atoms of the same 8 rows side by side, so that one box brings
+// whole rows of a page.  Keys, K-major: the next 8 rows are group_bytes further
+// (the columns' atoms are stepped over by the start address).
+__device__ __forceinline__ uint64_t key_desc(uint32_t address, uint32_t group_bytes)
 {
     uint64_t d = static_cast<uint64_t>((address & 0x3ffffu) >> 4);
-    d |= static_cast<uint64_t>(panel_bytes >> 4) << 16;
-    d |= static_cast<uint64_t>(1024 >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 16;
+    d |= static_cast<uint64_t>(group_bytes >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(2) << 61;
+    return d;
+}
+
+// Values, MN-major: the next 64 columns one atom, the next 8 rows group_bytes further.
+__device__ __forceinline__ uint64_t value_desc(uint32_t address, uint32_t group_bytes)
+{
+    uint64_t d = static_cast<uint64_t>((address & 0x3ffffu) >> 4);
+    d |= static_cast<uint64_t>(1024 >> 4) << 16;
+    d |= static_cast<uint64_t>(group_bytes >> 4) << 32;
     d |= static_cast<uint64_t>(1) << 46;
     d |= static_cast<uint64_t>(2) << 61;
     return d;
@@ -380,8 +407,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     {
         // ------------------------------------------------------------ producers --
         const int first_row = (warp - PRODUCER_WARP) * PRODUCER_ROWS; // this warp's rows of each tile
-        constexpr int rows_at_once = 32 / L::chunks, panels = D / 64;
-        const int boxes = box_rows ? PRODUCER_ROWS / box_rows * panels : 0; // of this warp's half tile
+        constexpr int rows_at_once = 32 / L::chunks;
+        const int boxes = box_rows ? PRODUCER_ROWS / box_rows : 0; // of this warp's half tile
         int slot = 0, round = 0; // uses of the slot so far
         int copied = -1, copied_segment = 0; // a slot whose copies have been issued and not yet announced
         int copied_draft = -1, copied_nodes = 0; // its first drafted row, -1: none; drafted rows
@@ -403,9 +430,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll 2
                 for (int row = max(first_row, copied_draft) + lane / L::chunks; row < end; row += rows_at_once)
                 {
-                    auto* at = reinterpret_cast<uint4*>(smem + L::ring_offset + copied * L::operand_bytes +
-                                                        (chunk >> 3) * L::panel_bytes + row * 128 +
-                                                        (((chunk & 7) ^ (row & 7)) << 4));
+                    auto* at = reinterpret_cast<uint4*>(smem + L::ring_offset + copied * L::operand_bytes + L::place(row, chunk));
                     const uint4 v = *at;
                     const uint32_t odd[4] = {nonfinite_mask<T>(v.x), nonfinite_mask<T>(v.y), nonfinite_mask<T>(v.z),
                                              nonfinite_mask<T>(v.w)};
@@ -436,20 +461,22 @@ __global__ void __launch_bounds__(THREADS, 1)
                 // Scores of keys behind the last are masked whatever they are; values have to be zeros.
                 const bool boxed = boxes && (!value || !Work::is_masked(g, tile));
                 // The tile's table entries are on their way while the slot is awaited.
-                int row_of_pool = 0;
+                int eight_rows = 0; // of the layer's two planes, in units of 8
                 long long low_rows = -1, high_rows = -1;
                 if (boxed)
                 {
                     if (lane < boxes)
                     {
-                        const int position = Work::base(g, tile) + first_row + lane / panels * box_rows;
+                        const int position = Work::base(g, tile) + first_row + lane * box_rows;
                         const int page = position < Work::limit(g, tile)
                                              ? cache_page(a.cache, g.e.sequence, g.e.held, position >> a.cache.page_shift)
                                              : -1;
                         if (page < 0 && position < Work::limit(g, tile) && a.error_word)
                             atomicOr(a.error_word, error_cache);
-                        row_of_pool = page < 0 ? a.cache.pages << a.cache.page_shift // outside: zeros
-                                               : (page << a.cache.page_shift) + (position & (a.cache.page_size() - 1));
+                        const int plane_groups = a.cache.pages << a.cache.page_shift >> 3;
+                        eight_rows = page < 0 ? 2 * plane_groups // outside: zeros
+                                              : (value ? plane_groups : 0) +
+                                                    ((page << a.cache.page_shift) + (position & (a.cache.page_size() - 1)) >> 3);
                     }
                 }
                 else
@@ -467,25 +494,20 @@ __global__ void __launch_bounds__(THREADS, 1)
                         bar_expect_tx(bar, L::operand_bytes / 2);
                     __syncwarp();
                     if (lane < boxes)
-                    {
-                        const int box = lane / panels, panel = lane - box * panels;
-                        tma_4d(base + panel * L::panel_bytes + (first_row + box * box_rows) * 128, &map, panel * 64,
-                               g.head, row_of_pool, value, bar);
-                    }
+                        tma_5d(base + (first_row + lane * box_rows >> 3) * L::group_bytes, &map, 0, 0, 0, g.head, eight_rows, bar);
                     announce(false);
                 }
                 else
                 {
                     const unsigned char* from = plane + (value ? a.cache.plane_bytes : 0);
                     const int chunk = lane % L::chunks;
-                    const uint32_t column = base + (chunk >> 3) * L::panel_bytes;
 #pragma unroll 8
                     for (int i = 0; i < PRODUCER_ROWS / rows_at_once; ++i)
                     {
                         const int row = i * rows_at_once + lane / L::chunks;
                         const long long offset =
                             __shfl_sync(0xffffffffu, i * rows_at_once < 32 ? low_rows : high_rows, row & 31);
-                        copy_16(column + (first_row + row) * 128 + (((chunk & 7) ^ (row & 7)) << 4),
+                        copy_16(base + L::place(first_row + row, chunk),
                                 from + (offset >= 0 ? offset + 16 * chunk : 0), offset >= 0 ? 16u : 0u);
                     }
                     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -602,14 +624,14 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (!ok)
                 return;
             const uint64_t q = sw128_desc(query + (TWO ? group * L::operand_bytes : 0));
-            const uint64_t k = sw128_desc(ring + s * L::operand_bytes);
+            const uint64_t k = key_desc(ring + s * L::operand_bytes, L::group_bytes);
             tc_fence_after();
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk)
             {
                 constexpr int unit = 16; // of a descriptor's address
-                const int at = ((kk >> 2) * L::panel_bytes + (kk & 3) * 32) / unit;
-                mma_shared(leader, tm + group * KEYS, q + at, k + at, score_idesc, kk != 0);
+                mma_shared(leader, tm + group * KEYS, q + ((kk >> 2) * L::panel_bytes + (kk & 3) * 32) / unit,
+                           k + ((kk >> 2) * 1024 + (kk & 3) * 32) / unit, score_idesc, kk != 0);
             }
             commit_if(leader, smem_u32(&tail.scores[group]));
             any = true;
@@ -618,11 +640,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         {
             if (!ok || !wait_all(tail.weights[group], made(group)))
                 return;
-            const uint64_t v = value_desc(ring + s * L::operand_bytes, L::panel_bytes);
+            const uint64_t v = value_desc(ring + s * L::operand_bytes, L::group_bytes);
             tc_fence_after();
 #pragma unroll
             for (int kk = 0; kk < KEYS / 16; ++kk)
-                mma_tmem(leader, tm + OUTPUT_COLUMN + group * 128, tm + group * KEYS + 8 * kk, v + kk * 2048 / 16,
+                mma_tmem(leader, tm + OUTPUT_COLUMN + group * 128, tm + group * KEYS + 8 * kk, v + kk * 2 * L::group_bytes / 16,
                          value_idesc, accumulate || kk != 0);
             commit_if(leader, smem_u32(&tail.products[group]));
             made.add(group, 1);
@@ -962,21 +984,23 @@ __global__ void __launch_bounds__(THREADS, 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLUMNS));
 }
 
-// The layer's two planes as [keys, values][row][head][column], in boxes of
-// `rows` rows of one head and 64 columns.
+// The layer's two planes as [8 rows][head][64 columns][row of 8][column], in
+// boxes of `rows` whole rows of one head.  A box per 64 columns is twice as many:
+// 64 x 16 nodes over pages of 16 took 159 us with them, 154 us with these.
 bool make_map(CUtensorMap* map, const TreeArgs& a, int rows)
 {
     const auto fn = encode_fn();
     const CacheView& c = a.cache;
     const cuuint64_t plane_rows = static_cast<cuuint64_t>(c.pages) << c.page_shift;
-    if (!fn || plane_rows >= 0x7fffffffull || c.plane_bytes >= 1ll << 40)
+    if (!fn || plane_rows >= 0x7fffffffull)
         return false;
-    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(a.heads), plane_rows, 2};
-    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(2 * a.head_dim), static_cast<cuuint64_t>(c.row_bytes),
-                                   static_cast<cuuint64_t>(c.plane_bytes)};
-    const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(rows), 1};
-    const cuuint32_t elem[4] = {1, 1, 1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, c.pool + 2ll * a.layer * c.plane_bytes, dims, strides, box, elem,
+    const cuuint64_t panels = static_cast<cuuint64_t>(a.head_dim / 64);
+    const cuuint64_t dims[5] = {64, 8, panels, static_cast<cuuint64_t>(a.heads), 2 * plane_rows / 8};
+    const cuuint64_t strides[4] = {static_cast<cuuint64_t>(c.row_bytes), 128, static_cast<cuuint64_t>(2 * a.head_dim),
+                                   8 * static_cast<cuuint64_t>(c.row_bytes)};
+    const cuuint32_t box[5] = {64, 8, static_cast<cuuint32_t>(panels), 1, static_cast<cuuint32_t>(rows / 8)};
+    const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, c.pool + 2ll * a.layer * c.plane_bytes, dims, strides, box, elem,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
