@@ -415,6 +415,9 @@ class PagedCache:
         return out
 
 
+_verify_types = {}
+
+
 def draft_verify(target, tokens, parents, coins, draws, draft=None, nodes=None, out=None, error_word=None):
     """Checks trees of drafted tokens against the target's probabilities (tsac_cuda_draft_verify).
 
@@ -422,33 +425,38 @@ def draft_verify(target, tokens, parents, coins, draws, draft=None, nodes=None, 
     int32 [batch][nodes], coins f32 [batch][nodes], draws f32 [batch] in [0, 1).
     Returns (accepted [batch], path [batch][nodes], token [batch]), int32, in
     `out` when given."""
-    import torch
     lib = _drafting()
+    if not _verify_types:
+        import torch
+        _verify_types.update({torch.bfloat16: 0, torch.float16: 1, torch.float32: 2, "ints": torch.int32})
     if target.dim() != 3 or not target.is_cuda:
         raise TsacError("target must be a CUDA tensor [batch][nodes][vocab]")
-    types = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
     shape = target.shape
     batch, most, vocab = shape
-    index, kind = target.get_device(), target.dtype
-    for name, t in (("target", target), ("draft", draft)):
-        if t is not None and (kind not in types or t.dtype is not kind or t.get_device() != index or t.shape != shape
-                              or (vocab > 1 and t.stride(2) != 1)):
-            raise TsacError(f"{name} must be bf16, fp16 or fp32 [batch][nodes][vocab], the vocabulary contiguous")
-    ints, floats, rows, ones = torch.int32, torch.float32, (batch, most), (batch,)
+    index, kind, ints, floats = target.get_device(), target.dtype, _verify_types["ints"], draws.dtype
+    strides = target.stride()
+    if kind not in _verify_types or (strides[2] != 1 and vocab > 1):
+        raise TsacError("target must be bf16, fp16 or fp32 [batch][nodes][vocab], the vocabulary contiguous")
+    if draft is not None and (draft.dtype is not kind or draft.get_device() != index or draft.shape != shape
+                              or (draft.stride(2) != 1 and vocab > 1)):
+        raise TsacError("draft must be of the target's type and shape, the vocabulary contiguous")
+    if _verify_types.get(floats) != 2:
+        raise TsacError("draws must be float32")
+    rows, ones = (batch, most), (batch,)
+    q, q_strides = (None, None) if draft is None else (draft.data_ptr(), _strides(draft.stride()[:2]))
+    tokens_at, parents_at = _whole(tokens, "tokens", ints, index, rows), _whole(parents, "parents", ints, index, rows)
     if out is None:
-        accepted, path, token = draws.new_empty(batch, dtype=ints), parents.new_empty(rows), draws.new_empty(batch, dtype=ints)
+        accepted, path, token = tokens.new_empty(batch), tokens.new_empty(rows), tokens.new_empty(batch)
         places = accepted.data_ptr(), path.data_ptr(), token.data_ptr()
     else:
         accepted, path, token = out
         places = (_whole(accepted, "accepted", ints, index, ones), _whole(path, "path", ints, index, rows),
                   _whole(token, "token", ints, index, ones))
-    word = None if error_word is None else _error_word(error_word, index)
     on = _Device.of(index)
-    on.call(lib.tsac_cuda_draft_verify, target.data_ptr(), _strides(target.stride()[:2]),
-            None if draft is None else draft.data_ptr(), None if draft is None else _strides(draft.stride()[:2]), types[kind],
-            _whole(tokens, "tokens", ints, index, rows), _whole(parents, "parents", ints, index, rows),
-            _whole(coins, "coins", floats, index, rows), _whole(draws, "draws", floats, index, ones),
-            _whole(nodes, "nodes", ints, index, ones), batch, most, vocab, *places, word, on.stream())
+    on.call(lib.tsac_cuda_draft_verify, target.data_ptr(), _strides(strides[:2]), q, q_strides, _verify_types[kind],
+            tokens_at, parents_at, _whole(coins, "coins", floats, index, rows), _whole(draws, "draws", floats, index, ones),
+            None if nodes is None else _whole(nodes, "nodes", ints, index, ones), batch, most, vocab, *places,
+            None if error_word is None else _error_word(error_word, index), on.stream())
     return accepted, path, token
 
 
