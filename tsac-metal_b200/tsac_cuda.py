@@ -276,7 +276,7 @@ class PagedCache:
             raise TsacError("pool must be a bf16 or fp16 CUDA tensor [layers][2][pages][page_size][kv_heads][head_dim]")
         self.pool, self.tables, self.counts, self.lengths, self.refs = pool, tables, counts, lengths, refs
         self.device, self.index, self.dtype = pool.device, pool.get_device(), pool.dtype
-        self._torch, self._int = torch, torch.int32
+        self._torch, self._int, self._bytes = torch, torch.int32, torch.empty(0, dtype=torch.uint8, device=self.device)
         if tables.dim() != 2:
             raise TsacError("tables must be [sequences][max_pages]")
         self.layers, _, self.pages, self.page_size, self.kv_heads, self.head_dim = pool.shape
@@ -292,7 +292,7 @@ class PagedCache:
         s.type = 0 if pool.dtype == torch.bfloat16 else 1
         self._struct, self._lib, self._on = s, _drafting(), _Device.of(self.index)
         self._cache = ctypes.addressof(s)
-        self._scratches = []
+        self._scratches, self._attention_bytes = [], {}
 
     @classmethod
     def empty(cls, layers, pages, page_size, kv_heads, head_dim, sequences, max_pages, dtype=None, device="cuda"):
@@ -310,7 +310,7 @@ class PagedCache:
         return _error_word(error_word, self.index)
 
     def _temporary(self, nbytes):
-        return self._torch.empty(max(nbytes, 16), dtype=self._torch.uint8, device=self.device)
+        return self._bytes.new_empty(max(nbytes, 16))
 
     def _kept(self, nbytes):
         """Temporary memory of the calls that change the cache, which must not overlap: kept from one to the next.
@@ -397,21 +397,25 @@ class PagedCache:
     def attention(self, layer, query, parents, out=None, nodes=None, sequences=None, scale=None, lse=None,
                   error_word=None):
         """Attention of each tree's nodes over the cache: query [entry][node][heads][head_dim] -> out."""
-        torch = self._torch
         if query.dim() != 4:
             raise TsacError("query must be [entry][node][heads][head_dim]")
         count, most, heads, _ = query.shape
-        shape = (count, most, heads, self.head_dim)
-        out = torch.empty(shape, dtype=self.dtype, device=self.device) if out is None else out
-        q, query_strides = _rows(query, "query", self.dtype, self.index, shape)
-        o, out_strides = _rows(out, "out", self.dtype, self.index, shape)
-        scratch = self._temporary(self._lib.tsac_cuda_tree_attention_scratch_bytes(self._cache, heads, most))
-        self._on.call(self._lib.tsac_cuda_tree_attention, self._cache, layer, self._list(sequences, count),
-                      _whole(parents, "parents", self._int, self.index, (count, most)),
-                      _whole(nodes, "nodes", self._int, self.index, (count,)), q, query_strides, o, out_strides,
-                      _whole(lse, "lse", torch.float32, self.index, (count, most, heads)), heads, count, most,
-                      self.head_dim ** -0.5 if scale is None else scale, scratch.data_ptr(), scratch.numel(),
-                      self._word(error_word), self._on.stream())
+        shape, index, ints, on = (count, most, heads, self.head_dim), self.index, self._int, self._on
+        out = query.new_empty(shape) if out is None else out
+        q, query_strides = _rows(query, "query", self.dtype, index, shape)
+        o, out_strides = _rows(out, "out", self.dtype, index, shape)
+        nbytes = self._attention_bytes.get((heads, most))
+        if nbytes is None:
+            nbytes = self._lib.tsac_cuda_tree_attention_scratch_bytes(self._cache, heads, most)
+            self._attention_bytes[heads, most] = nbytes
+        scratch = self._temporary(nbytes)
+        on.call(self._lib.tsac_cuda_tree_attention, self._cache, layer,
+                None if sequences is None else _whole(sequences, "sequences", ints, index, (count,)),
+                _whole(parents, "parents", ints, index, (count, most)),
+                None if nodes is None else _whole(nodes, "nodes", ints, index, (count,)), q, query_strides, o, out_strides,
+                None if lse is None else _whole(lse, "lse", self._torch.float32, index, (count, most, heads)), heads, count,
+                most, self.head_dim ** -0.5 if scale is None else scale, scratch.data_ptr(), nbytes,
+                None if error_word is None else _error_word(error_word, index), on.stream())
         return out
 
 
