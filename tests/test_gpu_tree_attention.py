@@ -399,3 +399,31 @@ def test_queries_that_are_not_finite_stay_in_their_rows(kind, dim, group, nodes,
         assert not torch.isfinite(out[b, n, h]).any()
         out[b, n, h], lse[b, n, h] = clean[b, n, h], clean_lse[b, n, h]
     s.check(out, lse)
+
+
+@pytest.mark.parametrize("dim,group,nodes", [(128, 1, 20), (64, 5, 40)])
+def test_positions_past_two_gigabytes_for_many_rows(dim, group, nodes):
+    """The same for the kernel of many rows, in the second of two layers: planes of more than 4 GiB."""
+    heads = 32768 // dim
+    cache = tsac_cuda.PagedCache.empty(2, 70, 1024, heads, dim, 2, 66, dtype=torch.float16)  # 64 MiB a page
+    torch.manual_seed(1)
+    used = [69, 3, 68]
+    cache.tables[1, :3] = ints(used)
+    cache.counts[1] = 3
+    cache.refs[used] = 1
+    length = 2050 - nodes
+    cache.lengths[1] = length
+    for page in used:
+        cache.pool[1, :, page].normal_()
+    parents = ints([[-1] + [n // 2 for n in range(nodes - 1)]])
+    query = torch.randn(1, nodes, heads * group, dim, device="cuda").to(torch.float16)
+    errors = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = cache.attention(1, query, parents, sequences=ints([1]), error_word=errors)
+    assert errors.item() == 0
+    keys, values = (cache.pool[1, i][used].flatten(0, 1)[:length + nodes] for i in (0, 1))
+    for head in (0, heads - 1):
+        mine = slice(head * group, (head + 1) * group)
+        want, _, size = drafting.attention(query[0, :, mine].cpu().double(), keys[:, head:head + 1].cpu().double(),
+                                           values[:, head:head + 1].cpu().double(), length, parents[0].tolist(), nodes, group, dim ** -0.5)
+        # h (A + |out|) plus a thousandth of A for the 32-bit parts and subnormals, as in Setup.check.
+        assert ((out[0, :, mine].cpu().double() - want).abs() <= 2.0 ** -11 * (size + want.abs()) + 1e-3 * size).all()
