@@ -200,3 +200,10 @@ def test_verification_leaves_the_target_distribution(with_draft):
                         got[first] += weight / grid ** 3
     # Each of three stages is off by at most one grid cell of its mass.
     assert np.abs(got - p).max() <= 3 / grid / 2 + 1e-12
+
+
+@pytest.mark.parametrize("scale", [3e38, -2.5e38])
+def test_scales_that_overflow_in_powers_of_two_are_refused(scale):
+    lib, c, s3 = tsac_cuda._drafting(), cache(), strides(1024, 512, 128)
+    refused(lib.tsac_cuda_tree_attention(ctypes.addressof(c), 0, None, FAKE, None, FAKE, s3, FAKE, s3, None, 4, 1, 1, scale,
+                                         FAKE, 1 << 40, None, None), "scale")

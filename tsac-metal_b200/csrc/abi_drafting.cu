@@ -248,7 +248,8 @@ int tsac_cuda_tree_attention(const tsac_cuda_paged_cache* cache, size_t layer, c
             require(heads >= 1 && heads <= 65536 && heads % cache->kv_heads == 0,
                     "query heads must be a multiple of the key heads");
             require(max_nodes >= 1 && max_nodes <= TSAC_CUDA_MAX_NODES, "tree node count out of range");
-            require(std::isfinite(scale), "softmax scale must be finite");
+            const float scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+            require(std::isfinite(scale_log2), "softmax scale must be finite, times log2(e) too");
             require_strides(query_strides, "query strides must be multiples of 8 elements");
             require_strides(out_strides, "output strides must be multiples of 8 elements");
             require(aligned16(query) && aligned16(out), "query and output must be 16-byte aligned");
@@ -278,7 +279,7 @@ int tsac_cuda_tree_attention(const tsac_cuda_paged_cache* cache, size_t layer, c
             a.lse = lse;
             a.count = static_cast<int>(count);
             a.max_nodes = static_cast<int>(max_nodes);
-            a.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+            a.scale_log2 = scale_log2;
             a.error_word = error_word;
             cuda_check(dev::tree_attention(a, static_cast<dev::ValueType>(cache->type), scratch,
                                            static_cast<cudaStream_t>(stream)),
