@@ -431,11 +431,17 @@ def codec_workload(args, rank, world, torch, dist):
 # ScalarAnalyzer::encode/decode build inside every call) before timing, so the
 # timed region holds coding only.
 _REF = {}
+_REF_LIBRARY = ROOT / "oracle" / "_ref" / "libtsac_ref.so"
+
+
+def _reference_missing():
+    """Why the reference path cannot be timed, or None.  (A pool whose workers cannot start never ends.)"""
+    return None if _REF_LIBRARY.exists() else f"{_REF_LIBRARY.relative_to(ROOT)} is not built (it needs the reference's sources)"
 
 
 def _reference_worker_init():
     import tsac_cuda
-    lib = ctypes.CDLL(str(ROOT / "oracle" / "_ref" / "libtsac_ref.so"))
+    lib = ctypes.CDLL(str(_REF_LIBRARY))
     lib.ref_last_error.restype = ctypes.c_char_p
     handle = ctypes.c_void_p()
     if lib.ref_session_create(str(tsac_cuda.seeded_package(0)).encode(), 2, 12, ctypes.byref(handle)) != 0:
@@ -733,7 +739,9 @@ def main():
               "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
               "data": "synthetic (seeded music-like PCM; seeded random-init weights)"}
     if args.impl == "reference":
-        if rank == 0:
+        if rank == 0 and _reference_missing():
+            print(json.dumps({"impl": "reference", "unavailable": _reference_missing()}), flush=True)
+        elif rank == 0:
             steps_run = max(1, min(args.steps, 2))
             cpu = codec_cpu(steps_run, REFERENCE_ARM_SECONDS)
             line = {"impl": "reference",
@@ -772,8 +780,9 @@ def main():
         result = qlinear_workload(args, rank, world, torch, dist)
     if rank == 0:
         if world == 1 and not args.no_cpu_baseline:
-            result["cpu_baseline"] = (codec_cpu(1, BASELINE_SAMPLE_SECONDS)
-                                      if args.workload == "codec" else None)
+            missing = _reference_missing()
+            result["cpu_baseline"] = (None if args.workload != "codec" else {"unavailable": missing} if missing
+                                      else codec_cpu(1, BASELINE_SAMPLE_SECONDS))
         line = {"metric": result.pop("metric"), "value": result.pop("value"),
                 "unit": result.pop("unit"), **common, **result}
         line["config"]["parallelism"] = (f"clip sharding over {world} GPU(s); no collective in the "
