@@ -522,7 +522,9 @@ int tsac_cuda_cache_keep(const tsac_cuda_paged_cache* cache, const int32_t* sequ
  * with L pages in use, the k-th used page from L on moves to the k-th free
  * page below L.  tables_out [sequences][max_pages] and refs_out [pages] may be
  * the cache's own; *live (device) receives L, so a caller may keep only the
- * pool's first L pages of each plane.  Pages that moved keep their old bytes. */
+ * pool's first L pages of each plane.  Pages that moved keep their old bytes.
+ * A negative count (it becomes 0) and a held table entry whose page is none or
+ * has no positive count (it becomes -1) are reported by bit 16. */
 size_t tsac_cuda_cache_compact_scratch_bytes(size_t pages);
 int tsac_cuda_cache_compact(const tsac_cuda_paged_cache* cache, int32_t* tables_out, int32_t* refs_out,
                             int32_t* live, void* scratch, size_t scratch_bytes,

@@ -534,3 +534,37 @@ def test_binding_refuses_other_dimensions():
     with pytest.raises(tsac_cuda.TsacError, match="32-bit word"):
         pair.gpu.release(error_word=torch.zeros(4, dtype=torch.uint8, device="cuda"))
     pair.check()
+
+
+@pytest.mark.parametrize("pages,in_place", [(64, False), (64, True), (1500, True), (40000, False)])
+def test_compaction_of_inconsistent_counts(pages, in_place):
+    """Negative counts and entries of pages without a count: reported, and never more moves than holes."""
+    rng = random.Random(pages)
+    cache = tsac_cuda.PagedCache.empty(1, pages, 2, 1, 8, 3, pages // 4)
+    refs = torch.tensor([rng.choice((-3, -1, 0, 0, 1, 2)) for _ in range(pages)], dtype=torch.int32)
+    refs[-1], refs[0] = 5, -1
+    live = [p for p in range(pages) if refs[p] > 0]
+    count = len(live)
+    cache.refs.copy_(refs)
+    cache.pool.copy_(torch.randn(cache.pool.shape))
+    pool = cache.pool.clone()
+    named = live[:pages // 8] + live[-pages // 16:] + [p for p in range(pages) if refs[p] <= 0][:pages // 16]
+    rng.shuffle(named)
+    cache.tables[1, :len(named)] = ints(named)
+    cache.counts[1] = len(named)
+    tables_out, refs_out = (cache.tables, cache.refs) if in_place else (torch.empty_like(cache.tables), torch.empty_like(cache.refs))
+    word = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert cache.compact(tables_out=tables_out, refs_out=refs_out, error_word=word).item() == count
+    assert word.item() == 16
+    holes = [p for p in range(count) if refs[p] <= 0]
+    moved = [p for p in live if p >= count]
+    assert len(holes) == len(moved)
+    to = {p: p for p in live} | dict(zip(moved, holes))
+    want = torch.zeros(pages, dtype=torch.int32)
+    want[[to[p] for p in live]] = refs[live]
+    assert torch.equal(refs_out.cpu(), want)
+    assert tables_out[1, :len(named)].tolist() == [to.get(p, -1) for p in named]
+    assert (tables_out[[0, 2]] == -1).all() and (tables_out[1, len(named):] == -1).all()
+    expected = pool.clone()
+    expected[:, :, holes] = pool[:, :, moved]
+    assert torch.equal(cache.pool, expected)

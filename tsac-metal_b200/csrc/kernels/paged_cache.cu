@@ -61,12 +61,12 @@ __device__ __forceinline__ int block_exclusive(int value, int* warp_sums, int& t
 }
 
 // Writes the lowest `limit` pages of [begin, end) whose reference count
-// passes `free_pages` (zero) or not (positive) to out, ascending; returns how
-// many there are (at most limit).  One pass of the block covers up to 32,768
-// pages: each warp owns a contiguous run, reads it coalesced with all loads in
-// flight, keeps one ballot per 32 pages (lane k the k-th), and the block scans
-// the warps' totals once.
-template <bool FREE> __device__ int select_pages(const int* refs, int begin, int end, int limit, int* out, int* warp_sums)
+// passes `test` to out, ascending; returns how many there are (at most limit).
+// One pass of the block covers up to 32,768 pages: each warp owns a contiguous
+// run, reads it coalesced with all loads in flight, keeps one ballot per 32
+// pages (lane k the k-th), and the block scans the warps' totals once.
+template <class Test>
+__device__ int select_pages(const int* refs, int begin, int end, int limit, int* out, int* warp_sums, Test test)
 {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int found = 0;
@@ -80,7 +80,7 @@ template <bool FREE> __device__ int select_pages(const int* refs, int begin, int
         for (int k = 0; k < groups; ++k)
         {
             const int page = first + k * 32 + lane;
-            const bool hit = page < end && (FREE ? refs[page] == 0 : refs[page] > 0);
+            const bool hit = page < end && test(refs[page]);
             const unsigned mask = __ballot_sync(0xffffffffu, hit);
             if (lane == k)
                 mine = mask;
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(PLAN_THREADS)
     }
     if (total == 0)
         return;
-    if (select_pages<true>(c.refs, 0, c.pages, total, s.free_pages, warp_sums) < total)
+    if (select_pages(c.refs, 0, c.pages, total, s.free_pages, warp_sums, [](int refs) { return refs == 0; }) < total)
     {
         if (t == 0)
             raise(error_word, error_pages);
@@ -637,7 +637,7 @@ struct CompactScratch
 {
     int* copies_count;
     int2* copies;  // (from, to)
-    int* map;      // [pages] a page's place after the call
+    int* map;      // [pages] a page's place after the call, -1: not in use
     int* selected; // [2][pages] live pages above the live count; holes below it
 };
 
@@ -653,9 +653,11 @@ CompactScratch compact_layout(void* scratch, size_t pages)
 }
 
 // With L pages live, the k-th live page at or above L moves into the k-th
-// hole below L: the fewest moves that leave the live pages at [0, L).
+// hole below L: the fewest moves that leave the live pages at [0, L).  Live is
+// a positive count and a hole anything else, so that there is a hole for every
+// move whatever the counts are; a negative one is reported and becomes 0.
 __global__ void __launch_bounds__(PLAN_THREADS)
-    cache_compact_plan_kernel(CacheView c, int* refs_out, int* live_out, CompactScratch s)
+    cache_compact_plan_kernel(CacheView c, int* refs_out, int* live_out, CompactScratch s, unsigned* error_word)
 {
     pdl_prologue();
     __shared__ int warp_sums[32];
@@ -665,13 +667,15 @@ __global__ void __launch_bounds__(PLAN_THREADS)
     for (int page = t; page < c.pages; page += PLAN_THREADS)
         mine += c.refs[page] > 0;
     block_exclusive(mine, warp_sums, live);
-    const int moves = select_pages<false>(c.refs, live, c.pages, c.pages, s.selected, warp_sums);
-    select_pages<true>(c.refs, 0, live, c.pages, s.selected + c.pages, warp_sums);
+    const int moves = select_pages(c.refs, live, c.pages, c.pages, s.selected, warp_sums, [](int refs) { return refs > 0; });
+    select_pages(c.refs, 0, live, c.pages, s.selected + c.pages, warp_sums, [](int refs) { return refs <= 0; });
     for (int page = t; page < c.pages; page += PLAN_THREADS)
     {
-        s.map[page] = page;
-        if (refs_out != c.refs)
-            refs_out[page] = c.refs[page];
+        const int refs = c.refs[page];
+        s.map[page] = refs > 0 ? page : -1;
+        if (refs < 0)
+            raise(error_word, error_cache);
+        refs_out[page] = refs > 0 ? refs : 0;
     }
     __syncthreads();
     for (int k = t; k < moves; k += PLAN_THREADS)
@@ -702,9 +706,10 @@ __global__ void __launch_bounds__(COPY_THREADS)
         const int sequence = static_cast<int>(at / c.max_pages), entry = static_cast<int>(at - static_cast<long long>(sequence) * c.max_pages);
         const int held = cache_held(c, sequence);
         const int page = cache_page(c, sequence, held, entry);
-        if (page < 0 && entry < held)
+        const int place = page < 0 ? -1 : s.map[page];
+        if (place < 0 && entry < held)
             raise(error_word, error_cache);
-        tables_out[at] = page < 0 ? -1 : s.map[page];
+        tables_out[at] = place;
     }
     copy_pages(c, s.copies, *s.copies_count);
 }
@@ -784,7 +789,7 @@ void cache_compact(const CacheView& c, int* tables_out, int* refs_out, int* live
                    unsigned* error_word, cudaStream_t stream)
 {
     const CompactScratch s = compact_layout(scratch, static_cast<size_t>(c.pages));
-    launch_pdl(cache_compact_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, stream, c, refs_out, live, s);
+    launch_pdl(cache_compact_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, stream, c, refs_out, live, s, error_word);
     note_launch();
     launch_pdl(cache_compact_kernel, dim3(copy_grid()), dim3(COPY_THREADS), 0, stream, c, tables_out, s, error_word);
     note_launch();
