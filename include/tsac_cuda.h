@@ -470,7 +470,8 @@ typedef struct tsac_cuda_paged_cache
  *              (max_pages always suffices)
  *   scratch    device, >= tsac_cuda_cache_reserve_scratch_bytes(count, slots), 16-byte aligned
  * All or nothing: too few free pages change nothing and OR 8 into
- * *error_word; an invalid entry (bit 16) changes nothing either. */
+ * *error_word; an invalid entry, or a held page in its range that has no
+ * positive count (bit 16), changes nothing either. */
 size_t tsac_cuda_cache_reserve_scratch_bytes(size_t count, size_t slots);
 int tsac_cuda_cache_reserve(const tsac_cuda_paged_cache* cache, const int32_t* sequences,
                             const int32_t* positions, size_t count, size_t slots, void* scratch,
@@ -478,14 +479,15 @@ int tsac_cuda_cache_reserve(const tsac_cuda_paged_cache* cache, const int32_t* s
 
 /* children[i], which must hold no page, becomes a copy of parents[i] that
  * shares the pages of its committed positions (device int32 [count] each).
- * A pair is refused (bit 16) when an earlier one names its child, or when its
- * parent is some pair's child. */
+ * A pair is refused (bit 16) when an earlier one names its child, when its
+ * parent is some pair's child, or when a page to share has no positive count. */
 int tsac_cuda_cache_fork(const tsac_cuda_paged_cache* cache, const int32_t* parents,
                          const int32_t* children, size_t count, unsigned* error_word, void* stream);
 
 /* Gives back the pages behind position positions[i] of each listed sequence
  * (positions NULL: all pages), and shortens its length to that if it is
- * longer.  A page becomes free when its last sequence gives it back. */
+ * longer.  A page becomes free when its last sequence gives it back.  The count
+ * of a page that has none left to give back stays as it was (bit 16). */
 int tsac_cuda_cache_release(const tsac_cuda_paged_cache* cache, const int32_t* sequences,
                             const int32_t* positions, size_t count, unsigned* error_word, void* stream);
 

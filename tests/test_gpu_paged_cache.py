@@ -568,3 +568,36 @@ def test_compaction_of_inconsistent_counts(pages, in_place):
     expected = pool.clone()
     expected[:, :, holes] = pool[:, :, moved]
     assert torch.equal(cache.pool, expected)
+
+
+def test_counts_below_the_entries_that_name_a_page():
+    """Tables and counts that a caller built wrongly: reported, and no count falls below zero."""
+    pair = Pair(pages=12, page_size=8, sequences=5, max_pages=4)
+    pair.grow([(0, 20), (1, 9)])
+    cache, errors = pair.gpu, pair.errors
+
+    def word():
+        value = errors.item()
+        errors.zero_()
+        return value
+
+    # Sequence 2 names the pages of sequence 0 (0, 1, 2) without being counted.
+    cache.tables[2], cache.counts[2], cache.lengths[2] = cache.tables[0].clone(), 3, 20
+    cache.release(sequences=ints([0]), error_word=errors)
+    assert word() == 0 and cache.refs.tolist()[:5] == [0, 0, 0, 1, 1]
+    state = _state(cache)
+    cache.reserve(ints([1, 3]), sequences=ints([3, 2]), error_word=errors)
+    assert word() == 16 and _same(cache, state)
+    cache.fork(ints([2]), ints([4]), error_word=errors)
+    assert word() == 16 and _same(cache, state)
+    cache.release(sequences=ints([2, 1]), error_word=errors)
+    assert word() == 16 and cache.refs.tolist() == [0] * 12 and cache.counts.tolist() == [0] * 5
+    assert (cache.tables == -1).all() and cache.lengths.tolist() == [0] * 5
+    # Many holders of one page with a count of two, and a count that is negative already.
+    cache = tsac_cuda.PagedCache.empty(1, 3, 4, 1, 8, 4096, 2)
+    cache.tables[:, 0], cache.tables[:, 1] = 1, 2
+    cache.counts.fill_(2)
+    cache.lengths.fill_(8)
+    cache.refs.copy_(ints([0, 2, -7]))
+    cache.release(error_word=errors)
+    assert word() == 16 and cache.refs.tolist() == [0, 0, -7] and cache.counts.sum().item() == 0

@@ -225,9 +225,10 @@ __global__ void __launch_bounds__(PLAN_THREADS)
         {
             const int item = i * slots + j - w.first;
             const int page = cache_page(c, w.sequence, w.held, j);
-            if (page < 0)
+            const int refs = page < 0 ? 0 : c.refs[page];
+            if (refs < 1)
                 bad = 1;
-            else if (c.refs[page] > 1)
+            else if (refs > 1)
                 s.shared[atomicAdd(&shared_count, 1)] = make_int2(page, item);
             s.flags[item] = 0;
         }
@@ -383,7 +384,10 @@ __global__ void __launch_bounds__(256)
     {
         bool broken = false;
         for (int j = threadIdx.x; j < share; j += 256)
-            broken |= cache_page(c, parent, share, j) < 0;
+        {
+            const int page = cache_page(c, parent, share, j);
+            broken |= page < 0 || c.refs[page] < 1; // counts only rise in this launch, from 1 at least
+        }
         bad = __syncthreads_or(broken);
     }
     if (bad)
@@ -432,10 +436,15 @@ __global__ void __launch_bounds__(256)
     for (int j = stay + threadIdx.x; j < held; j += 256)
     {
         const int page = table[j];
-        if (static_cast<unsigned>(page) < static_cast<unsigned>(c.pages))
-            atomicSub(&c.refs[page], 1);
-        else
+        if (static_cast<unsigned>(page) >= static_cast<unsigned>(c.pages))
+        {
             broken = true;
+        }
+        else if (atomicSub(&c.refs[page], 1) < 1)
+        {
+            atomicAdd(&c.refs[page], 1); // more entries than the count says: it stays as it was
+            broken = true;
+        }
         table[j] = -1;
     }
     if (broken)
