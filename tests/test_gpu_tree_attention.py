@@ -427,3 +427,27 @@ def test_positions_past_two_gigabytes_for_many_rows(dim, group, nodes):
                                            values[:, head:head + 1].cpu().double(), length, parents[0].tolist(), nodes, group, dim ** -0.5)
         # h (A + |out|) plus a thousandth of A for the 32-bit parts and subnormals, as in Setup.check.
         assert ((out[0, :, mine].cpu().double() - want).abs() <= 2.0 ** -11 * (size + want.abs()) + 1e-3 * size).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group,nodes", [(1, 24), (4, 33), (16, 20)])
+@pytest.mark.parametrize("length", [1, 61, 63, 126, 131, 382])
+def test_drafted_values_that_are_not_finite_at_any_start(dim, group, nodes, length):
+    """Drafted rows that begin anywhere in a tile, so that the lanes that look at a row are not those that
+    copied it, every fourth node with an undefined value."""
+    s = Setup("bf16", dim, 2, group, 16, [length, length + 1], [nodes, nodes], seed=length)
+    clean, clean_lse = s.run()
+    damaged = s.cache.pool.clone()
+    marks = [(b, node, (7 * node + b) % dim) for b in (0, 1) for node in range(0, nodes, 4)]
+    for b, node, column in marks:
+        at = s.lengths[b] + node
+        damaged[0, 1, s.tables[b, at // 16], at % 16, 1, column] = math.nan
+    s.cache.pool.copy_(damaged)
+    hit = torch.zeros_like(clean, dtype=torch.bool)
+    for b, node, column in marks:
+        for n, seen in enumerate(drafting.ancestors(s.parents[b], nodes)):
+            hit[b, n, group:, column] |= node in seen
+    for _ in range(5):
+        out, lse = s.run()
+        assert torch.equal(torch.isnan(out), hit) and torch.equal(lse, clean_lse)
+        s.check(torch.where(hit, clean, out), lse)

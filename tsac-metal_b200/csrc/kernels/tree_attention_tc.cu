@@ -423,6 +423,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
             if (copied_draft >= 0)
             {
+                __syncwarp(); // a wait covers a lane's own copies, and the rows below are other lanes'
                 // 0 x NaN would reach rows that do not see the node: values that are not
                 // finite leave the product and are added where they are seen.
                 const int chunk = lane % L::chunks;
