@@ -451,3 +451,26 @@ def test_drafted_values_that_are_not_finite_at_any_start(dim, group, nodes, leng
         out, lse = s.run()
         assert torch.equal(torch.isnan(out), hit) and torch.equal(lse, clean_lse)
         s.check(torch.where(hit, clean, out), lse)
+
+
+@pytest.mark.parametrize("kind,dim,group", [("bf16", 128, 8), ("fp16", 64, 5), ("bf16", 64, 2)])
+def test_undefined_values_in_some_of_many_trees(kind, dim, group):
+    """Several items one after another in each CTA, some with drafted values that are undefined: the marks
+    of one never reach the next."""
+    count, nodes = 60, 48
+    s = Setup(kind, dim, 8, group, 16, [(37 * b) % 300 for b in range(count)], [nodes - b % 5 for b in range(count)], seed=4)
+    clean, clean_lse = s.run()
+    damaged = s.cache.pool.clone()
+    hit = torch.zeros_like(clean, dtype=torch.bool)
+    for b in range(0, count, 3):
+        for head in range(8):
+            node, column = (5 * b + 11 * head) % s.nodes[b], (b + 9 * head) % dim
+            at = s.lengths[b] + node
+            damaged[0, 1, s.tables[b, at // 16], at % 16, head, column] = math.nan
+            for n, seen in enumerate(drafting.ancestors(s.parents[b], s.nodes[b])):
+                hit[b, n, head * group:(head + 1) * group, column] |= node in seen
+    s.cache.pool.copy_(damaged)
+    for _ in range(5):
+        out, lse = s.run()
+        assert torch.equal(torch.isnan(out), hit) and torch.equal(lse, clean_lse)
+    s.check(torch.where(hit, clean, out), lse, entries=[0, 1, 2, 27, 58])

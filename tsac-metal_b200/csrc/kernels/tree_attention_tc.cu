@@ -871,7 +871,9 @@ __global__ void __launch_bounds__(THREADS, 1)
             tc_fence_after();
             products_seen.first += made.first;
             products_seen.second += made.second;
-            const unsigned long long tainted = has_draft ? tail.tainted[segment % TAINT_SLOTS] : 0ull;
+            // One lane's answer for the warp, whose threads load TMEM together for each of the nodes.
+            const unsigned long long tainted =
+                __shfl_sync(0xffffffffu, has_draft ? tail.tainted[segment % TAINT_SLOTS] : 0ull, 0);
             const int draft_group = TWO ? group : (tiles - 1) & 1; // whose P is the drafted tile's
             const bool whole = g.tile_begin == 0 && has_draft;
             // A piece that begins its item goes to the CTA's second place, any other to its first.
@@ -967,11 +969,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                 shared_items[cta] = TreeShared{g.list_entry, g.head, g.first_row,
                                                Work::owner(start.units, g.item_start + g.e.tiles - 1, start.ctas) - cta + 1,
                                                g.e.nodes};
-            if constexpr (!TWO)
-                softmax_sync(); // the groups' statistics and the tainted nodes have been read
-            else if (tainted)
+            // The groups' statistics and the tainted nodes have been read.  Whether to wait must not depend on
+            // the nodes: after a wait that gave up, the threads may have read them at different times.
+            if (!TWO || has_draft)
                 softmax_sync();
-            if (t == 0 && tainted)
+            if (t == 0 && has_draft)
                 tail.tainted[segment % TAINT_SLOTS] = 0;
             tc_fence_before();
             bar_arrive(smem_u32(&tail.done));
