@@ -555,6 +555,9 @@ int tsac_cuda_cache_compact(const tsac_cuda_paged_cache* cache, int32_t* tables_
  * of the pool is reported likewise and read as zeros.  The same sequence may be
  * listed more than once.  The order of the sums depends on all lengths and
  * nodes of the call, and on nothing else.  max_nodes 1 is plain decoding.
+ * Bit 4 of *error_word: a bounded wait of the kernel for many rows gave up
+ * (after a second; a fault of the device or of this library); the rows that it
+ * could not finish hold NaN.
  * head_dim 64 or 128; max_nodes <= TSAC_CUDA_MAX_NODES. */
 size_t tsac_cuda_tree_attention_scratch_bytes(const tsac_cuda_paged_cache* cache, size_t heads,
                                               size_t max_nodes);

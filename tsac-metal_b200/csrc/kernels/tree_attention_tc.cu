@@ -50,7 +50,7 @@
 // Every wait is bounded (tc_common.cuh).  One that gives up raises
 // error_timeout and the CTA's abort flag; softmax threads then run through
 // their loops without waiting, so that no thread waits at a barrier that
-// others have left.
+// others have left, and give NaN for the rows that they could not finish.
 #include "kernels/half_types.cuh"
 #include "kernels/launch_count.hpp"
 #include "kernels/pdl.cuh"
@@ -847,6 +847,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const Both<int> made{TWO ? tiles : (tiles + 1) / 2, TWO ? tiles : tiles / 2};
             if (made(group))
                 wait(tail.products[group], products_seen(group) + made(group) - 1);
+            sum = ok ? sum : NAN;
             Both<float> part{1.0f, 1.0f}; // factors of the groups' outputs
             if constexpr (!TWO)
             {
@@ -865,7 +866,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 maximum = fmaxf(m0, m1);
                 part.first = m0 == -INFINITY ? 0.0f : power_of_two(m0 - maximum);
                 part.second = m1 == -INFINITY ? 0.0f : power_of_two(m1 - maximum);
-                sum = sum0 * part.first + sum1 * part.second;
+                sum = ok ? sum0 * part.first + sum1 * part.second : NAN;
             }
             __syncwarp();
             tc_fence_after();
