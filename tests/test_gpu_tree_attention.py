@@ -474,3 +474,40 @@ def test_undefined_values_in_some_of_many_trees(kind, dim, group):
         out, lse = s.run()
         assert torch.equal(torch.isnan(out), hit) and torch.equal(lse, clean_lse)
     s.check(torch.where(hit, clean, out), lse, entries=[0, 1, 2, 27, 58])
+
+
+@pytest.mark.parametrize("kind,dim,group,nodes", [("fp16", 64, 1, 1), ("fp16", 128, 4, 4), ("fp16", 64, 4, 32), ("fp16", 128, 3, 7),
+                                                  ("fp16", 64, 8, 64), ("fp16", 128, 8, 64), ("bf16", 128, 4, 4), ("bf16", 64, 8, 20)])
+@pytest.mark.parametrize("nats", [16.0, 18.0, 20.0])
+@pytest.mark.parametrize("sink", [0, 19000])
+def test_small_weights_beside_a_dominant_key(kind, dim, group, nodes, nats, sink):
+    """One key far above 20,000 others, with zeros as its value: the others' weights are the output, and
+    fp16 has to hold them.  A weight is rounded by half a step of itself, or by 2^-25 where it is subnormal;
+    with the row's largest at 2^10 at least that is 2^-35 per key in units of the largest.  The sequence is
+    listed often enough that no item is split over many CTAs, each of which would have a maximum of its own."""
+    length, page, scale, count = 20_000, 64, dim ** -0.5, 296
+    g = torch.Generator().manual_seed(dim + nodes)
+    pages = -(-(length + nodes) // page)
+    keys = torch.randn(pages * page, dim, generator=g) * 0.3
+    values = 1.0 + 0.25 * torch.randn(pages * page, dim, generator=g)
+    keys[sink], values[sink] = nats / math.sqrt(dim), 0.0
+    query = (1.0 + 0.05 * torch.randn(1, nodes, group, dim, generator=g)).to(TYPES[kind]).cuda()
+    pool = torch.stack((keys, values)).view(1, 2, pages, page, 1, dim).to(TYPES[kind]).cuda()
+    cache = tsac_cuda.PagedCache(pool, torch.arange(pages, dtype=torch.int32, device="cuda")[None], ints([pages]), ints([length]),
+                                 torch.ones(pages, dtype=torch.int32, device="cuda"))
+    lse = torch.empty(count, nodes, group, device="cuda")
+    out = cache.attention(0, query.expand(count, -1, -1, -1), ints([[-1] + [0] * (nodes - 1)] * count), lse=lse,
+                          sequences=torch.zeros(count, dtype=torch.int32, device="cuda")).double()
+    k, v = (pool[0, i].reshape(-1, dim)[:length + nodes].double() for i in (0, 1))
+    z = torch.einsum("nhd,kd->nhk", query[0].double(), k) * scale
+    for n in range(nodes):  # node 0 and children of it
+        z[n, :, length + 1:length + max(1, n)] = -math.inf
+        z[n, :, length + n + 1:] = -math.inf
+    p = torch.softmax(z, -1)
+    want, size, want_lse = p @ v, p @ v.abs(), torch.logsumexp(z, -1)
+    half, total = torch.finfo(TYPES[kind]).eps / 2, length + nodes
+    reach = (query[0].double().abs().amax((0, 1)) * k.abs().amax(0)).sum().item() * scale
+    fine = (2 * (dim + 2) * reach + 2 * total) * 2.0 ** -23
+    tiny = 2.0 ** -25 + total * 2.0 ** -35 * v.abs().max().item() if kind == "fp16" else 0.0
+    assert ((out - want).abs() <= half * (1 + fine) * size + half * want.abs() + fine * size + tiny).all()
+    assert ((lse.double() - want_lse).abs() <= fine + 4 * 2.0 ** -23 * (1 + want_lse.abs())).all()

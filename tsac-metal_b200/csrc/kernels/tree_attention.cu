@@ -6,7 +6,10 @@
 // warp keeps a running maximum, sum and output of its rows over its share of
 // the keys, and the shares are joined at the end (warps in shared memory, CTAs
 // in a second small launch).  Sums and outputs are 32-bit; p is rounded to the
-// input type for the second product, as its operand must be.
+// input type for the second product, as its operand must be.  For fp16 the
+// reference is 15 below the running maximum (Half2::weight_powers): a p then
+// keeps all its bits down to 2^-29 of the row's largest, and is nothing from
+// 2^-40 on.
 //
 // Bound: the keys and values cross HBM once per key head, M / 2 multiply-adds
 // per byte for M query rows; up to 32 rows that is below what mma.sync
@@ -143,7 +146,8 @@ __global__ void __launch_bounds__(THREADS, 2)
             }
         }
         float o[D / 8][4] = {};
-        float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+        // The running maximum less Half2::weight_powers: what p is a power of two from.
+        float reference[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
 
         int stage = 0;
         for (int tile = tile_begin; tile < tile_end; ++tile)
@@ -206,7 +210,7 @@ __global__ void __launch_bounds__(THREADS, 2)
                     sees = Work::visible(g, tile, warp * WARP_KEYS / 32, last && row < rows ? masks[row / a.group] : 0ull) >>
                            (first_bit + 2 * (lane & 3)); // this lane's keys: bits 0 and 1 of each 8
                 }
-                float z[2 * NT], best = top[r];
+                float z[2 * NT], best = -INFINITY;
 #pragma unroll
                 for (int k = 0; k < 2 * NT; ++k)
                 {
@@ -217,9 +221,10 @@ __global__ void __launch_bounds__(THREADS, 2)
                 }
                 best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
                 best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
+                best = fmaxf(reference[r], best - Half2<T>::weight_powers);
                 const float shift = best == -INFINITY ? 0.0f : best; // rows that have seen nothing yet
-                const float scale = power_of_two(top[r] - shift);
-                top[r] = best;
+                const float scale = power_of_two(reference[r] - shift);
+                reference[r] = best;
                 float partial = 0.0f;
 #pragma unroll
                 for (int k = 0; k < 2 * NT; ++k)
@@ -309,7 +314,7 @@ __global__ void __launch_bounds__(THREADS, 2)
             sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
             if ((lane & 3) == 0)
             {
-                row_max[warp][8 * r + (lane >> 2)] = top[r];
+                row_max[warp][8 * r + (lane >> 2)] = reference[r];
                 row_sum[warp][8 * r + (lane >> 2)] = sum[r];
             }
         }
@@ -323,7 +328,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
             for (int w = 0; w < WARPS; ++w)
                 best = fmaxf(best, row_max[w][row]);
-            const float scale = best == -INFINITY ? 0.0f : power_of_two(top[r] - best);
+            const float scale = best == -INFINITY ? 0.0f : power_of_two(reference[r] - best);
 #pragma unroll
             for (int n = 0; n < D / 8; ++n)
                 *reinterpret_cast<float2*>(merge + (warp * L::ROWS + row) * D + 8 * n + 2 * (lane & 3)) =

@@ -320,7 +320,8 @@ struct TreeShared
     int nodes;
 };
 
-// A piece's row: running maximum (of scores x log2(e)), sum, and the unscaled output.
+// A piece's row: the number that its weights are powers of two from, near the
+// running maximum of scores x log2(e), and the sum and output of those weights.
 constexpr int TREE_PIECE_HEAD = 4; // floats before a row's outputs, 16-byte aligned: maximum, sum
 inline __host__ __device__ long long tree_piece_floats(int rows, int head_dim)
 {

@@ -31,11 +31,15 @@
 //                   nodes over up to 4,096 positions).
 //   warp 11         the query rows of the next segment, as soon as the last
 //                   scores of this one are made, and its tree's masks.
-// The running maximum is a whole number and moves only when a row's scores
-// exceed it by more than 8 (in powers of two): p then stays below 256, which
-// bf16, fp16 and the 32-bit sums hold as well as 1, scores are read once, and
-// what has been computed with the old maximum, p of the same tile included, is
-// rescaled rarely and by powers of two.  The loop over a tile's scores is kept
+// The reference that p is a power of two from is a whole number and moves only
+// when a row's scores exceed it by more than LIMIT: scores are read once, and
+// what has been computed with the old reference, p of the same tile included, is
+// rescaled rarely and by powers of two.  For bf16 it is the running maximum with
+// a slack of 8: p stays below 2^8, which bf16 and the 32-bit sums hold as well
+// as 1.  For fp16 it is 11 below the maximum with a slack of 4: p stays below
+// 2^15 and the row's largest is 2^10 at least, so that a p keeps all its bits
+// down to 2^-24 of it and is nothing from 2^-35 on.  (A slack of 2 costs
+// rescaling: 2 x 64 nodes over 131,072 positions 267 us, 253 with 4 and with 8.)  The loop over a tile's scores is kept
 // small: unrolled over the whole tile it delayed the MMA warp (64 x 16 nodes 172
 // against 162 us), and exponentials of some pairs by a polynomial on the FMA
 // pipes gained nothing over the special function units' 16 per clock.
@@ -71,7 +75,6 @@ constexpr int MMA_WARP = 8, PRODUCER_WARP = 9, PRODUCERS = 64, PRODUCER_ROWS = K
 constexpr int QUERY_WARP = PRODUCER_WARP + PRODUCERS / 32;
 constexpr int THREADS = (QUERY_WARP + 1) * 32;
 constexpr int TMEM_COLUMNS = 512, OUTPUT_COLUMN = 256; // S of the groups at 0 and 128, O at 256 and 384
-constexpr float RESCALE = 8.0f;                        // powers of two
 constexpr int TAINT_SLOTS = 16; // segments that the producers can be ahead of the epilogue, and more
 
 template <int D, bool TWO> struct Tiles
@@ -339,6 +342,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     pdl_prologue();
     using L = Tiles<D, TWO>;
     using Work = TreeWork<KEYS, L::ROWS, 3>;
+    // Powers of two: how far a score may exceed the reference, and how far the one that moves it does.
+    constexpr bool narrow = Half2<T>::weight_powers > 0.0f;
+    constexpr float LIMIT = narrow ? Half2<T>::weight_powers : 8.0f, PLACE = narrow ? LIMIT - 4.0f : 0.0f;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                            ~static_cast<uintptr_t>(1023));
@@ -756,7 +762,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
             // A warp without a live row has nothing to compute: whatever its lanes of TMEM hold stays there.
             const bool busy = __any_sync(0xffffffffu, live);
-            float maximum = -INFINITY, sum = 0.0f;
+            float reference = -INFINITY, sum = 0.0f;
             for (int j = TWO ? 0 : group; j < tiles; j += TWO ? 1 : 2)
             {
                 const int tile = g.tile_begin + j;
@@ -785,11 +791,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                             best[k >> 1 & 3] = max3(best[k >> 1 & 3], __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
                         const float highest = max3(best[0], best[1], fmaxf(best[2], best[3]));
                         const float top = highest == -INFINITY ? -INFINITY : highest * scale;
-                        if (__any_sync(0xffffffffu, top > maximum + RESCALE))
+                        if (__any_sync(0xffffffffu, top > reference + LIMIT))
                         {
-                            const float raised = fmaxf(maximum, ceilf(top));
-                            const float shrink = maximum == -INFINITY ? 0.0f : power_of_two(maximum - raised);
-                            maximum = raised;
+                            const float raised = fmaxf(reference, ceilf(top) - PLACE);
+                            const float shrink = reference == -INFINITY ? 0.0f : power_of_two(reference - raised);
+                            reference = raised;
                             sum *= shrink;
                             part = mul_pair(part, make_pair(shrink, shrink));
                             // P of this tile's earlier scores, then the output; its last product is
@@ -819,7 +825,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                                 tmem_store16(my_output + 16 * b, w);
                             }
                         }
-                        const float shift = maximum == -INFINITY ? 0.0f : -maximum;
+                        const float shift = reference == -INFINITY ? 0.0f : -reference;
                         uint32_t p[16];
 #pragma unroll
                         for (int k = 0; k < 32; k += 2)
@@ -852,7 +858,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             if constexpr (!TWO)
             {
                 // The groups exchange their statistics in TMEM, in columns of S that P leaves free.
-                tmem_store2(my_scores + KEYS / 2, __float_as_uint(maximum), __float_as_uint(sum));
+                tmem_store2(my_scores + KEYS / 2, __float_as_uint(reference), __float_as_uint(sum));
                 tmem_wait_stores();
                 tc_fence_before();
                 softmax_sync();
@@ -863,9 +869,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                 tc_fence_after();
                 const float m0 = __uint_as_float(tmem_load1(lanes + KEYS / 2)), m1 = __uint_as_float(tmem_load1(lanes + KEYS + KEYS / 2));
                 const float sum0 = __uint_as_float(tmem_load1(lanes + KEYS / 2 + 1)), sum1 = __uint_as_float(tmem_load1(lanes + KEYS + KEYS / 2 + 1));
-                maximum = fmaxf(m0, m1);
-                part.first = m0 == -INFINITY ? 0.0f : power_of_two(m0 - maximum);
-                part.second = m1 == -INFINITY ? 0.0f : power_of_two(m1 - maximum);
+                reference = fmaxf(m0, m1);
+                part.first = m0 == -INFINITY ? 0.0f : power_of_two(m0 - reference);
+                part.second = m1 == -INFINITY ? 0.0f : power_of_two(m1 - reference);
                 sum = ok ? sum0 * part.first + sum1 * part.second : NAN;
             }
             __syncwarp();
@@ -957,13 +963,13 @@ __global__ void __launch_bounds__(THREADS, 1)
             {
                 if (!whole)
                 {
-                    piece[0] = maximum;
+                    piece[0] = reference;
                     piece[1] = sum;
                 }
                 else if (a.lse)
                 {
                     a.lse[(static_cast<long long>(g.list_entry) * a.max_nodes + node) * a.heads * a.group + query_head] =
-                        sum == 0.0f ? -INFINITY : (maximum + log2f(sum)) * 0.6931471805599453f;
+                        sum == 0.0f ? -INFINITY : (reference + log2f(sum)) * 0.6931471805599453f;
                 }
             }
             if (g.tile_begin == 0 && !whole && t == 0)
