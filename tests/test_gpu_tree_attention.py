@@ -511,3 +511,26 @@ def test_small_weights_beside_a_dominant_key(kind, dim, group, nodes, nats, sink
     tiny = 2.0 ** -25 + total * 2.0 ** -35 * v.abs().max().item() if kind == "fp16" else 0.0
     assert ((out - want).abs() <= half * (1 + fine) * size + half * want.abs() + fine * size + tiny).all()
     assert ((lse.double() - want_lse).abs() <= fine + 4 * 2.0 ** -23 * (1 + want_lse.abs())).all()
+
+
+@pytest.mark.parametrize("kind,dim,group,nodes", [("fp16", 64, 1, 3), ("bf16", 128, 2, 8), ("fp16", 64, 4, 17), ("fp16", 128, 8, 33), ("bf16", 64, 4, 40)])
+def test_scores_of_any_size(kind, dim, group, nodes):
+    """Scores of up to 2^36 in powers of two, exact in 32 bits before the scale and far apart: the largest keys
+    share the row, and the log of the sum is their score."""
+    s = Setup(kind, dim, 1, group, 16, [700, 5], [nodes, nodes], seed=20)
+    g = torch.Generator().manual_seed(20)
+    s.pool[:, 0] = 0.0
+    s.pool[:, 0, ..., 3] = torch.randint(-100, 101, s.pool[:, 0, ..., 3].shape, generator=g).to(s.pool.dtype)
+    s.cache.pool.copy_(s.pool)
+    s.query[:] = 0.0
+    s.query[..., 3] = 2.0 ** 15 * torch.where(torch.arange(nodes) % 3 == 2, -1, 1)[:, None]
+    for power in range(0, 14):
+        scale = 2.0 ** power * (1 + 0.07 * power)
+        out, lse = s.run(scale=scale)
+        for b in (0, 1):
+            keys, values = s.rows(b)
+            want, want_lse, size = drafting.attention(s.query[b].double(), keys, values, s.lengths[b], s.parents[b], nodes, group, scale)
+            half = torch.finfo(TYPES[kind]).eps / 2
+            # Weights of equal scores are equal but for their own rounding; the others are nothing.
+            assert ((out[b] - want).abs() <= 2 * half * (size + want.abs()) + 2.0 ** -25).all(), (power, b)
+            assert ((lse[b] - want_lse).abs() <= 4 * 2.0 ** -23 * (1 + want_lse.abs())).all(), (power, b)

@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(THREADS, 2)
                 }
                 best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
                 best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
-                best = fmaxf(reference[r], best - Half2<T>::weight_powers);
+                best = fmaxf(reference[r], __fadd_ru(best, -Half2<T>::weight_powers)); // p is 2^weight_powers at most
                 const float shift = best == -INFINITY ? 0.0f : best; // rows that have seen nothing yet
                 const float scale = power_of_two(reference[r] - shift);
                 reference[r] = best;

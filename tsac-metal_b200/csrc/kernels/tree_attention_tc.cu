@@ -791,9 +791,21 @@ __global__ void __launch_bounds__(THREADS, 1)
                             best[k >> 1 & 3] = max3(best[k >> 1 & 3], __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
                         const float highest = max3(best[0], best[1], fmaxf(best[2], best[3]));
                         const float top = highest == -INFINITY ? -INFINITY : highest * scale;
-                        if (__any_sync(0xffffffffu, top > reference + LIMIT))
+                        // From 2^23 on (and below infinity) a product's rounding moves a weight by powers of two: the
+                        // scores are then rounded like the maximum that the reference comes from.
+                        const bool coarse = (__float_as_uint(top) & 0x7fffffffu) - 0x4b000000u < 0x34800000u;
+                        float factor = scale;
+                        if (__any_sync(0xffffffffu, coarse || top > reference + LIMIT))
                         {
-                            const float raised = fmaxf(reference, ceilf(top) - PLACE);
+                            if (__any_sync(0xffffffffu, coarse))
+                            {
+                                const float early = coarse ? scale : 1.0f;
+                                factor = coarse ? 1.0f : scale;
+#pragma unroll
+                                for (int k = 0; k < 32; ++k)
+                                    s[k] = __float_as_uint(__uint_as_float(s[k]) * early);
+                            }
+                            const float raised = fmaxf(reference, __fadd_ru(ceilf(top), -PLACE));
                             const float shrink = reference == -INFINITY ? 0.0f : power_of_two(reference - raised);
                             reference = raised;
                             sum *= shrink;
@@ -832,7 +844,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         {
                             float x, y;
                             split(fma_pair(make_pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])),
-                                           make_pair(scale, scale), make_pair(shift, shift)),
+                                           make_pair(factor, factor), make_pair(shift, shift)),
                                   x, y);
                             x = power_of_two(x);
                             y = power_of_two(y);
