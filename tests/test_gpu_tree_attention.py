@@ -534,3 +534,18 @@ def test_scores_of_any_size(kind, dim, group, nodes):
             # Weights of equal scores are equal but for their own rounding; the others are nothing.
             assert ((out[b] - want).abs() <= 2 * half * (size + want.abs()) + 2.0 ** -25).all(), (power, b)
             assert ((lse[b] - want_lse).abs() <= 4 * 2.0 ** -23 * (1 + want_lse.abs())).all(), (power, b)
+
+
+@pytest.mark.parametrize("kind,dim,group,nodes", [("bf16", 128, 2, 7), ("fp16", 64, 1, 16), ("fp16", 128, 4, 20), ("bf16", 64, 8, 30)])
+@pytest.mark.parametrize("length", [3, 20, 3000])
+def test_rows_of_undefined_scores(kind, dim, group, nodes, length):
+    """A query row with a NaN: its output and its log of the sum are NaN, whole items and shared ones alike."""
+    s = Setup(kind, dim, 2, group, 16, [length, 20], [nodes, nodes], seed=21)
+    clean, clean_lse = s.run()
+    hit = torch.zeros_like(clean_lse, dtype=torch.bool)
+    for b, n, h in ((0, 0, 0), (0, nodes - 1, 2 * group - 1), (1, nodes // 2, group)):
+        s.query[b, n, h, 5] = math.nan
+        hit[b, n, h] = True
+    out, lse = s.run()
+    assert torch.equal(torch.isnan(lse), hit) and torch.equal(torch.isnan(out), hit[..., None].expand_as(out))
+    assert torch.equal(lse[~hit], clean_lse[~hit]) and torch.equal(out[~hit], clean[~hit])

@@ -351,7 +351,8 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
             for (int w = 0; w < WARPS; ++w)
             {
-                total += best == -INFINITY ? 0.0f : row_sum[w][row] * power_of_two(row_max[w][row] - best);
+                // A row of undefined scores has no maximum, but an undefined sum.
+                total += best == -INFINITY ? row_sum[w][row] : row_sum[w][row] * power_of_two(row_max[w][row] - best);
                 const float4 x = *reinterpret_cast<const float4*>(merge + (w * L::ROWS + row) * D + column);
                 v.x += x.x;
                 v.y += x.y;
