@@ -549,3 +549,17 @@ def test_rows_of_undefined_scores(kind, dim, group, nodes, length):
     out, lse = s.run()
     assert torch.equal(torch.isnan(lse), hit) and torch.equal(torch.isnan(out), hit[..., None].expand_as(out))
     assert torch.equal(lse[~hit], clean_lse[~hit]) and torch.equal(out[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("kind,dim,group,nodes", [("bf16", 128, 1, 5), ("fp16", 64, 2, 8), ("bf16", 64, 4, 17), ("fp16", 128, 8, 33)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_a_scale_of_zero_hides_nothing(kind, dim, group, nodes, bad):
+    """Zero times a score that is not finite is undefined, in a row of many keys and of one."""
+    s = Setup(kind, dim, 2, group, 16, [300, 20, 0], [nodes, nodes, nodes], seed=18)
+    hit = torch.zeros(3, nodes, 2 * group, dtype=torch.bool)
+    for b, n, h in ((1, nodes - 1, 0), (2, 0, group), (2, 0, 0)):
+        s.query[b, n, h, 3] = bad
+        hit[b, n, h] = True
+    out, lse = s.run(scale=0.0)
+    assert torch.equal(torch.isnan(lse), hit) and torch.equal(torch.isnan(out), hit[..., None].expand_as(out))
+    assert torch.isfinite(out[~hit]).all()

@@ -544,9 +544,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     else if (warp == QUERY_WARP)
     {
         // -------------------------------------------------------------- queries --
-        // A negative scale turns the query's signs and a zero one clears it, so that the
-        // softmax's factor is positive: the largest product is the largest score.
-        const uint32_t turn = a.scale_log2 < 0.0f ? 0x80008000u : 0u, keep = a.scale_log2 == 0.0f ? 0u : ~0u;
+        // A negative scale turns the query's signs and a zero one clears it (to NaN where it is not
+        // finite, as the product with zero is), so that the softmax's factor is positive: the largest
+        // product is the largest score.
+        const bool zero = a.scale_log2 == 0.0f;
+        const auto turned = [&](uint32_t v) { return zero ? nonfinite_mask<T>(v) : v ^ 0x80008000u; };
         constexpr int rows_at_once = 32 / L::chunks;
         const int chunk = lane % L::chunks;
         for (int segment = 0; ok && cursor.next(a, g); ++segment)
@@ -591,7 +593,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 {
                     auto* at = reinterpret_cast<uint4*>(smem + place(row));
                     const uint4 v = *at;
-                    *at = make_uint4((v.x ^ turn) & keep, (v.y ^ turn) & keep, (v.z ^ turn) & keep, (v.w ^ turn) & keep);
+                    *at = make_uint4(turned(v.x), turned(v.y), turned(v.z), turned(v.w));
                 }
             fence_async_proxy();
             __syncwarp();
