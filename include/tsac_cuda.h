@@ -572,7 +572,9 @@ int tsac_cuda_tree_attention(const tsac_cuda_paged_cache* cache, size_t layer, c
  * From node 0 on, the children of the current node are tried in ascending
  * order; w is the target's row p there, x the child's token, u its coin:
  *   draft NULL:  accepted when u * (1 - the rejected siblings' p) < p(x); the
- *                rejected tokens then leave w
+ *                rejected tokens then leave w.  The 1 stands for the row's sum:
+ *                as far as that is not 1 (16-bit rows are rounded), what is kept
+ *                departs from the target's distribution
  *   draft given: accepted when u * q(x) < w(x) with q the draft's row at the
  *                current node; a rejection makes w = max(w - q, 0) / its sum
  *                (w stays where that sum is 0)
