@@ -586,7 +586,9 @@ int tsac_cuda_tree_attention(const tsac_cuda_paged_cache* cache, size_t layer, c
  *            vocabulary is contiguous
  *   tokens, parents  device int32 [batch][max_nodes]; node 0's are not read.  A
  *            token outside the vocabulary has probability 0
- *   coins    device f32 [batch][max_nodes], draws device f32 [batch], in [0, 1)
+ *   coins    device f32 [batch][max_nodes], draws device f32 [batch], in [0, 1).
+ *            A draw below 0 or undefined is taken as 0, one from 1 on gives the
+ *            last token of positive weight
  *   nodes    device int32 [batch] or NULL: max_nodes each
  *   accepted device int32 [batch]: nodes kept, node 0 included (0 without nodes)
  *   path     device int32 [batch][max_nodes]: the kept nodes, then -1: what

@@ -213,3 +213,20 @@ def test_binding_refuses_error_words_of_other_sizes():
                  torch.zeros(0, dtype=torch.int32, device="cuda")):
         with pytest.raises(tsac_cuda.TsacError, match="32-bit word"):
             tsac_cuda.draft_verify(target, tokens, parents, coins, draws, error_word=word)
+
+
+@pytest.mark.parametrize("with_draft", [False, True])
+@pytest.mark.parametrize("vocab", [64, 9001])
+@pytest.mark.parametrize("draw", [-0.25, -float("inf"), float("nan"), 1.0, 7.0])
+def test_draws_outside_the_interval_give_a_token(with_draft, vocab, draw):
+    """Every output is written, with a token of positive weight."""
+    target, tokens, parents, coins, draws, draft = case(3, 4, vocab, "fp32", with_draft, 6)
+    target[..., :5], target[..., -3:] = 0.0, 0.0
+    draws[1] = draw
+    out = tuple(torch.full(s, 99999, dtype=torch.int32, device="cuda") for s in ((3,), (3, 4), (3,)))
+    tsac_cuda.draft_verify(target.cuda(), tokens.cuda(), parents.cuda(), coins.cuda(), draws.cuda(),
+                           draft=None if draft is None else draft.cuda(), out=out)
+    want = drafting.verify(target[1].double().numpy(), tokens[1].tolist(), parents[1].tolist(), coins[1].double().tolist(),
+                           1.0 if draw >= 1 else 0.0, None if draft is None else draft[1].double().numpy(), 4)
+    assert out[1][1].tolist() == want[0] + [-1] * (4 - len(want[0])) and out[2][1].item() == want[1]
+    assert target[1, want[0][-1], want[1]] > 0

@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(THREADS, (DRAFT ? 512 : 1024) / THREADS) draft
     nodes = nodes < 0 ? 0 : (nodes < a.max_nodes ? nodes : a.max_nodes);
     const T* target = static_cast<const T*>(a.target) + sequence * a.target_batch;
     const T* draft = DRAFT ? static_cast<const T*>(a.draft) + sequence * a.draft_batch : nullptr;
-    const float draw = a.draws[sequence];
+    const float draw = fmaxf(a.draws[sequence], 0.0f); // outside [0, 1): the first or the last token of positive weight
     if (t < DRAFT_MAX_NODES)
     {
         const bool there = t < nodes;
