@@ -510,8 +510,8 @@ int tsac_cuda_cache_append(const tsac_cuda_paged_cache* cache, size_t layer, con
 /* Keeps the accepted rows: in every layer row start + path[i][j] moves to
  * start + j for j < accepted[i], and the sequence's new length start +
  * accepted[i] is written to lengths_out [sequences] (the cache's own lengths,
- * or another buffer that overlaps neither them nor starts; other sequences'
- * entries are left as they were).
+ * or another buffer, which overlaps nothing else that the call is given; other
+ * sequences' entries are left as they were).
  *   path  device int32 [count][width], ascending; entries from accepted[i] on
  *         are not read
  *   starts device int32 [count] or NULL: the sequences' lengths */

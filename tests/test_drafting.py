@@ -207,3 +207,24 @@ def test_scales_that_overflow_in_powers_of_two_are_refused(scale):
     lib, c, s3 = tsac_cuda._drafting(), cache(), strides(1024, 512, 128)
     refused(lib.tsac_cuda_tree_attention(ctypes.addressof(c), 0, None, FAKE, None, FAKE, s3, FAKE, s3, None, 4, 1, 1, scale,
                                          FAKE, 1 << 40, None, None), "scale")
+
+
+@pytest.mark.parametrize("place", ["sequences", "path", "accepted"])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_new_lengths_over_another_argument_are_refused(place, in_place):
+    """Every plane's CTA reads the lists while the first one writes the new lengths."""
+    lib = tsac_cuda._drafting()
+    c = cache(tables=3 * FAKE, counts=4 * FAKE, lengths=5 * FAKE, refs=6 * FAKE)
+    out = c.lengths if in_place else 7 * FAKE
+    given = dict(sequences=8 * FAKE, path=9 * FAKE, accepted=10 * FAKE)
+    given[place] = out + 12 if place != "path" else out - 4 * (2 * 3 - 1)  # the last of one over an end of the other
+    refused(lib.tsac_cuda_cache_keep(ctypes.addressof(c), given["sequences"], given["path"], given["accepted"], None, out, 2, 3,
+                                     None, None), "overlap another argument")
+
+
+@pytest.mark.parametrize("name", ["tables", "counts", "refs"])
+def test_new_lengths_over_the_cache_are_refused(name):
+    lib = tsac_cuda._drafting()
+    c = cache(tables=3 * FAKE, counts=4 * FAKE, lengths=5 * FAKE, refs=6 * FAKE)
+    refused(lib.tsac_cuda_cache_keep(ctypes.addressof(c), None, 8 * FAKE, 9 * FAKE, None, getattr(c, name) + 4, 2, 3, None, None),
+            "overlap another argument")

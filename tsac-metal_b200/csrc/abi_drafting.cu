@@ -187,6 +187,14 @@ int tsac_cuda_cache_keep(const tsac_cuda_paged_cache* cache, const int32_t* sequ
                     "new lengths overlap the cache's lengths");
             require(!starts || !overlap(lengths_out, cache->sequences, starts, count),
                     "new lengths overlap the starts");
+            // Other CTAs still read these when the first new length is written.
+            require(!(sequences && overlap(lengths_out, cache->sequences, sequences, count)) &&
+                        !overlap(lengths_out, cache->sequences, path, count * width) &&
+                        !overlap(lengths_out, cache->sequences, accepted, count) &&
+                        (lengths_out == v.lengths || (!overlap(lengths_out, cache->sequences, v.counts, cache->sequences) &&
+                                                      !overlap(lengths_out, cache->sequences, v.refs, cache->pages) &&
+                                                      !overlap(lengths_out, cache->sequences, v.tables, cache->sequences * cache->max_pages))),
+                    "new lengths overlap another argument");
             require_device();
             if (count == 0)
                 return;
