@@ -544,7 +544,8 @@ int tsac_cuda_cache_compact(const tsac_cuda_paged_cache* cache, int32_t* tables_
  *            with the given strides in elements (multiples of 8; the last
  *            dimension is contiguous), 16-byte aligned.  heads is a multiple
  *            of kv_heads: query head h reads key head h / (heads / kv_heads).
- *            out may be query itself (the same strides), but not overlap it otherwise
+ *            out may be query itself (the same strides), but not overlap it
+ *            otherwise; its rows must not overlap one another
  *   lse      device f32 [count][max_nodes][heads] or NULL: log of the sum of
  *            exponentials
  *   scratch  device, >= tsac_cuda_tree_attention_scratch_bytes(cache, heads,

@@ -228,3 +228,29 @@ def test_new_lengths_over_the_cache_are_refused(name):
     c = cache(tables=3 * FAKE, counts=4 * FAKE, lengths=5 * FAKE, refs=6 * FAKE)
     refused(lib.tsac_cuda_cache_keep(ctypes.addressof(c), None, 8 * FAKE, 9 * FAKE, None, getattr(c, name) + 4, 2, 3, None, None),
             "overlap another argument")
+
+
+@pytest.mark.parametrize("strides_,count,nodes,overlap", [
+    ((1024, 512, 128), 4, 2, None), ((128, 2048, 512), 4, 2, None), ((512, 2048, 128), 4, 3, None), ((8, 512, 128), 1, 2, None),
+    ((-1024, 512, 128), 4, 2, None), ((0, 512, 128), 4, 2, "output rows"), ((1024, 0, 128), 4, 2, "output rows"),
+    ((1024, 512, 0), 4, 2, "output rows"), ((1024, 512, 120), 4, 2, "output rows"), ((1016, 512, 128), 4, 2, "output rows"),
+    ((512, 512, 128), 4, 2, "output rows"), ((1024, -504, 128), 4, 2, "output rows"), ((1 << 60, 512, 128), 4, 2, "output rows"),
+    ((1024, 512, -128), 4, 2, None), ((0, 0, 128), 1, 1, None)])
+def test_outputs_that_overlap_themselves_are_refused(strides_, count, nodes, overlap):
+    lib, c = tsac_cuda._drafting(), cache()
+    status = lib.tsac_cuda_tree_attention(ctypes.addressof(c), 0, None, FAKE, None, FAKE, strides(1024, 512, 128), 64 * FAKE,
+                                          strides(*strides_), None, 4, count, nodes, 1.0, None, 0, None, None)
+    if overlap:
+        refused(status, "output rows overlap")
+    elif torch.cuda.is_available():
+        refused(status, "scratch too small")
+    else:
+        assert status == tsac_cuda.ERROR_DEVICE
+
+
+@pytest.mark.parametrize("other", [(1024, 512, 256), (2048, 512, 128), (1024, 1024, 128)])
+def test_output_in_place_of_the_query_needs_its_strides(other):
+    lib, c = tsac_cuda._drafting(), cache()
+    for a, b in (((1024, 512, 128), other), (other, (1024, 512, 128))):
+        refused(lib.tsac_cuda_tree_attention(ctypes.addressof(c), 0, None, FAKE, None, FAKE, strides(*a), FAKE, strides(*b), None,
+                                             4, 2, 2, 1.0, None, 0, None, None), "output")

@@ -5,8 +5,10 @@
 #include "kernels/paged_cache.cuh"
 #include "kernels/tree_attention.cuh"
 
+#include <algorithm>
 #include <bit>
 #include <cmath>
+#include <utility>
 
 namespace
 {
@@ -60,6 +62,27 @@ void require_strides(const ptrdiff_t strides[3], const char* what)
     require(strides, "null argument");
     for (int k = 0; k < 3; ++k)
         require(strides[k] % 8 == 0, what);
+}
+
+// Whether no two of the [entry][node][head] rows of `row` elements share one: each
+// dimension, taken from the smallest stride up, steps over all that lies inside it.
+bool rows_apart(const ptrdiff_t strides[3], const size_t sizes[3], size_t row)
+{
+    std::pair<size_t, size_t> steps[3]; // (stride, size)
+    for (int k = 0; k < 3; ++k)
+        steps[k] = {sizes[k] > 1 ? (strides[k] < 0 ? size_t{0} - static_cast<size_t>(strides[k]) : static_cast<size_t>(strides[k])) : SIZE_MAX,
+                    sizes[k]};
+    std::sort(steps, steps + 3);
+    size_t span = row;
+    for (const auto& [stride, size] : steps)
+    {
+        if (size <= 1)
+            continue;
+        if (stride < span || stride > SIZE_MAX / 4 / size)
+            return false;
+        span += stride * (size - 1);
+    }
+    return true;
 }
 
 bool overlap(const int32_t* a, size_t m, const int32_t* b, size_t n)
@@ -261,6 +284,11 @@ int tsac_cuda_tree_attention(const tsac_cuda_paged_cache* cache, size_t layer, c
             require_strides(query_strides, "query strides must be multiples of 8 elements");
             require_strides(out_strides, "output strides must be multiples of 8 elements");
             require(aligned16(query) && aligned16(out), "query and output must be 16-byte aligned");
+            const size_t sizes[3] = {count, max_nodes, heads};
+            require(count == 0 || rows_apart(out_strides, sizes, cache->head_dim), "output rows overlap one another");
+            for (int k = 0; k < 3 && count; ++k)
+                require(out != query || sizes[k] == 1 || out_strides[k] == query_strides[k],
+                        "output in place of the query needs the query's strides");
             require_device();
             require(scratch && aligned16(scratch) &&
                         scratch_bytes >= tsac_cuda_tree_attention_scratch_bytes(cache, heads, max_nodes),
