@@ -549,7 +549,8 @@ int tsac_cuda_cache_compact(const tsac_cuda_paged_cache* cache, int32_t* tables_
  *   lse      device f32 [count][max_nodes][heads] or NULL: log of the sum of
  *            exponentials
  *   scratch  device, >= tsac_cuda_tree_attention_scratch_bytes(cache, heads,
- *            max_nodes), 16-byte aligned; calls that overlap need their own
+ *            max_nodes), asked for with the cache's device current, 16-byte
+ *            aligned; calls that overlap need their own
  * A row that sees nothing gives zeros and -infinity.  A value that is not
  * finite reaches the rows that see it and no others.  An entry whose length
  * and nodes exceed its pages is skipped (bit 16); a table entry that is no page

@@ -563,3 +563,38 @@ def test_a_scale_of_zero_hides_nothing(kind, dim, group, nodes, bad):
     out, lse = s.run(scale=0.0)
     assert torch.equal(torch.isnan(lse), hit) and torch.equal(torch.isnan(out), hit[..., None].expand_as(out))
     assert torch.isfinite(out[~hit]).all()
+
+
+def test_scratch_is_sized_by_the_caches_device(monkeypatch):
+    """Whichever device is current: here a second one is pretended, and every call of the library has to find
+    the cache's own in its place."""
+    s = Setup("bf16", 64, 1, 2, 16, [40], [4], seed=22)
+    current, calls = [7], []
+
+    class Guard:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            current.append(self.index)
+
+        def __exit__(self, *exc):
+            current.pop()
+
+    class Library:
+        def __getattr__(self, name):
+            fn = getattr(tsac_cuda._drafting(), name)
+
+            def called(*arguments):
+                calls.append((name, current[-1]))
+                return fn(*arguments)
+            return called
+
+    on = tsac_cuda._Device(s.cache.index)
+    monkeypatch.setattr(on, "_current", lambda: current[-1])
+    monkeypatch.setattr(on, "_cuda", type("Cuda", (), {"device": Guard}))
+    monkeypatch.setattr(s.cache, "_on", on)
+    monkeypatch.setattr(s.cache, "_lib", Library())
+    s.check(*s.run())
+    assert {name for name, _ in calls} == {"tsac_cuda_tree_attention", "tsac_cuda_tree_attention_scratch_bytes"}
+    assert all(device == s.cache.index for _, device in calls), calls

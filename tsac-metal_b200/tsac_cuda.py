@@ -205,12 +205,14 @@ class _Device:
     def stream(self) -> int:
         return self._stream(self.index)
 
-    def call(self, fn, *arguments) -> None:
+    def ask(self, fn, *arguments) -> int:
         if self._current() == self.index:
-            status = fn(*arguments)
-        else:
-            with self._cuda.device(self.index):
-                status = fn(*arguments)
+            return fn(*arguments)
+        with self._cuda.device(self.index):
+            return fn(*arguments)
+
+    def call(self, fn, *arguments) -> None:
+        status = self.ask(fn, *arguments)
         if status != OK:
             check(status)
 
@@ -406,7 +408,8 @@ class PagedCache:
         o, out_strides = _rows(out, "out", self.dtype, index, shape)
         nbytes = self._attention_bytes.get((heads, most))
         if nbytes is None:
-            nbytes = self._lib.tsac_cuda_tree_attention_scratch_bytes(self._cache, heads, most)
+            # By the cache's device: the size depends on its multiprocessors.
+            nbytes = on.ask(self._lib.tsac_cuda_tree_attention_scratch_bytes, self._cache, heads, most)
             self._attention_bytes[heads, most] = nbytes
         scratch = self._temporary(nbytes)
         on.call(self._lib.tsac_cuda_tree_attention, self._cache, layer,
