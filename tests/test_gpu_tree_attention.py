@@ -598,3 +598,25 @@ def test_scratch_is_sized_by_the_caches_device(monkeypatch):
     s.check(*s.run())
     assert {name for name, _ in calls} == {"tsac_cuda_tree_attention", "tsac_cuda_tree_attention_scratch_bytes"}
     assert all(device == s.cache.index for _, device in calls), calls
+
+
+def test_gradients_are_refused_not_dropped():
+    s = Setup("bf16", 64, 1, 2, 16, [40], [4], seed=23)
+    query, trees, rows = s.query.cuda(), ints(s.parents), torch.ones(1, 4, 1, 64, dtype=torch.bfloat16, device="cuda")
+    s.cache.append(0, rows, rows)
+    want = s.cache.attention(0, query, trees)
+    learned, learned_rows = query.clone().requires_grad_(), rows.clone().requires_grad_()
+    with pytest.raises(tsac_cuda.TsacError, match="query requires a gradient"):
+        s.cache.attention(0, learned, trees)
+    with pytest.raises(tsac_cuda.TsacError, match="out requires a gradient"):
+        s.cache.attention(0, query, trees, learned)
+    with pytest.raises(tsac_cuda.TsacError, match="keys requires a gradient"):
+        s.cache.append(0, learned_rows, rows)
+    with pytest.raises(tsac_cuda.TsacError, match="values requires a gradient"):
+        s.cache.append(0, rows, learned_rows)
+    with pytest.raises(tsac_cuda.TsacError, match="pool requires a gradient"):
+        tsac_cuda.PagedCache(s.cache.pool.clone().requires_grad_(), s.cache.tables, s.cache.counts, s.cache.lengths, s.cache.refs)
+    for block in (torch.no_grad, torch.inference_mode):
+        with block():
+            assert torch.equal(s.cache.attention(0, learned, trees), want)
+            s.cache.append(0, learned_rows, learned_rows)

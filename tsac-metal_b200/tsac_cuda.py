@@ -143,6 +143,8 @@ def qlinear(weights, scales, bias, x, y, scratch, residual=None, error_word=None
 # tensors; calls are asynchronous on the current stream of the tensors' device
 # and may be captured into a CUDA graph.  Temporary device memory comes from
 # torch's allocator in each call, so overlapping calls and graphs share none.
+# There is no backward: tensors that require a gradient are refused outside
+# torch.no_grad().
 MAX_NODES = 64
 
 
@@ -248,11 +250,21 @@ def _strides(values):
     return array
 
 
+def _no_gradient(t, name):
+    """These calls have no backward: a gradient that autograd would have to carry through one is refused."""
+    if t.requires_grad:
+        import torch
+        if torch.is_grad_enabled():
+            raise TsacError(f"{name} requires a gradient, which the drafting calls do not carry: call them under torch.no_grad()")
+
+
 def _rows(t, name, dtype, index, shape):
     """Address and strides of a [entry][node][head][dim] tensor with a contiguous last dimension."""
     strides = t.stride()
     if t.dtype is not dtype or t.get_device() != index or t.shape != shape or (strides[-1] != 1 and shape[-1] > 1):
         raise TsacError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on cuda:{index}, its last dimension contiguous")
+    if t.requires_grad:
+        _no_gradient(t, name)
     array = _stride_arrays.get((strides, shape))
     if array is None:
         if len(_stride_arrays) >= 1024:
@@ -276,6 +288,7 @@ class PagedCache:
         import torch
         if pool.dim() != 6 or pool.shape[1] != 2 or not pool.is_cuda or pool.dtype not in (torch.bfloat16, torch.float16):
             raise TsacError("pool must be a bf16 or fp16 CUDA tensor [layers][2][pages][page_size][kv_heads][head_dim]")
+        _no_gradient(pool, "pool")
         self.pool, self.tables, self.counts, self.lengths, self.refs = pool, tables, counts, lengths, refs
         self.device, self.index, self.dtype = pool.device, pool.get_device(), pool.dtype
         self._torch, self._int, self._bytes = torch, torch.int32, torch.empty(0, dtype=torch.uint8, device=self.device)
