@@ -601,3 +601,16 @@ def test_counts_below_the_entries_that_name_a_page():
     cache.refs.copy_(ints([0, 2, -7]))
     cache.release(error_word=errors)
     assert word() == 16 and cache.refs.tolist() == [0, 0, -7] and cache.counts.sum().item() == 0
+
+
+@pytest.mark.parametrize("name", ["pool", "tables", "counts", "lengths", "refs"])
+def test_the_bound_tensors_cannot_be_exchanged(name):
+    """The calls go on with the addresses that the cache was made with."""
+    pair = Pair()
+    pair.grow([(0, 5)])
+    before = getattr(pair.gpu, name)
+    with pytest.raises(tsac_cuda.TsacError, match=f"{name} is bound"):
+        setattr(pair.gpu, name, before.clone())
+    assert getattr(pair.gpu, name) is before
+    pair.gpu.lengths += 0  # in place
+    pair.check()

@@ -280,9 +280,18 @@ class PagedCache:
     pool: [layers][2: keys, values][pages][page_size][kv_heads][head_dim], bf16
     or fp16; tables int32 [sequences][max_pages]; counts, lengths int32
     [sequences]; refs int32 [pages].  The tensors stay the caller's: reading,
-    saving or replacing their contents between calls is fine.  Keep the object
-    as long as a CUDA graph that was captured from its calls.
+    saving or replacing their contents between calls is fine.  The tensors
+    themselves stay the same ones: their addresses are bound here, and a cache
+    over other tensors is a new object.  Keep the object as long as a CUDA graph
+    that was captured from its calls.
     """
+
+    _bound = frozenset(("pool", "tables", "counts", "lengths", "refs"))
+
+    def __setattr__(self, name, value):
+        if name in self._bound and name in self.__dict__ and self.__dict__[name] is not value:
+            raise TsacError(f"{name} is bound to the cache: copy into it, or make a PagedCache over other tensors")
+        object.__setattr__(self, name, value)
 
     def __init__(self, pool, tables, counts, lengths, refs):
         import torch
