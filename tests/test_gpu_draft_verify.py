@@ -230,3 +230,18 @@ def test_draws_outside_the_interval_give_a_token(with_draft, vocab, draw):
                            1.0 if draw >= 1 else 0.0, None if draft is None else draft[1].double().numpy(), 4)
     assert out[1][1].tolist() == want[0] + [-1] * (4 - len(want[0])) and out[2][1].item() == want[1]
     assert target[1, want[0][-1], want[1]] > 0
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("vocab", [50, 20000])
+def test_infinite_draft_probabilities_at_a_rejection(kind, vocab):
+    """An infinite q takes its token's excess to nothing and leaves the others'; one that is drafted is rejected."""
+    target, tokens, parents, coins, draws, draft = case(4, 2, vocab, kind, True, 5, chain=True)
+    coins[:, 1] = 0.75
+    for b in (1, 2):
+        target[b, 0, int(tokens[b, 1])] = 0.0  # rejected
+    likely = int(torch.argmax(target[1, 0].float() - draft[1, 0].float()))
+    draft[1, 0, likely] = float("inf")
+    draft[3, 0, int(tokens[3, 1])] = float("inf")
+    accepted, _, token = check(target, tokens, parents, coins, draws, draft)
+    assert accepted[1:] == [1, 1, 1] and token[1] != likely and token[3] != int(tokens[3, 1])
