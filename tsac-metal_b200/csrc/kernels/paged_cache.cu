@@ -369,17 +369,15 @@ __global__ void __launch_bounds__(256)
     pdl_prologue();
     const int i = blockIdx.x;
     const int parent = cache_sequence(c, parents, i), child = cache_sequence(c, children, i);
+    const bool named = parent >= 0 && child >= 0;
+    // Read before the list is: one round trip for both.
+    const int length = named ? c.lengths[parent] : 0, held = named ? cache_held(c, parent) : 0;
+    const bool empty = named && c.counts[child] == 0;
     bool clash = false;
     for (int k = threadIdx.x; k < count; k += 256)
         clash |= (k < i && children[k] == child) || children[k] == parent;
-    bool bad = parent < 0 || child < 0 || __syncthreads_or(clash);
-    int share = 0, length = 0;
-    if (!bad)
-    {
-        length = c.lengths[parent];
-        share = length > 0 ? (length - 1 >> c.page_shift) + 1 : 0;
-        bad = length < 0 || share > cache_held(c, parent) || c.counts[child] != 0;
-    }
+    const int share = length > 0 ? (length - 1 >> c.page_shift) + 1 : 0;
+    bool bad = __syncthreads_or(clash) || !empty || length < 0 || share > held;
     if (!bad)
     {
         bool broken = false;
@@ -672,9 +670,15 @@ __global__ void __launch_bounds__(PLAN_THREADS)
     __shared__ int warp_sums[32];
     const int t = threadIdx.x;
     int mine = 0, live;
+    bool negative = false;
 #pragma unroll 4
     for (int page = t; page < c.pages; page += PLAN_THREADS)
+    {
         mine += c.refs[page] > 0;
+        negative |= c.refs[page] < 0;
+    }
+    if (negative)
+        raise(error_word, error_cache);
     block_exclusive(mine, warp_sums, live);
     const int moves = select_pages(c.refs, live, c.pages, c.pages, s.selected, warp_sums, [](int refs) { return refs > 0; });
     select_pages(c.refs, 0, live, c.pages, s.selected + c.pages, warp_sums, [](int refs) { return refs <= 0; });
@@ -682,8 +686,6 @@ __global__ void __launch_bounds__(PLAN_THREADS)
     {
         const int refs = c.refs[page];
         s.map[page] = refs > 0 ? page : -1;
-        if (refs < 0)
-            raise(error_word, error_cache);
         refs_out[page] = refs > 0 ? refs : 0;
     }
     __syncthreads();
