@@ -535,9 +535,12 @@ int tsac_cuda_cache_compact(const tsac_cuda_paged_cache* cache, int32_t* tables_
 /* Attention of every node of each listed sequence's tree over the committed
  * positions and the node's own ancestors, itself included, whose keys and
  * values lie at positions length + ancestor:
- *   out = softmax(scale * q k^T) v over those positions, 32-bit softmax and sums.
+ *   out = softmax(scale * q k^T) v over those positions, scores, softmax and sums
+ * in 32 bits; the weights are rounded to the cache's type for their product with
+ * v, half a step relative to each (fp16: as long as one is above 2^-24 of the
+ * row's largest, and none is lost above 2^-35).
  *   parents  device int32 [count][max_nodes]; -1: a root; below -1: the node
- *            sees no drafted node, not even itself
+ *            sees no drafted node, not even itself, nor do its descendants see it
  *   nodes    device int32 [count] or NULL: max_nodes each.  Rows of later
  *            nodes, and of sequences without nodes, are left as they were
  *   query, out  device [count][max_nodes][heads][head_dim] of the cache's type
@@ -545,14 +548,16 @@ int tsac_cuda_cache_compact(const tsac_cuda_paged_cache* cache, int32_t* tables_
  *            dimension is contiguous), 16-byte aligned.  heads is a multiple
  *            of kv_heads: query head h reads key head h / (heads / kv_heads).
  *            out may be query itself (the same strides), but not overlap it
- *            otherwise; its rows must not overlap one another
+ *            otherwise; its rows must not overlap one another: each stride steps
+ *            over all that dimensions of smaller strides span
  *   lse      device f32 [count][max_nodes][heads] or NULL: log of the sum of
  *            exponentials
  *   scratch  device, >= tsac_cuda_tree_attention_scratch_bytes(cache, heads,
  *            max_nodes), asked for with the cache's device current, 16-byte
  *            aligned; calls that overlap need their own
- * A row that sees nothing gives zeros and -infinity.  A value that is not
- * finite reaches the rows that see it and no others.  An entry whose length
+ * A row that sees nothing, or nothing but scores of -infinity, gives zeros and
+ * -infinity.  A value that is not finite reaches the rows that see it and no
+ * others.  An entry whose length
  * and nodes exceed its pages is skipped (bit 16); a table entry that is no page
  * of the pool is reported likewise and read as zeros.  The same sequence may be
  * listed more than once.  The order of the sums depends on all lengths and

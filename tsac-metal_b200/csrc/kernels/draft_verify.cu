@@ -25,8 +25,10 @@
 //
 // All sums and the excess are in 64 bits: the token is an integer that one
 // rounding near a border would change, and 32-bit partial sums over 10^5
-// probabilities are off by up to 10^5 * 2^-24.  The conversions and additions
-// take a few percent of the time the loads take.
+// probabilities are off by up to 10^5 * 2^-24.  They are not what bounds a
+// call: with 32-bit sums 160 rows of 131,072 fp32 values took 27.7 us in place
+// of 28.2, 148 rows, one per SM, 24.9 in place of 25.1 (48 rows of 50,001 bf16
+// values with a draft, short as they are, 11.4 in place of 12.8).
 #include "kernels/draft_verify.cuh"
 #include "kernels/error_bits.hpp"
 #include "kernels/launch_count.hpp"

@@ -30,12 +30,17 @@ struct TreeArgs
 
 // The work is measured in units: one key tile of one item, an item being the
 // query rows [first, first + ROWS) (node-major, then query head of the group)
-// of one list entry and key head.  The committed positions of a sequence make
-// ceil(length / KEYS) tiles and its drafted nodes one tile of their own, so
-// only that last tile needs the tree's mask.  CTA c of the first g = min(grid, U)
-// takes the units [U c / g, U (c + 1) / g): equal shares, none of them empty,
-// whatever the lengths, with at most two items of each CTA shared with its
-// neighbours.
+// of one list entry and key head.  An item's last tile begins at last_base and
+// holds the last committed keys and, behind them, all drafted nodes: last_base
+// is the last multiple of KEYS where they fit, else of 64.  Before it lie
+// ceil(last_base / KEYS) tiles, the last of them half full in that second case.
+// So only the last tile needs the tree's mask, and a half-full one before it a
+// limit.  Each item counts START units more than its tiles, in front of them:
+// what it costs to begin and end one, in tiles (measured).  CTA c of the first
+// g = min(grid, U) takes the units [U c / g, U (c + 1) / g): equal shares, none
+// of them empty, whatever the lengths, with at most two items of each CTA shared
+// with its neighbours.  A share that ends before an item's first tile leaves the
+// item to the next CTA.
 template <int KEYS, int ROWS, int START> struct TreeWork
 {
     static constexpr int keys_per_tile = KEYS, rows_per_item = ROWS;

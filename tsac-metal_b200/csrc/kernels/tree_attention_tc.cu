@@ -22,10 +22,11 @@
 //                   exponentials overlap the other's products.
 //   warps 9, 10     producers, half of each key or value tile each, into a ring
 //                   of shared-memory slots in the 128-byte swizzle that the MMA
-//                   reads, by TMA: one box per page (or 64 rows), a lane each.  Value tiles with rows behind the last position
-//                   come by 16-byte asynchronous copies that make those rows
-//                   zeros, as does everything where TMA does not serve: pages of
-//                   fewer than 8 rows (a swizzle atom), or 2^31 rows in a plane.
+//                   reads, by TMA: one box per page (or 64 rows), a lane each.
+//                   Value tiles with rows behind the last position come by
+//                   16-byte asynchronous copies that make those rows zeros, as
+//                   does everything where TMA does not serve: pages of fewer
+//                   than 8 rows (a swizzle atom), or 2^31 rows in a plane.
 //                   Copies of every tile by the two warps bound the kernel by
 //                   their address arithmetic (290 against 209 us for 64 x 16
 //                   nodes over up to 4,096 positions).
@@ -45,11 +46,15 @@
 // pipes gained nothing over the special function units' 16 per clock.
 //
 // What bounds it now.  128 rows: the loads (64 x 16 nodes 154 us, the same with
-// products and softmax left out).  256 rows: power.  2 x 64 nodes over 131,072
-// positions take 238 us, at 1.6 GHz under the 1,000 W limit, where loads alone
-// take 160, products and loads 168 to 193, softmax and loads 184 to 200; issuing
-// a group's next scores without waiting for its product, or handing P on in two
-// parts, gained 7 to 16 us in those and nothing in the whole.
+// products and softmax left out).  256 rows: products and exponentials, which
+// overlap little.  A tile needs 2,048 clocks of each (32 MMAs of 128 x 128 x 16
+// at 64, 32,768 exponentials at 16 per clock); 2 x 64 nodes over up to 131,072
+// positions, 94 tiles per SM, take 4,500 (253 us at 1.68 GHz) to 4,900 clocks a
+// tile (293 us at 1.56 GHz, after seconds at the 1,000 W limit, which sets the
+// clock).  Loads alone take 160 us, products and loads 168 to 193, softmax and
+// loads 184 to 200; issuing a group's next scores without waiting for its
+// product, or handing P on in two parts, gained 7 to 16 us in those and nothing
+// in the whole.
 //
 // Every wait is bounded (tc_common.cuh).  One that gives up raises
 // error_timeout and the CTA's abort flag; softmax threads then run through

@@ -141,8 +141,10 @@ def qlinear(weights, scales, bias, x, y, scratch, residual=None, error_word=None
 # Paged key/value cache, tree attention and draft verification
 # (include/tsac_cuda.h states each operation).  Arguments are torch CUDA
 # tensors; calls are asynchronous on the current stream of the tensors' device
-# and may be captured into a CUDA graph.  Temporary device memory comes from
-# torch's allocator in each call, so overlapping calls and graphs share none.
+# and may be captured into a CUDA graph.  Attention takes its temporary device
+# memory from torch's allocator in each call, so that overlapping calls and
+# graphs share none; reserve and compact, which must not overlap on one cache,
+# keep theirs with it.
 # There is no backward: tensors that require a gradient are refused outside
 # torch.no_grad().
 MAX_NODES = 64
