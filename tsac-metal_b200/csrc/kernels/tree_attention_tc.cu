@@ -769,7 +769,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 
             // A warp without a live row has nothing to compute: whatever its lanes of TMEM hold stays there.
             const bool busy = __any_sync(0xffffffffu, live);
-            float reference = -INFINITY, sum = 0.0f;
+            // Scores above `threshold` move the reference; -infinity: every tile takes that way.
+            float reference = -INFINITY, threshold = -INFINITY, sum = 0.0f;
             for (int j = TWO ? 0 : group; j < tiles; j += TWO ? 1 : 2)
             {
                 const int tile = g.tile_begin + j;
@@ -798,12 +799,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                             best[k >> 1 & 3] = max3(best[k >> 1 & 3], __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
                         const float highest = max3(best[0], best[1], fmaxf(best[2], best[3]));
                         const float top = highest == -INFINITY ? -INFINITY : highest * scale;
-                        // From 2^23 on (and below infinity) a product's rounding moves a weight by powers of two: the
-                        // scores are then rounded like the maximum that the reference comes from.
-                        const bool coarse = (__float_as_uint(top) & 0x7fffffffu) - 0x4b000000u < 0x34800000u;
                         float factor = scale;
-                        if (__any_sync(0xffffffffu, coarse || top > reference + LIMIT))
+                        if (__any_sync(0xffffffffu, top > threshold))
                         {
+                            // From 2^23 on (and below infinity) a product's rounding moves a weight by powers of
+                            // two: the scores are then rounded like the maximum that the reference comes from.
+                            const bool coarse = fabsf(top) >= 0x1p23f && fabsf(top) < INFINITY;
                             if (__any_sync(0xffffffffu, coarse))
                             {
                                 const float early = coarse ? scale : 1.0f;
@@ -815,6 +816,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                             const float raised = fmaxf(reference, __fadd_ru(ceilf(top), -PLACE));
                             const float shrink = reference == -INFINITY ? 0.0f : power_of_two(reference - raised);
                             reference = raised;
+                            threshold = fabsf(raised) >= 0x1p22f && fabsf(raised) < INFINITY ? -INFINITY : raised + LIMIT;
                             sum *= shrink;
                             part = mul_pair(part, make_pair(shrink, shrink));
                             // P of this tile's earlier scores, then the output; its last product is
