@@ -210,13 +210,15 @@ class _Device:
         return self._stream(self.index)
 
     def ask(self, fn, *arguments) -> int:
-        if self._current() == self.index:
-            return fn(*arguments)
+        """What fn answers with the device current."""
         with self._cuda.device(self.index):
             return fn(*arguments)
 
     def call(self, fn, *arguments) -> None:
-        status = self.ask(fn, *arguments)
+        if self._current() == self.index:
+            status = fn(*arguments)
+        else:
+            status = self.ask(fn, *arguments)
         if status != OK:
             check(status)
 
@@ -260,10 +262,10 @@ def _no_gradient(t, name):
             raise TsacError(f"{name} requires a gradient, which the drafting calls do not carry: call them under torch.no_grad()")
 
 
-def _rows(t, name, dtype, index, shape):
-    """Address and strides of a [entry][node][head][dim] tensor with a contiguous last dimension."""
+def _rows(t, name, dtype, index, shape, found=None):
+    """Address and strides of a [entry][node][head][dim] tensor with a contiguous last dimension; found: its shape, where known."""
     strides = t.stride()
-    if t.dtype is not dtype or t.get_device() != index or t.shape != shape or (strides[-1] != 1 and shape[-1] > 1):
+    if t.dtype is not dtype or t.get_device() != index or (found or t.shape) != shape or (strides[-1] != 1 and shape[-1] > 1):
         raise TsacError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on cuda:{index}, its last dimension contiguous")
     if t.requires_grad:
         _no_gradient(t, name)
@@ -291,7 +293,8 @@ class PagedCache:
     _bound = frozenset(("pool", "tables", "counts", "lengths", "refs"))
 
     def __setattr__(self, name, value):
-        if name in self._bound and name in self.__dict__ and self.__dict__[name] is not value:
+        # (Not by __dict__: asking for it would make every later attribute of the object slower.)
+        if name in self._bound and getattr(self, name, value) is not value:
             raise TsacError(f"{name} is bound to the cache: copy into it, or make a PagedCache over other tensors")
         object.__setattr__(self, name, value)
 
@@ -383,11 +386,12 @@ class PagedCache:
 
     def append(self, layer, keys, values, nodes=None, sequences=None, starts=None, error_word=None):
         """Stores [entry][node][kv_heads][head_dim] rows of one layer behind each sequence's length (or at starts)."""
-        if keys.dim() != 4:
+        found = keys.shape
+        if len(found) != 4:
             raise TsacError("keys must be [entry][node][kv_heads][head_dim]")
-        count, most, _, _ = keys.shape
+        count, most, _, _ = found
         shape, index, ints = (count, most, self.kv_heads, self.head_dim), self.index, self._int
-        k, key_strides = _rows(keys, "keys", self.dtype, index, shape)
+        k, key_strides = _rows(keys, "keys", self.dtype, index, shape, found)
         v, value_strides = _rows(values, "values", self.dtype, index, shape)
         self._on.call(self._lib.tsac_cuda_cache_append, self._cache, layer, k, key_strides, v, value_strides,
                       sequences if sequences is None else _whole(sequences, "sequences", ints, index, (count,)),
@@ -423,12 +427,13 @@ class PagedCache:
     def attention(self, layer, query, parents, out=None, nodes=None, sequences=None, scale=None, lse=None,
                   error_word=None):
         """Attention of each tree's nodes over the cache: query [entry][node][heads][head_dim] -> out."""
-        if query.dim() != 4:
+        found = query.shape
+        if len(found) != 4:
             raise TsacError("query must be [entry][node][heads][head_dim]")
-        count, most, heads, _ = query.shape
+        count, most, heads, _ = found
         shape, index, ints, on = (count, most, heads, self.head_dim), self.index, self._int, self._on
         out = query.new_empty(shape) if out is None else out
-        q, query_strides = _rows(query, "query", self.dtype, index, shape)
+        q, query_strides = _rows(query, "query", self.dtype, index, shape, found)
         o, out_strides = _rows(out, "out", self.dtype, index, shape)
         nbytes = self._attention_bytes.get((heads, most))
         if nbytes is None:
