@@ -40,10 +40,11 @@
 // as 1.  For fp16 it is 11 below the maximum with a slack of 4: p stays below
 // 2^15 and the row's largest is 2^10 at least, so that a p keeps all its bits
 // down to 2^-24 of it and is nothing from 2^-35 on.  (A slack of 2 costs
-// rescaling: 2 x 64 nodes over 131,072 positions 267 us, 253 with 4 and with 8.)  The loop over a tile's scores is kept
-// small: unrolled over the whole tile it delayed the MMA warp (64 x 16 nodes 172
-// against 162 us), and exponentials of some pairs by a polynomial on the FMA
-// pipes gained nothing over the special function units' 16 per clock.
+// rescaling: 2 x 64 nodes over 131,072 positions 267 us, 253 with 4 and with 8.)
+// The loop over a tile's scores is kept small: unrolled over the whole tile it
+// delayed the MMA warp (64 x 16 nodes 172 against 162 us), and exponentials of
+// some pairs by a polynomial on the FMA pipes gained nothing over the special
+// function units' 16 per clock.
 //
 // What bounds it now.  128 rows: the loads (64 x 16 nodes 154 us, the same with
 // products and softmax left out).  256 rows: products and exponentials, which
